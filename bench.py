@@ -21,6 +21,7 @@ Prints ONE JSON line on rank 0, including
 import argparse
 import json
 import os
+import subprocess
 import sys
 import time
 
@@ -251,7 +252,6 @@ def main():
         # `python bench.py --gpus N` without a launcher: re-launch this script as N ranks (one process per GPU) under
         # torch.distributed.run on this node and pass the ranks' output through (rank 0 prints the JSON line).
         import socket
-        import subprocess
         with socket.socket() as sk:
             sk.bind(("127.0.0.1", 0))
             port = sk.getsockname()[1]
@@ -310,11 +310,12 @@ def main():
         except Exception as e:
             # A capture that was invalidated leaves the HIP runtime and torch's generator in a sticky error state (probed:
             # tools/parity/capture_failure_probe.py -- every later launch in the process fails), so "stay on the eager path" has
-            # to mean a fresh process: re-run this command with --no-graph (one GPU; a rank of a multi-process job cannot).
+            # to mean a fresh process: re-run this command with --no-graph (one GPU; a rank of a multi-process job cannot), as a child whose
+            # exit code becomes this process's (a process that holds the GPU is not replaced; its own teardown is skipped, the runtime being unusable).
             print(f"[bench] graph capture unavailable ({type(e).__name__}: {str(e)[:200]}); re-running eagerly (--no-graph)", file=sys.stderr, flush=True)
             if world > 1:
                 raise
-            os.execv(sys.executable, [sys.executable, os.path.abspath(__file__)] + sys.argv[1:] + ["--no-graph"])
+            os._exit(subprocess.call([sys.executable, os.path.abspath(__file__)] + sys.argv[1:] + ["--no-graph"]))
     # n iterations per replay: the ~0.3 ms a graph launch costs on top of its kernels is paid once per n iterations (GanTrainer.capture_multi)
     n_multi = args.graph_iters if (graphed and world == 1 and args.graph_iters > 1) else 1
     if n_multi > 1:
@@ -323,7 +324,7 @@ def main():
                 n_multi = 1
         except Exception as e:   # (sticky, as above: a fresh process with one iteration per replay)
             print(f"[bench] multi-iteration capture unavailable ({type(e).__name__}: {str(e)[:200]}); re-running with --graph-iters 1", file=sys.stderr, flush=True)
-            os.execv(sys.executable, [sys.executable, os.path.abspath(__file__)] + sys.argv[1:] + ["--graph-iters", "1"])
+            os._exit(subprocess.call([sys.executable, os.path.abspath(__file__)] + sys.argv[1:] + ["--graph-iters", "1"]))
     step = (lambda: trainer.step_graphed(real, label, bbox, None)) if graphed else (lambda: trainer.step(real, label, bbox, None, None))
     multi = [(real, label, bbox, None)] * n_multi
 
