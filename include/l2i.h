@@ -473,6 +473,57 @@ int l2i_in_relu_up2_bwd(const float* x, const float* g, float* dx, void* dx_op, 
 int l2i_up2_nhwc_fwd(const float* x, float* out, void* out_op, int op_dtype, long long N, int S, int C, void* stream);
 int l2i_up2_nhwc_bwd(const float* g, float* dx, void* dx_op, int op_dtype, long long N, int S, int C, void* stream);
 
+/* ---- attention conditioning: operators beside the normalisation, attention, label-embedding and dropout launches above, for generators whose maps
+ * look at their layout (or another sequence) by attention. x_dtype / y_dtype / ...: 0 = f32, 1 = bf16, each on its own. The `_scratch` functions
+ * give the f32 scratch (16-byte aligned, contents undefined before and after, not shared by launches that may run at the same time) that a call
+ * of these sizes needs; 0: NULL is fine. */
+
+/* Group normalisation of NHWC maps x [B][HW][C] over G groups of C / G consecutive channels, then act 0: none, 1: ReLU, 2: SiLU
+ * (the per-image counterpart of the batch statistics of model/norm_module.py:163-186): y = act((x - mean) rstd gamma + beta), biased variance.
+ * gamma, beta [C] f32 or NULL (1, 0); mean, rstd [B][G] are kept for bwd. C <= 4096.
+ * bwd: dx (x's type) and dgamma, dbeta [C] (written), each optional; dy has y's type. */
+int l2i_group_norm_scratch(int B, long long HW, int C, int G, int bwd, long long* floats);
+int l2i_group_norm_fwd(const void* x, int x_dtype, const float* gamma, const float* beta, void* y, int y_dtype, float* mean, float* rstd, int B,
+                       long long HW, int C, int G, float eps, int act, float* scratch, long long scratch_floats, void* stream);
+int l2i_group_norm_bwd(const void* x, int x_dtype, const float* gamma, const float* beta, const float* mean, const float* rstd, const void* dy,
+                       int y_dtype, void* dx, float* dgamma, float* dbeta, int B, long long HW, int C, int G, int act, float* scratch,
+                       long long scratch_floats, void* stream);
+
+/* Attention of queries [B][Lq][Hk G][D] to states [B][Lk][Hk][D] of another length (what l2i_box_attention_* is for a layout's objects among
+ * themselves, model/resnet_generator_app_v2.py:79-120): query head h reads state head h / G; D a multiple of 8 up to 128; one type for all.
+ * q, k, v: element strides of batch, position and head (any, 0 among them, in whole 16 bytes; the D values are consecutive; 16-byte aligned).
+ * lengths [B] int32 or NULL: keys at and behind it are not read. mask: bytes, address b mb + i mq + j, 0 = key j is masked for query i, or NULL;
+ * mq = 0: one row for all queries, whose masked keys are not read either. A pair that is masked for some queries only weighs zero: its values
+ * have to be finite. A query without a live key gives zeros (and no gradient).
+ * out [B][Lq][Hk G][D] contiguous; lse [B][Hk][Lq G] (optional in fwd) is kept for bwd.
+ * bwd: out, dout, dq [B][Lq][Hk G][D] and dk, dv [B][Lk][Hk][D] contiguous and 16-byte aligned; dq, and dk with dv, optional. */
+int l2i_cross_attention_scratch(int B, int Lq, int Lk, int Hk, int G, int D, int bwd, long long* floats);
+int l2i_cross_attention_fwd(const void* q, const void* k, const void* v, int dtype, const int* lengths, const unsigned char* mask, void* out,
+                            float* lse, int B, int Lq, int Lk, int Hk, int G, int D, long long qb, long long ql, long long qh, long long kb,
+                            long long kl, long long kh, long long vb, long long vl, long long vh, long long mb, long long mq, float scale,
+                            float* scratch, long long scratch_floats, void* stream);
+int l2i_cross_attention_bwd(const void* q, const void* k, const void* v, int dtype, const int* lengths, const unsigned char* mask,
+                            const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, int B, int Lq, int Lk, int Hk,
+                            int G, int D, long long qb, long long ql, long long qh, long long kb, long long kl, long long kh, long long vb,
+                            long long vl, long long vh, long long mb, long long mq, float scale, float* scratch, long long scratch_floats,
+                            void* stream);
+
+/* out[i] = scale * weight[tokens[i]] (rows of D; the lookup of model/resnet_generator_app_v2.py:437 for tables and batches of any size);
+ * a token outside [0, V) or equal to padding_idx (-1: none) gives zeros.
+ * bwd: dw [V][D] (written, every row) = scale * sum of the dy rows of each token, in f32, in the order of their positions. */
+int l2i_embedding_fwd(const void* weight, int w_dtype, const long long* tokens, void* out, int out_dtype, long long n, int V, int D,
+                      float scale, int padding_idx, void* stream);
+int l2i_embedding_bwd_scratch(long long n, int D, long long* floats);
+int l2i_embedding_bwd(const long long* tokens, const void* dy, int dy_dtype, void* dw, int dw_dtype, long long n, int V, int D, float scale,
+                      int padding_idx, float* scratch, long long scratch_floats, void* stream);
+
+/* out[i] = (word_i >= threshold ? in[i] * scale : 0) + res[i] (res: optional, out's type): elementwise dropout with drop probability
+ * threshold / 2^32 (the elementwise counterpart of l2i_channel_dropout, model/resnet_generator_app_v2.py:739). word_i = word i % 4 of
+ * Philox4x32-10 with key rng[0] and counter (i / 4, layer, rng[1]); rng [2] int64 on the device: seed, offset. used (optional) [2] receives the
+ * pair this launch read: its own backward is the same call with in = dy, rng = used. n <= 2^34, layer >= 0. */
+int l2i_dropout(const void* in, int in_dtype, const void* res, void* out, int out_dtype, const long long* rng, long long* used, long long n,
+                long long threshold, float scale, int layer, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

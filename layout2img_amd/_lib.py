@@ -83,6 +83,18 @@ SIGNATURES = {
     "l2i_image_nhwc_bwd": [_p, _p, _p, _ll, _i, _i, _i, _i, _p],
     "l2i_resize_bilinear_bwd": [_p, _p, _ll, _i, _i, _i, _i, _p],
     "l2i_channel_dropout": [_p, _p, _p, _ll, _i, _i, _f, _p],
+    "l2i_group_norm_scratch": [_i, _ll, _i, _i, _i, _p],
+    "l2i_group_norm_fwd": [_p, _i, _p, _p, _p, _i, _p, _p, _i, _ll, _i, _i, _f, _i, _p, _ll, _p],
+    "l2i_group_norm_bwd": [_p, _i, _p, _p, _p, _p, _p, _i, _p, _p, _p, _i, _ll, _i, _i, _i, _p, _ll, _p],
+    "l2i_cross_attention_scratch": [_i, _i, _i, _i, _i, _i, _i, _p],
+    "l2i_cross_attention_fwd": [_p, _p, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _f,
+                                _p, _ll, _p],
+    "l2i_cross_attention_bwd": [_p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll,
+                                _ll, _ll, _f, _p, _ll, _p],
+    "l2i_embedding_fwd": [_p, _i, _p, _p, _i, _ll, _i, _i, _f, _i, _p],
+    "l2i_embedding_bwd_scratch": [_ll, _i, _p],
+    "l2i_embedding_bwd": [_p, _p, _i, _p, _i, _ll, _i, _i, _f, _i, _p, _ll, _p],
+    "l2i_dropout": [_p, _i, _p, _p, _i, _p, _p, _ll, _ll, _f, _i, _p],
     "l2i_psp_stages_fwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _i, _f, _f, _p],
     "l2i_psp_stages_bwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _i, _p],
 }

@@ -9,7 +9,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libl2i_hip.so")
-SOURCES = ["conv_igemm.hip", "conv_wgrad.hip", "weights.hip", "norm.hip", "roi_align.hip", "attention.hip", "misc.hip", "psp.hip", "layout.hip"]
+SOURCES = ["conv_igemm.hip", "conv_wgrad.hip", "weights.hip", "norm.hip", "roi_align.hip", "attention.hip", "misc.hip", "psp.hip", "layout.hip",
+           "groupnorm.hip", "cross_attention.hip", "embedding.hip", "dropout.hip"]
 # (packed f32 instructions are off in device code: some of their forms have given wrong results on MI355X now and then, with no error; the host
 #  pass warns that it does not know the feature)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wno-unused-result",

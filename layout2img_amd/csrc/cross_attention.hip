@@ -1,0 +1,720 @@
+// Attention of a map's (or a sequence's) queries to the states of another sequence, forward and backward.
+//
+//   S_ij = scale q_i . k_j over the live keys j of query i;  P = softmax_j(S);  out_i = sum_j P_ij v_j   (no live key: out_i = 0)
+//   backward, g = dL/dout:  D_i = g_i . out_i;  dS_ij = P_ij (g_i . v_j - D_i);
+//   dq_i = scale sum_j dS_ij k_j;  dk_j = scale sum_i dS_ij q_i;  dv_j = sum_i P_ij g_i
+// A key is live when it lies below its image's length and its mask byte is not zero. Hq = Hk G query heads: head h reads state head h / G;
+// the G heads of a group are G further ROWS of the same problem (row r = (query r / G, head r % G)), so that a tile of states is read
+// once for the whole group and dk / dv sum over the group without a further pass.
+//
+// Products run on MFMA 32x32 tiles (bf16: 32x32x16; f32: 32x32x2, exact), one pass over the states with the running maximum and sum of the
+// softmax. S is computed transposed (keys along the accumulator's rows, queries along its lanes): a lane then owns one query, the maximum
+// and sum are in-lane plus one exchange between the wave's halves, and the accumulator's registers ARE the B operand of P V with no
+// movement, because the sum over keys may run in any order as long as V is read in the same one: bf16 V^T comes from LDS by
+// the transposing read (ds_read_b64_tr_b16), f32 V by plain reads. Probabilities enter P V (and dS the gradient products) rounded to bf16 in
+// the bf16 kernels (relative 2^-9, as small as the rounding of the inputs); maxima, sums, S, D and all accumulators are f32.
+#include "common.h"
+#include <type_traits>
+
+typedef __attribute__((ext_vector_type(8))) __bf16 b16x8_t;
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+
+struct XaArgs {
+    const void *q, *k, *v; void* o;          // o, g, dq: [B][Lq][H][D]; dk, dv: [B][Lk][Hk][D]
+    const void* g; void *dq, *dk, *dv;
+    float* lse;                               // [B Hk][R] log2 of the softmax's denominator; +inf for a row without a live key
+    float* delta;                             // [B Hk][R] D
+    float* part; float* ml;                   // splits: [ns][B Hk][R][D] sums, [ns][B Hk][R] (max, sum); backward [2][ns][B Hk][Lk][D]
+    const int* len; const unsigned char* mask;
+    long long qb, ql, qh, kb, kl, kh, vb, vl, vh, mb, mq;   // strides in elements (mask: bytes; mq = 0: one mask row for all queries)
+    int B, Lq, Lk, Hk, G, D, R, ns;
+    float scale, c;                           // c = scale log2(e)
+};
+
+// ---- LDS tiles: rows of CH 16-byte chunks, chunk c of row r at place c ^ f(r): 16 rows at one chunk (row reads) and 4 rows x 4 chunks
+// (transposing reads) each fall on 16 different 16-byte bank groups
+template <int CH> __device__ __forceinline__ int xa_at(int row, int chunk) {
+    int f;
+    if constexpr (CH == 4) f = (row >> 2) & 3;
+    else if constexpr (CH == 8) f = (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    else f = ((row & 3) << 2) | ((row >> 2) & 3);
+    return (row * CH + (chunk ^ f)) * 16;
+}
+
+// ---- acc[a's row][b's row] += a . b over one step of dims (bf16: 16, f32: 8): a, b = the lane's 16-byte chunk 2 s + lane / 32 of its row
+__device__ __forceinline__ void xa_dot(f32x16_t& acc, const uint4& a, const uint4& b, bf16_t) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8_t, a), __builtin_bit_cast(b16x8_t, b), acc, 0, 0, 0);
+}
+__device__ __forceinline__ void xa_dot(f32x16_t& acc, const uint4& a, const uint4& b, float) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), acc, 0, 0, 0);
+}
+
+// ---- acc[d][lane] += sum over 32 tile rows i of tile[row0 + i][d] p_i(lane); p: an accumulator (register r of a lane = row 8 (r / 4) + 4 (lane / 32) + r % 4)
+template <int CH, int ND>
+__device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, int row0, const f32x16_t& p, bf16_t) {
+    const int lane = threadIdx.x & 63, h = lane >> 5, i = lane & 15, d16 = (lane >> 4) & 1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        uint4 pb;
+        pb.x = f2bf2(p[8 * t], p[8 * t + 1]); pb.y = f2bf2(p[8 * t + 2], p[8 * t + 3]);
+        pb.z = f2bf2(p[8 * t + 4], p[8 * t + 5]); pb.w = f2bf2(p[8 * t + 6], p[8 * t + 7]);
+        const int ra = row0 + 16 * t + 4 * h + (i >> 2);
+#pragma unroll
+        for (int db = 0; db < ND; ++db) {
+            const int chunk = db * 4 + d16 * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
+            typedef __attribute__((address_space(3))) s16x4_t lds4_t;
+            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t*)(tile + xa_at<CH>(ra, chunk) + sub));
+            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t*)(tile + xa_at<CH>(ra + 8, chunk) + sub));
+            bf16x8_t a;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { a[e] = lo[e]; a[4 + e] = hi[e]; }
+            acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8_t, a), __builtin_bit_cast(b16x8_t, pb), acc[db], 0, 0, 0);
+        }
+    }
+}
+template <int CH, int ND>
+__device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, int row0, const f32x16_t& p, float) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int row = row0 + 8 * (r >> 2) + 4 * h + (r & 3);
+#pragma unroll
+        for (int db = 0; db < ND; ++db) {
+            const int col = db * 32 + (lane & 31);
+            const float a = *reinterpret_cast<const float*>(tile + xa_at<CH>(row, col >> 2) + (col & 3) * 4);
+            acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[db], 0, 0, 0);
+        }
+    }
+}
+
+// workgroups go to the eight XCDs in turn: give each XCD a contiguous range of tiles, so that the tiles which read the same states share its L2
+__device__ __forceinline__ int xa_tile_id(int n) {
+    const int per = (n + 7) >> 3;
+    return (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+}
+__device__ __forceinline__ int xa_row_query(const XaArgs& p, int r) { return p.G == 1 ? r : (int)((unsigned)r / (unsigned)p.G); }
+__device__ __forceinline__ int xa_len(const XaArgs& p, int b) {
+    if (!p.len) return p.Lk;
+    const int n = p.len[b];
+    return n < 0 ? 0 : (n < p.Lk ? n : p.Lk);
+}
+
+// a tile of NR rows x CH chunks on its way to LDS through registers; row(i) -> pointer to the row's first element or null (zeros)
+template <typename T, int CH, int NR> struct XaStage {
+    static constexpr int N = NR * CH / 256;
+    uint4 r[N];
+    template <typename F> __device__ __forceinline__ void load(int D, F row) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int idx = threadIdx.x + 256 * i, chunk = idx % CH;
+            const T* src = row(idx / CH);
+            r[i] = make_uint4(0, 0, 0, 0);
+            if (src && chunk * (16 / (int)sizeof(T)) < D) r[i] = *reinterpret_cast<const uint4*>(src + chunk * (16 / (int)sizeof(T)));
+        }
+    }
+    __device__ __forceinline__ void store(char* tile) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int idx = threadIdx.x + 256 * i;
+            *reinterpret_cast<uint4*>(tile + xa_at<CH>(idx / CH, idx % CH)) = r[i];
+        }
+    }
+};
+// the lane's chunks of a row as a product operand
+template <typename T, int CH> __device__ __forceinline__ void xa_row_frag(uint4 (&f)[CH / 2], const T* src, int D) {
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int s = 0; s < CH / 2; ++s) {
+        const int e = (2 * s + h) * (16 / (int)sizeof(T));
+        f[s] = make_uint4(0, 0, 0, 0);
+        if (src && e < D) f[s] = *reinterpret_cast<const uint4*>(src + e);
+    }
+}
+// live bits of four consecutive keys j .. j + 3 of a mask row of Lk bytes (none is read outside the row)
+__device__ __forceinline__ unsigned xa_mask4(const unsigned char* row, int j, int Lk) {
+    unsigned w = 0;
+    if (Lk >= 4) {
+        const int jj = min(j, Lk - 4), sh = min(8 * (j - jj), 31);   // (bytes behind the row's end fall out of the word; j - jj > 3: nothing is left that counts)
+        __builtin_memcpy(&w, row + jj, 4);
+        w = j - jj > 3 ? 0u : w >> sh;
+    } else {
+        for (int e = 0; e < 3; ++e) if (j + e < Lk && row[j + e]) w |= 1u << (8 * e);
+    }
+    w = ((((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w) >> 7) & 0x01010101u;   // one bit a byte: byte != 0
+    return (w * 0x01020408u) >> 24 & 15u;
+}
+// live bits of the lane's 16 scores of 32 keys from j0 on: bit r = key j0 + 8 (r / 4) + 4 h + r % 4. kbits: the keys' own 32 bits
+// (length, mask row of all queries), row: the query's own mask row or null
+__device__ __forceinline__ unsigned xa_live(unsigned kbits, const unsigned char* row, int j0, int Lk) {
+    const int h = (threadIdx.x & 63) >> 5;
+    unsigned m = 0;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) m |= ((kbits >> (8 * a + 4 * h)) & 15u) << (4 * a);
+    if (row) {
+        unsigned q = 0;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) q |= xa_mask4(row, j0 + 8 * a + 4 * h, Lk) << (4 * a);
+        m &= q;
+    }
+    return m;
+}
+__device__ __forceinline__ float xa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }   // (below 2^-126: 0)
+// Between a matrix instruction and the first read of its result no branch may join: the compiler's wait count there follows one of the joining
+// paths only. Live bits are therefore made in front of the products, masked and unmasked tiles are separate straight bodies, and behind a
+// loop of products this wait stands.
+__device__ __forceinline__ void xa_settle() { asm volatile("s_nop 15\n\ts_nop 7" ::: "memory"); }
+
+// ------------------------------------------------------------------------------------------------ forward
+// WQ = 4: four waves x 32 rows, every wave reads all 64 keys of a tile. WQ = 1: 32 rows (a single token, a few), the four waves each take
+// 32 of the tile's 128 keys with a softmax of their own and are joined at the end. ns > 1: the tiles of states are cut in ns ranges,
+// joined by xa_join_kernel.
+template <typename T, int DP, int WQ>
+__global__ __launch_bounds__(256) void xa_fwd_kernel(XaArgs p, int nqt, int total) {
+    constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, KW = WQ == 4 ? 64 : 32, KT = KW * (4 / WQ), QT = 32 * WQ;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    char *ks = smem, *vs = smem + KT * CH * 16;
+    const int id = xa_tile_id(total);
+    if (id >= total) return;
+    const int bh = id / (nqt * p.ns), rest = id - bh * nqt * p.ns, split = rest / nqt, qt = rest - split * nqt;
+    const int b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int r = qt * QT + (WQ == 4 ? wave * 32 : 0) + (lane & 31);
+    const int iq = r < p.R ? xa_row_query(p, r) : 0, head = hk * p.G + (r < p.R ? r - iq * p.G : 0);
+    const int len = xa_len(p, b), nt = (len + KT - 1) / KT, per = (nt + p.ns - 1) / p.ns;
+    const int t0 = split * per, t1 = min(nt, t0 + per);
+    uint4 qf[S];
+    xa_row_frag<T, CH>(qf, r < p.R ? reinterpret_cast<const T*>(p.q) + b * p.qb + (long long)iq * p.ql + head * p.qh : nullptr, p.D);
+    const T* kp = reinterpret_cast<const T*>(p.k) + b * p.kb + hk * p.kh;
+    const T* vp = reinterpret_cast<const T*>(p.v) + b * p.vb + hk * p.vh;
+    const unsigned char* mb = p.mask ? p.mask + b * p.mb : nullptr;
+    const bool kmask = mb && p.mq == 0;
+    const unsigned char* mrow = mb && !kmask ? mb + (long long)iq * p.mq : nullptr;   // (null or not: the same for the whole launch)
+    auto krow = [&](int t) { return [=](int i) -> const T* { const int j = t * KT + i; return j < len && (!kmask || mb[j]) ? kp + j * p.kl : nullptr; }; };
+    auto vrow = [&](int t) { return [=](int i) -> const T* { const int j = t * KT + i; return j < len && (!kmask || mb[j]) ? vp + j * p.vl : nullptr; }; };
+    XaStage<T, CH, KT> sk, sv;
+    f32x16_t oacc[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[d][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    if (t0 < t1) { sk.load(p.D, krow(t0)); sv.load(p.D, vrow(t0)); }
+    for (int t = t0; t < t1; ++t) {
+        __syncthreads();
+        sk.store(ks); sv.store(vs);
+        __syncthreads();
+        if (t + 1 < t1) { sk.load(p.D, krow(t + 1)); sv.load(p.D, vrow(t + 1)); }
+        const int row0 = WQ == 4 ? 0 : wave * 32, j0 = t * KT + row0;
+        const int jl = j0 + lane;
+        const unsigned long long kbits = __ballot(lane < KW && jl < len && (!kmask || mb[jl]));
+        auto body = [&](auto masked) {
+            f32x16_t sc[KW / 32];
+            unsigned live[KW / 32];
+            if constexpr (decltype(masked)::value) {
+#pragma unroll
+                for (int kb = 0; kb < KW / 32; ++kb) live[kb] = xa_live((unsigned)(kbits >> (32 * kb)), mrow, j0 + 32 * kb, p.Lk);
+            }
+            float tm = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < KW / 32; ++kb) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[kb][e] = 0.f;
+#pragma unroll
+                for (int s = 0; s < S; ++s) xa_dot(sc[kb], *reinterpret_cast<const uint4*>(ks + xa_at<CH>(row0 + kb * 32 + (lane & 31), 2 * s + h)), qf[s], T());
+            }
+#pragma unroll
+            for (int kb = 0; kb < KW / 32; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    sc[kb][e] *= p.c;
+                    if constexpr (decltype(masked)::value) sc[kb][e] = (live[kb] >> e) & 1 ? sc[kb][e] : -INFINITY;
+                    tm = fmaxf(tm, sc[kb][e]);
+                }
+            tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+            const float mn = fmaxf(m, tm), ref = mn == -INFINITY ? 0.f : mn, al = xa_exp2(m - ref);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) oacc[d][e] *= al;
+#pragma unroll
+            for (int kb = 0; kb < KW / 32; ++kb) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) { sc[kb][e] = xa_exp2(sc[kb][e] - ref); l += sc[kb][e]; }
+                xa_tdot<CH, ND>(oacc, vs, row0 + kb * 32, sc[kb], T());
+            }
+        };
+        if (!mrow && kbits == (KW == 64 ? ~0ull : 0xffffffffull)) body(std::false_type());
+        else body(std::true_type());
+    }
+    xa_settle();
+    l += __shfl_xor(l, 32, 64);
+    if constexpr (WQ == 1) {   // the four waves' softmaxes, in wave order
+        float* ob = reinterpret_cast<float*>(smem);                       // [4][DP][32]
+        float* st = reinterpret_cast<float*>(smem + 2 * KT * CH * 16);    // [4][32] max, [4][32] sum
+        __syncthreads();
+        if (lane < 32) { st[wave * 32 + lane] = m; st[128 + wave * 32 + lane] = l; }
+        __syncthreads();
+        const int n = lane & 31;
+        const float mn = fmaxf(fmaxf(st[n], st[32 + n]), fmaxf(st[64 + n], st[96 + n])), ref = mn == -INFINITY ? 0.f : mn;
+        const float al = xa_exp2(m - ref);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) ob[(wave * DP + d * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + n] = oacc[d][e] * al;
+        l = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) l += st[128 + w * 32 + n] * xa_exp2(st[w * 32 + n] - ref);
+        m = mn;
+        __syncthreads();
+        if (wave >= ND) return;   // wave d joins block d of the dims
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int dd = wave * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+            oacc[0][e] = (ob[dd * 32 + n] + ob[(DP + dd) * 32 + n]) + (ob[(2 * DP + dd) * 32 + n] + ob[(3 * DP + dd) * 32 + n]);
+        }
+    }
+    if (r >= p.R) return;
+    const size_t row = (size_t)bh * p.R + r;
+    if (p.ns > 1) {
+        float* o = p.part + ((size_t)split * p.B * p.Hk * p.R + row) * p.D;
+        if (h == 0 && (WQ == 4 || wave == 0)) { float* q = p.ml + ((size_t)split * p.B * p.Hk * p.R + row) * 2; q[0] = m; q[1] = l; }
+#pragma unroll
+        for (int d = 0; d < (WQ == 1 ? 1 : ND); ++d)
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const int dd = (WQ == 1 ? wave : d) * 32 + 8 * a + 4 * h;
+                if (dd < p.D) *reinterpret_cast<float4*>(o + dd) = make_float4(oacc[d][4 * a], oacc[d][4 * a + 1], oacc[d][4 * a + 2], oacc[d][4 * a + 3]);
+            }
+        return;
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    if (p.lse && h == 0 && (WQ == 4 || wave == 0)) p.lse[row] = l > 0.f ? m + log2f(l) : INFINITY;
+    T* o = reinterpret_cast<T*>(p.o) + (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D;
+#pragma unroll
+    for (int d = 0; d < (WQ == 1 ? 1 : ND); ++d)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const int dd = (WQ == 1 ? wave : d) * 32 + 8 * a + 4 * h;
+            const float v[4] = {oacc[d][4 * a] * inv, oacc[d][4 * a + 1] * inv, oacc[d][4 * a + 2] * inv, oacc[d][4 * a + 3] * inv};
+            if (dd < p.D) Op4<T>::store(o + dd, v);
+        }
+}
+
+// the ns ranges of a row, in range order: 32 lanes a row, four dims a lane
+template <typename T>
+__global__ __launch_bounds__(256) void xa_join_kernel(XaArgs p) {
+    const long long rows = (long long)p.B * p.Hk * p.R, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const int d = (threadIdx.x & 31) * 4;
+    float mn = -INFINITY;
+    for (int s = 0; s < p.ns; ++s) mn = fmaxf(mn, p.ml[((size_t)s * rows + row) * 2]);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.ns; ++s) {
+        const float* q = p.ml + ((size_t)s * rows + row) * 2;
+        const float w = xa_exp2(q[0] - ref);
+        l += q[1] * w;
+        if (d < p.D) {
+            const float4 a = *reinterpret_cast<const float4*>(p.part + ((size_t)s * rows + row) * p.D + d);
+            o[0] += a.x * w; o[1] += a.y * w; o[2] += a.z * w; o[3] += a.w * w;
+        }
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    if (p.lse && d == 0) p.lse[row] = l > 0.f ? mn + log2f(l) : INFINITY;
+    if (d >= p.D) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
+    const int bh = (int)(row / p.R), r = (int)(row - (long long)bh * p.R), b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int iq = xa_row_query(p, r), head = hk * p.G + r - iq * p.G;
+    Op4<T>::store(reinterpret_cast<T*>(p.o) + (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D + d, o);
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dq (and D)
+// Four waves x 32 rows, tiles of 64 keys, as the forward; also leaves D for the kernel behind it.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void xa_dq_kernel(XaArgs p, int nqt, int total) {
+    constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, KT = 64;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    char *ks = smem, *vs = smem + KT * CH * 16;
+    const int id = xa_tile_id(total);
+    if (id >= total) return;
+    const int bh = id / nqt, qt = id - bh * nqt, b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int r = qt * 128 + wave * 32 + (lane & 31);
+    const bool on = r < p.R;
+    const int iq = on ? xa_row_query(p, r) : 0, head = hk * p.G + (on ? r - iq * p.G : 0);
+    const int len = xa_len(p, b), nt = (len + KT - 1) / KT;
+    const size_t orow = (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D;
+    uint4 qf[S], gf[S];
+    xa_row_frag<T, CH>(qf, on ? reinterpret_cast<const T*>(p.q) + b * p.qb + (long long)iq * p.ql + head * p.qh : nullptr, p.D);
+    xa_row_frag<T, CH>(gf, on ? reinterpret_cast<const T*>(p.g) + orow : nullptr, p.D);
+    float dl = 0.f;
+    {
+        uint4 of[S];
+        xa_row_frag<T, CH>(of, on ? reinterpret_cast<const T*>(p.o) + orow : nullptr, p.D);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            constexpr int E = 16 / (int)sizeof(T);
+            const T* ga = reinterpret_cast<const T*>(&gf[s]);
+            const T* oa = reinterpret_cast<const T*>(&of[s]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) dl += OpT<T>::to(ga[e]) * OpT<T>::to(oa[e]);
+        }
+        dl += __shfl_xor(dl, 32, 64);
+    }
+    const float ls = on ? p.lse[(size_t)bh * p.R + r] : INFINITY;
+    if (on && h == 0) p.delta[(size_t)bh * p.R + r] = dl;
+    if (!p.dq) return;   // (uniform over the launch)
+    const T* kp = reinterpret_cast<const T*>(p.k) + b * p.kb + hk * p.kh;
+    const T* vp = reinterpret_cast<const T*>(p.v) + b * p.vb + hk * p.vh;
+    const unsigned char* mb = p.mask ? p.mask + b * p.mb : nullptr;
+    const bool kmask = mb && p.mq == 0;
+    const unsigned char* mrow = mb && !kmask ? mb + (long long)iq * p.mq : nullptr;   // (null or not: the same for the whole launch)
+    auto krow = [&](int t) { return [=](int i) -> const T* { const int j = t * KT + i; return j < len && (!kmask || mb[j]) ? kp + j * p.kl : nullptr; }; };
+    auto vrow = [&](int t) { return [=](int i) -> const T* { const int j = t * KT + i; return j < len && (!kmask || mb[j]) ? vp + j * p.vl : nullptr; }; };
+    XaStage<T, CH, KT> sk, sv;
+    f32x16_t acc[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+    if (nt) { sk.load(p.D, krow(0)); sv.load(p.D, vrow(0)); }
+    for (int t = 0; t < nt; ++t) {
+        __syncthreads();
+        sk.store(ks); sv.store(vs);
+        __syncthreads();
+        if (t + 1 < nt) { sk.load(p.D, krow(t + 1)); sv.load(p.D, vrow(t + 1)); }
+        const int jl = t * KT + lane;
+        const unsigned long long kbits = __ballot(jl < len && (!kmask || mb[jl]));
+        auto body = [&](auto masked) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                unsigned live = 0;
+                if constexpr (decltype(masked)::value) live = xa_live((unsigned)(kbits >> (32 * kb)), mrow, t * KT + 32 * kb, p.Lk);
+                f32x16_t sc, dp;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) { sc[e] = 0.f; dp[e] = 0.f; }
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    const int at = xa_at<CH>(kb * 32 + (lane & 31), 2 * s + h);
+                    xa_dot(sc, *reinterpret_cast<const uint4*>(ks + at), qf[s], T());
+                    xa_dot(dp, *reinterpret_cast<const uint4*>(vs + at), gf[s], T());
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    sc[e] = xa_exp2(sc[e] * p.c - ls) * (dp[e] - dl);
+                    if constexpr (decltype(masked)::value) sc[e] = (live >> e) & 1 ? sc[e] : 0.f;
+                }
+                xa_tdot<CH, ND>(acc, ks, kb * 32, sc, T());
+            }
+        };
+        if (!mrow && kbits == ~0ull) body(std::false_type());
+        else body(std::true_type());
+    }
+    xa_settle();
+    if (!on) return;
+    T* o = reinterpret_cast<T*>(p.dq) + orow;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const int dd = d * 32 + 8 * a + 4 * h;
+            const float v[4] = {acc[d][4 * a] * p.scale, acc[d][4 * a + 1] * p.scale, acc[d][4 * a + 2] * p.scale, acc[d][4 * a + 3] * p.scale};
+            if (dd < p.D) Op4<T>::store(o + dd, v);
+        }
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dk, dv
+// A lane owns one key. WK = 4: four waves x 32 keys, every wave reads all 64 rows of a tile of queries. WK = 1: 32 keys, the waves each
+// take 32 of the tile's 128 rows and are joined at the end. ns > 1: the rows are cut in ns ranges, added in range order by xa_fold_kernel.
+template <typename T, int DP, int WK>
+__global__ __launch_bounds__(256) void xa_dkv_kernel(XaArgs p, int nkt, int total) {
+    constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, RW = WK == 4 ? 64 : 32, RT = RW * (4 / WK);
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    char *qs = smem, *gs = smem + RT * CH * 16;
+    float* lss = reinterpret_cast<float*>(smem + 2 * RT * CH * 16);   // [RT] lse, [RT] D, [RT] query of the row
+    float* dls = lss + RT;
+    int* iqs = reinterpret_cast<int*>(dls + RT);
+    const int id = xa_tile_id(total);
+    if (id >= total) return;
+    const int bh = id / (nkt * p.ns), rest = id - bh * nkt * p.ns, kt = rest / p.ns, split = rest - kt * p.ns;
+    const int b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int key = kt * 32 * WK + (WK == 4 ? wave * 32 : 0) + (lane & 31);
+    const int len = xa_len(p, b);
+    const unsigned char* mb = p.mask ? p.mask + b * p.mb : nullptr;
+    const bool kmask = mb && p.mq == 0, klive = key < len && (!kmask || mb[key]);
+    const bool qmask = mb && !kmask;
+    const int nt = kt * 32 * WK < len ? (p.R + RT - 1) / RT : 0, per = (nt + p.ns - 1) / p.ns;
+    const int t0 = split * per, t1 = min(nt, t0 + per);
+    uint4 kf[S], vf[S];
+    xa_row_frag<T, CH>(kf, klive ? reinterpret_cast<const T*>(p.k) + b * p.kb + hk * p.kh + key * p.kl : nullptr, p.D);
+    xa_row_frag<T, CH>(vf, klive ? reinterpret_cast<const T*>(p.v) + b * p.vb + hk * p.vh + key * p.vl : nullptr, p.D);
+    const T* qp = reinterpret_cast<const T*>(p.q) + b * p.qb + hk * p.G * p.qh;
+    const T* gp = reinterpret_cast<const T*>(p.g) + ((size_t)b * p.Lq * p.Hk + hk) * p.G * p.D;
+    auto qrow = [&](int t) { return [=](int i) -> const T* {
+        const int r = t * RT + i;
+        if (r >= p.R) return nullptr;
+        const int iq = xa_row_query(p, r);
+        return qp + (long long)iq * p.ql + (r - iq * p.G) * p.qh; }; };
+    auto grow = [&](int t) { return [=](int i) -> const T* {
+        const int r = t * RT + i;
+        if (r >= p.R) return nullptr;
+        const int iq = xa_row_query(p, r);
+        return gp + ((size_t)iq * p.Hk * p.G + (r - iq * p.G)) * p.D; }; };
+    XaStage<T, CH, RT> sq, sg;
+    f32x16_t dk[ND], dv[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { dk[d][e] = 0.f; dv[d][e] = 0.f; }
+    if (t0 < t1) { sq.load(p.D, qrow(t0)); sg.load(p.D, grow(t0)); }
+    for (int t = t0; t < t1; ++t) {
+        __syncthreads();
+        sq.store(qs); sg.store(gs);
+        if (threadIdx.x < RT) {
+            const int r = t * RT + threadIdx.x;
+            const bool on = r < p.R;
+            lss[threadIdx.x] = on ? p.lse[(size_t)bh * p.R + r] : INFINITY;   // (a row behind the last: probabilities 0)
+            dls[threadIdx.x] = on ? p.delta[(size_t)bh * p.R + r] : 0.f;
+            iqs[threadIdx.x] = on ? xa_row_query(p, r) : 0;
+        }
+        __syncthreads();
+        if (t + 1 < t1) { sq.load(p.D, qrow(t + 1)); sg.load(p.D, grow(t + 1)); }
+        auto body = [&](auto masked) {
+#pragma unroll
+            for (int rb = 0; rb < RW / 32; ++rb) {
+                const int row0 = (WK == 4 ? 0 : wave * 32) + rb * 32;
+                unsigned live = klive ? 0xffffu : 0u;
+                if constexpr (decltype(masked)::value) {
+                    if (qmask && klive) {
+                        live = 0;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) live |= (mb[(long long)iqs[row0 + 8 * (e >> 2) + 4 * h + (e & 3)] * p.mq + key] != 0 ? 1u : 0u) << e;
+                    }
+                }
+                f32x16_t pr, ds;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) { pr[e] = 0.f; ds[e] = 0.f; }
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    const int at = xa_at<CH>(row0 + (lane & 31), 2 * s + h);
+                    xa_dot(pr, *reinterpret_cast<const uint4*>(qs + at), kf[s], T());
+                    xa_dot(ds, *reinterpret_cast<const uint4*>(gs + at), vf[s], T());
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int row = row0 + 8 * (e >> 2) + 4 * h + (e & 3);
+                    pr[e] = xa_exp2(pr[e] * p.c - lss[row]);
+                    ds[e] = pr[e] * (ds[e] - dls[row]);
+                    if constexpr (decltype(masked)::value) {
+                        pr[e] = (live >> e) & 1 ? pr[e] : 0.f;
+                        ds[e] = (live >> e) & 1 ? ds[e] : 0.f;
+                    }
+                }
+                xa_tdot<CH, ND>(dv, gs, row0, pr, T());
+                xa_tdot<CH, ND>(dk, qs, row0, ds, T());
+            }
+        };
+        if (!qmask && __ballot(klive) == ~0ull) body(std::false_type());
+        else body(std::true_type());
+    }
+    xa_settle();
+    if constexpr (WK == 1) {   // the four waves' rows, in wave order; wave d keeps block d of the dims
+        float* ob = reinterpret_cast<float*>(smem);   // [4][DP][32]
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            __syncthreads();
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) ob[(wave * DP + d * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + (lane & 31)] = which ? dv[d][e] : dk[d][e];
+            __syncthreads();
+            if (wave < ND) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int dd = wave * 32 + 8 * (e >> 2) + 4 * h + (e & 3), n = lane & 31;
+                    const float s = (ob[dd * 32 + n] + ob[(DP + dd) * 32 + n]) + (ob[(2 * DP + dd) * 32 + n] + ob[(3 * DP + dd) * 32 + n]);
+                    if (which) dv[0][e] = s; else dk[0][e] = s;
+                }
+            }
+        }
+        if (wave >= ND) return;
+    }
+    if (key >= p.Lk) return;
+#pragma unroll
+    for (int d = 0; d < (WK == 1 ? 1 : ND); ++d)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const int dd = (WK == 1 ? wave : d) * 32 + 8 * a + 4 * h;
+            if (dd >= p.D) continue;
+            const float vk[4] = {dk[d][4 * a] * p.scale, dk[d][4 * a + 1] * p.scale, dk[d][4 * a + 2] * p.scale, dk[d][4 * a + 3] * p.scale};
+            const float vv[4] = {dv[d][4 * a], dv[d][4 * a + 1], dv[d][4 * a + 2], dv[d][4 * a + 3]};
+            if (p.ns > 1) {
+                const size_t n = (size_t)p.B * p.Hk * p.Lk * p.D, at = ((size_t)bh * p.Lk + key) * p.D + dd;
+                Op4<float>::store(p.part + (size_t)split * n + at, vk);
+                Op4<float>::store(p.part + (size_t)(p.ns + split) * n + at, vv);
+            } else {
+                const size_t at = (((size_t)b * p.Lk + key) * p.Hk + hk) * p.D + dd;
+                Op4<T>::store(reinterpret_cast<T*>(p.dk) + at, vk);
+                Op4<T>::store(reinterpret_cast<T*>(p.dv) + at, vv);
+            }
+        }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void xa_fold_kernel(XaArgs p) {
+    const long long n = (long long)p.B * p.Hk * p.Lk * p.D, i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    const float* src = p.part + (size_t)blockIdx.y * p.ns * n + i;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < p.ns; ++k) {
+        const float4 a = *reinterpret_cast<const float4*>(src + (size_t)k * n);
+        s[0] += a.x; s[1] += a.y; s[2] += a.z; s[3] += a.w;
+    }
+    const long long row = i / p.D;
+    const int d = (int)(i - row * p.D), bh = (int)(row / p.Lk), key = (int)(row - (long long)bh * p.Lk), b = bh / p.Hk, hk = bh - b * p.Hk;
+    Op4<T>::store(reinterpret_cast<T*>(blockIdx.y ? p.dv : p.dk) + (((size_t)b * p.Lk + key) * p.Hk + hk) * p.D + d, s);
+}
+
+// ------------------------------------------------------------------------------------------------ entry points
+#define XA_WGS 512   // workgroups that fill the chip: 256 CUs, two each
+static int xa_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+// ranges of the states (forward) for `tiles` workgroups over `nt` tiles of states: enough workgroups, at least two tiles each
+static int xa_splits(long long tiles, long long nt) {
+    if (tiles >= XA_WGS || nt < 2) return 1;
+    long long ns = (XA_WGS + tiles - 1) / tiles;
+    if (ns > nt / 2) ns = nt / 2;
+    if (ns > 64) ns = 64;
+    return ns < 1 ? 1 : (int)ns;
+}
+struct XaPlan { int wq, nqt, ns, wk, nkt, nsb; };
+static XaPlan xa_plan(int B, long long R, int Lk, int Hk) {
+    XaPlan q;
+    q.wq = R <= 32 ? 1 : 4;
+    q.nqt = (int)((R + 32 * q.wq - 1) / (32 * q.wq));
+    const int kt = q.wq == 4 ? 64 : 128;
+    q.ns = xa_splits((long long)B * Hk * q.nqt, (Lk + kt - 1) / kt);
+    q.wk = Lk <= 32 ? 1 : 4;
+    q.nkt = (Lk + 32 * q.wk - 1) / (32 * q.wk);
+    const int rt = q.wk == 4 ? 64 : 128;
+    q.nsb = xa_splits((long long)B * Hk * q.nkt, (R + rt - 1) / rt);
+    return q;
+}
+static bool xa_bad(int B, int Lq, int Lk, int Hk, int G, int D, int dtype) {
+    if (B < 1 || Lq < 1 || Lk < 0 || Hk < 1 || G < 1 || D < 8 || D > 128 || D % 8 || (dtype & ~1)) return true;
+    const long long R = (long long)Lq * G;
+    // (rows, tiles and workgroups are counted in 32 bits; the offsets of rows in 64)
+    return R > (1LL << 30) || Lk > (1 << 30) || (long long)B * Hk * ((R + 31) / 32) > (1LL << 28) || (long long)B * Hk * ((Lk + 31) / 32) > (1LL << 28);
+}
+extern "C" int l2i_cross_attention_scratch(int B, int Lq, int Lk, int Hk, int G, int D, int bwd, long long* floats) {
+    if (!floats || xa_bad(B, Lq, Lk, Hk, G, D, 0)) return L2I_ERR_ARG;
+    const long long R = (long long)Lq * G;
+    const XaPlan q = xa_plan(B, R, Lk, Hk);
+    if (bwd) *floats = ((long long)B * Hk * R + 3) / 4 * 4 + (q.nsb > 1 ? 2LL * q.nsb * B * Hk * Lk * D : 0);
+    else *floats = q.ns > 1 ? (long long)q.ns * B * Hk * R * (D + 2) : 0;
+    return L2I_OK;
+}
+template <typename K>
+static int xa_lds(K kernel, size_t lds) {
+    return lds > 64 * 1024 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess ? L2I_ERR_LAUNCH : L2I_OK;
+}
+static unsigned xa_grid(long long total) { return (unsigned)((total + 7) / 8 * 8); }
+
+template <typename T, int DP, int WQ>
+static int xa_fwd_launch(const XaArgs& a, const XaPlan& q, hipStream_t s) {
+    const int kt = WQ == 4 ? 64 : 128, total = a.B * a.Hk * q.nqt * a.ns;
+    const size_t lds = (size_t)2 * kt * DP * sizeof(T) + (WQ == 1 ? 256 * sizeof(float) : 0);
+    if (int e = xa_lds(xa_fwd_kernel<T, DP, WQ>, lds)) return e;
+    hipLaunchKernelGGL((xa_fwd_kernel<T, DP, WQ>), dim3(xa_grid(total)), dim3(256), lds, s, a, q.nqt, total);
+    return L2I_OK;
+}
+template <typename T>
+static int xa_fwd_type(const XaArgs& a, const XaPlan& q, hipStream_t s) {
+    const int dp = xa_dp(a.D);
+    int e;
+    if (q.wq == 1) e = dp == 32 ? xa_fwd_launch<T, 32, 1>(a, q, s) : dp == 64 ? xa_fwd_launch<T, 64, 1>(a, q, s) : xa_fwd_launch<T, 128, 1>(a, q, s);
+    else e = dp == 32 ? xa_fwd_launch<T, 32, 4>(a, q, s) : dp == 64 ? xa_fwd_launch<T, 64, 4>(a, q, s) : xa_fwd_launch<T, 128, 4>(a, q, s);
+    if (e) return e;
+    if (a.ns > 1) {
+        const long long rows = (long long)a.B * a.Hk * a.R;
+        hipLaunchKernelGGL((xa_join_kernel<T>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a);
+    }
+    return L2I_OK;
+}
+template <typename T, int DP>
+static int xa_bwd_launch(const XaArgs& a, const XaPlan& q, hipStream_t s) {
+    const int nqt = (a.R + 127) / 128, tq = a.B * a.Hk * nqt, tk = a.B * a.Hk * q.nkt * a.ns;
+    const size_t lq = (size_t)2 * 64 * DP * sizeof(T);
+    if (int e = xa_lds(xa_dq_kernel<T, DP>, lq)) return e;
+    hipLaunchKernelGGL((xa_dq_kernel<T, DP>), dim3(xa_grid(tq)), dim3(256), lq, s, a, nqt, tq);
+    if (!a.dk || a.Lk == 0) return L2I_OK;
+    const int rt = q.wk == 4 ? 64 : 128;
+    const size_t lk = (size_t)2 * rt * DP * sizeof(T) + (size_t)rt * 12;
+    if (q.wk == 4) {
+        if (int e = xa_lds(xa_dkv_kernel<T, DP, 4>, lk)) return e;
+        hipLaunchKernelGGL((xa_dkv_kernel<T, DP, 4>), dim3(xa_grid(tk)), dim3(256), lk, s, a, q.nkt, tk);
+    } else {
+        if (int e = xa_lds(xa_dkv_kernel<T, DP, 1>, lk)) return e;
+        hipLaunchKernelGGL((xa_dkv_kernel<T, DP, 1>), dim3(xa_grid(tk)), dim3(256), lk, s, a, q.nkt, tk);
+    }
+    if (a.ns > 1) {
+        const long long n = (long long)a.B * a.Hk * a.Lk * a.D;
+        hipLaunchKernelGGL((xa_fold_kernel<T>), dim3((unsigned)((n / 4 + 255) / 256), 2), dim3(256), 0, s, a);
+    }
+    return L2I_OK;
+}
+// strides: 16-byte steps between any two rows, so that every row starts on a 16-byte boundary
+static bool xa_rows_ok(const void* t, long long sb, long long sl, long long sh, int dtype) {
+    const long long e = dtype ? 8 : 4;
+    return !((size_t)t & 15) && sb % e == 0 && sl % e == 0 && sh % e == 0 && sb >= 0 && sl >= 0 && sh >= 0;
+}
+static void xa_setup(XaArgs& a, const void* q, const void* k, const void* v, const int* lengths, const unsigned char* mask, int B, int Lq, int Lk, int Hk,
+                     int G, int D, long long qb, long long ql, long long qh, long long kb, long long kl, long long kh, long long vb, long long vl, long long vh,
+                     long long mb, long long mq, float scale) {
+    a.q = q; a.k = k; a.v = v; a.len = lengths; a.mask = mask; a.B = B; a.Lq = Lq; a.Lk = Lk; a.Hk = Hk; a.G = G; a.D = D; a.R = Lq * G;
+    a.qb = qb; a.ql = ql; a.qh = qh; a.kb = kb; a.kl = kl; a.kh = kh; a.vb = vb; a.vl = vl; a.vh = vh; a.mb = mb; a.mq = mq;
+    a.scale = scale; a.c = scale * 1.44269504088896340736f;
+}
+extern "C" int l2i_cross_attention_fwd(const void* q, const void* k, const void* v, int dtype, const int* lengths, const unsigned char* mask, void* out,
+                                       float* lse, int B, int Lq, int Lk, int Hk, int G, int D, long long qb, long long ql, long long qh, long long kb,
+                                       long long kl, long long kh, long long vb, long long vl, long long vh, long long mb, long long mq, float scale,
+                                       float* scratch, long long scratch_floats, void* stream) {
+    long long need = 0;
+    if (xa_bad(B, Lq, Lk, Hk, G, D, dtype) || !q || !out || (Lk && (!k || !v)) || mb < 0 || mq < 0 || ((size_t)out & 15)) return L2I_ERR_ARG;
+    if (!xa_rows_ok(q, qb, ql, qh, dtype) || !xa_rows_ok(k, kb, kl, kh, dtype) || !xa_rows_ok(v, vb, vl, vh, dtype)) return L2I_ERR_ARG;
+    if (l2i_cross_attention_scratch(B, Lq, Lk, Hk, G, D, 0, &need) != L2I_OK) return L2I_ERR_ARG;
+    if (need && (!scratch || ((size_t)scratch & 15) || scratch_floats < need)) return L2I_ERR_ARG;
+    XaArgs a = {};
+    xa_setup(a, q, k, v, lengths, mask, B, Lq, Lk, Hk, G, D, qb, ql, qh, kb, kl, kh, vb, vl, vh, mb, mq, scale);
+    const XaPlan pl = xa_plan(B, a.R, Lk, Hk);
+    a.o = out; a.lse = lse; a.ns = pl.ns;
+    a.part = scratch; a.ml = scratch + (size_t)pl.ns * B * Hk * a.R * D;
+    const int e = dtype ? xa_fwd_type<bf16_t>(a, pl, (hipStream_t)stream) : xa_fwd_type<float>(a, pl, (hipStream_t)stream);
+    return e ? e : l2i_check_launch();
+}
+extern "C" int l2i_cross_attention_bwd(const void* q, const void* k, const void* v, int dtype, const int* lengths, const unsigned char* mask, const void* out,
+                                       const float* lse, const void* dout, void* dq, void* dk, void* dv, int B, int Lq, int Lk, int Hk, int G, int D,
+                                       long long qb, long long ql, long long qh, long long kb, long long kl, long long kh, long long vb, long long vl,
+                                       long long vh, long long mb, long long mq, float scale, float* scratch, long long scratch_floats, void* stream) {
+    long long need = 0;
+    if (xa_bad(B, Lq, Lk, Hk, G, D, dtype) || !q || !out || !lse || !dout || (Lk && (!k || !v)) || mb < 0 || mq < 0) return L2I_ERR_ARG;
+    if ((dk == nullptr) != (dv == nullptr) || (((size_t)out | (size_t)dout | (size_t)dq | (size_t)dk | (size_t)dv) & 15)) return L2I_ERR_ARG;
+    if (!xa_rows_ok(q, qb, ql, qh, dtype) || !xa_rows_ok(k, kb, kl, kh, dtype) || !xa_rows_ok(v, vb, vl, vh, dtype)) return L2I_ERR_ARG;
+    if (l2i_cross_attention_scratch(B, Lq, Lk, Hk, G, D, 1, &need) != L2I_OK || !scratch || ((size_t)scratch & 15) || scratch_floats < need) return L2I_ERR_ARG;
+    XaArgs a = {};
+    xa_setup(a, q, k, v, lengths, mask, B, Lq, Lk, Hk, G, D, qb, ql, qh, kb, kl, kh, vb, vl, vh, mb, mq, scale);
+    const XaPlan pl = xa_plan(B, a.R, Lk, Hk);
+    a.o = const_cast<void*>(out); a.lse = const_cast<float*>(lse); a.g = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.ns = pl.nsb;
+    a.delta = scratch; a.part = scratch + ((long long)B * Hk * a.R + 3) / 4 * 4;
+    hipStream_t s = (hipStream_t)stream;
+    const int dp = xa_dp(D);
+    int e;
+    if (dtype) e = dp == 32 ? xa_bwd_launch<bf16_t, 32>(a, pl, s) : dp == 64 ? xa_bwd_launch<bf16_t, 64>(a, pl, s) : xa_bwd_launch<bf16_t, 128>(a, pl, s);
+    else e = dp == 32 ? xa_bwd_launch<float, 32>(a, pl, s) : dp == 64 ? xa_bwd_launch<float, 64>(a, pl, s) : xa_bwd_launch<float, 128>(a, pl, s);
+    return e ? e : l2i_check_launch();
+}

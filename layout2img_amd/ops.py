@@ -6,9 +6,12 @@ are planar (B, O, H, W) f32. Everything here requires a GPU and the built librar
 fallback of any kind.
 """
 import ctypes
+import functools
+import math
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .arena import GemmWeight, PassCtx
@@ -2019,3 +2022,317 @@ class ChannelDropoutFn(Function):
 def channel_dropout(x, u, prob):
     return ChannelDropoutFn.apply(x, u, prob)
 
+
+
+# ----------------------------------------------------------------------------- attention conditioning
+# Operators of a block whose map looks at its layout (or at another sequence) by attention: group norm, cross attention, the states'
+# embedding, dropout. f32 and bf16 tensors; the scratch of a call is its own (two captured graphs never share it).
+_ACTS = {None: 0, "relu": 1, "silu": 2}
+
+
+def _op(t, what, *dtypes):
+    """t, a tensor of one of the types (default: f32 or bf16)."""
+    dtypes = dtypes or (torch.float32, torch.bfloat16)
+    if not torch.is_tensor(t):
+        raise RuntimeError(f"{what}: a tensor expected, got {type(t).__name__}")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{what}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    return t
+
+
+def _same_device(t, *others):
+    """Every tensor of a call lives on the current device (behind the checks of shapes and types, which need none)."""
+    dev = _lib.current_device() if t.is_cuda else None
+    for o in (t,) + others:
+        if o is not None and (not o.is_cuda or o.device.index != dev):
+            _chk(o)   # (its message)
+            raise RuntimeError(f"tensors of one call on {t.device} and {o.device}")
+
+
+def _op_dtype(dtype, default, what):
+    dtype = default if dtype is None else dtype
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f"{what}: op_dtype is torch.float32 or torch.bfloat16, got {dtype}")
+    return dtype
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_floats(name, *sizes):
+    n = (ctypes.c_longlong * 1)()
+    _lib.call(name, *sizes, n)
+    return n[0]
+
+
+def _scratch(device, name, *sizes):
+    """(tensor | None, pointer, floats) of the f32 scratch the library asks for: from the caching allocator, per call."""
+    n = _scratch_floats(name, *sizes)
+    if n == 0:
+        return None, None, 0
+    t = torch.empty(n, dtype=torch.float32, device=device)
+    return t, t.data_ptr(), n
+
+
+def _wants_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _group_norm_fwd(x, groups, weight, bias, eps, act, op_dtype):
+    B, C = x.shape[0], x.shape[-1]
+    HW = x.numel() // (B * C)
+    y = torch.empty(x.shape, dtype=op_dtype, device=x.device)
+    st = torch.empty((2, B, groups), dtype=torch.float32, device=x.device)
+    ws, wp, wn = _scratch(x.device, "l2i_group_norm_scratch", B, HW, C, groups, 0)
+    _lib.call("l2i_group_norm_fwd", x.data_ptr(), _code(x.dtype), _p(weight), _p(bias), y.data_ptr(), _code(op_dtype), st[0].data_ptr(),
+              st[1].data_ptr(), B, HW, C, groups, float(eps), act, wp, wn, _stream())
+    return y, st
+
+
+class GroupNormActFn(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act, op_dtype):
+        y, st = _group_norm_fwd(x, groups, weight, bias, eps, act, op_dtype)
+        ctx.save_for_backward(x, weight, bias, st)
+        ctx.cfg = (groups, act, op_dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, st = ctx.saved_tensors
+        groups, act, op_dtype = ctx.cfg
+        dy = dy.contiguous()
+        B, C = x.shape[0], x.shape[-1]
+        HW = x.numel() // (B * C)
+        nx, nw, nb = ctx.needs_input_grad[:3]
+        dx = torch.empty_like(x) if nx else None
+        dw = torch.empty_like(weight) if nw else None
+        db = torch.empty_like(bias) if nb else None
+        ws, wp, wn = _scratch(x.device, "l2i_group_norm_scratch", B, HW, C, groups, 1)
+        _lib.call("l2i_group_norm_bwd", x.data_ptr(), _code(x.dtype), _p(weight), _p(bias), st[0].data_ptr(), st[1].data_ptr(), dy.data_ptr(),
+                  _code(op_dtype), _p(dx), _p(dw), _p(db), B, HW, C, groups, act, wp, wn, _stream())
+        return dx, dw, db, None, None, None, None
+
+
+def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act=None, op_dtype=None):
+    """act((x - mean) / sqrt(var + eps) * weight + bias) of a channels-last map x (B, ..., C), f32 or bf16, with biased moments over each image's
+    `groups` groups of C / groups consecutive channels. weight, bias: (C,) f32 or None (1, 0). act: None | "relu" | "silu". op_dtype: the
+    result's type (default: x's)."""
+    _op(x, "group_norm_act: x")
+    op_dtype = _op_dtype(op_dtype, x.dtype, "group_norm_act")
+    if x.dim() < 2 or x.numel() == 0 or not x.is_contiguous():
+        raise RuntimeError(f"group_norm_act: a contiguous (B, ..., C) map with values expected, got {tuple(x.shape)}, strides {x.stride()}")
+    C = x.shape[-1]
+    if not isinstance(groups, int) or groups < 1 or C % groups:
+        raise RuntimeError(f"group_norm_act: {C} channels do not divide into {groups} groups")
+    if C > 4096 or x.shape[0] > 65535:
+        raise RuntimeError(f"group_norm_act: at most 4096 channels and 65535 images, got {C} and {x.shape[0]}")
+    if act not in _ACTS:
+        raise RuntimeError(f"group_norm_act: act is None, 'relu' or 'silu', got {act!r}")
+    for t, what in ((weight, "weight"), (bias, "bias")):
+        if t is not None and (_op(t, "group_norm_act: " + what, torch.float32).shape != (C,) or not t.is_contiguous()):
+            raise RuntimeError(f"group_norm_act: {what} is a contiguous ({C},) tensor, got {tuple(t.shape)}, strides {t.stride()}")
+    _same_device(x, weight, bias)
+    if _wants_grad(x, weight, bias):
+        return GroupNormActFn.apply(x, weight, bias, groups, eps, _ACTS[act], op_dtype)
+    return _group_norm_fwd(x, groups, weight, bias, eps, _ACTS[act], op_dtype)[0]
+
+
+def _strides3(t):
+    """Element strides of (batch, position, head); a dimension of one has none."""
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3]))
+
+
+def _xa_args(q, k, v, lengths, mask):
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1], k.shape[2]
+    mb = mq = 0
+    if mask is not None:
+        mb, mq = (s if n > 1 else 0 for s, n in zip(mask.stride()[:2], mask.shape[:2]))
+    return (B, Lq, Lk, Hk, H // Hk, D), _strides3(q) + _strides3(k) + _strides3(v) + (mb, mq)
+
+
+def _cross_attention_fwd(q, k, v, lengths, mask, scale, want_lse):
+    sizes, strides = _xa_args(q, k, v, lengths, mask)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[0] * q.shape[1] * q.shape[2], dtype=torch.float32, device=q.device) if want_lse else None
+    ws, wp, wn = _scratch(q.device, "l2i_cross_attention_scratch", *sizes, 0)
+    _lib.call("l2i_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _code(q.dtype), _p(lengths), _p(mask), out.data_ptr(), _p(lse),
+              *sizes, *strides, scale, wp, wn, _stream())
+    return out, lse
+
+
+class CrossAttentionFn(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, mask, scale):
+        out, lse = _cross_attention_fwd(q, k, v, lengths, mask, scale, True)
+        ctx.save_for_backward(q, k, v, lengths, mask, out, lse)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        q, k, v, lengths, mask, out, lse = ctx.saved_tensors
+        sizes, strides = _xa_args(q, k, v, lengths, mask)
+        g = _aligned(g.contiguous())
+        nq, nk, nv = ctx.needs_input_grad[:3]
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if nq else None
+        dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) if nk or nv else None for _ in range(2))
+        ws, wp, wn = _scratch(q.device, "l2i_cross_attention_scratch", *sizes, 1)
+        _lib.call("l2i_cross_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _code(q.dtype), _p(lengths), _p(mask), out.data_ptr(),
+                  lse.data_ptr(), g.data_ptr(), _p(dq), _p(dk), _p(dv), *sizes, *strides, ctx.scale, wp, wn, _stream())
+        return dq, dk if nk else None, dv if nv else None, None, None, None
+
+
+def _aligned(t):
+    """A gradient that starts inside another tensor may start off a 16-byte boundary: copied then."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
+    """softmax(scale q k^T) v of queries q (B, Lq, H, D) over the states k, v (B, Lk, Hk, D) of another sequence -> (B, Lq, H, D), all f32 or all bf16.
+    H is a multiple of Hk: query head h reads state head h // (H // Hk). D: a multiple of 8, at most 128. scale: default 1 / sqrt(D).
+    lengths: (B,) int32, states at and behind a sequence's length do not exist. mask: (B | 1, Lq | 1, Lk) bool, False = query i does not see state j.
+    A query that sees no state gives zeros. What `lengths` or a mask row shared by all queries takes out is not read, whatever it holds; a state
+    that only some queries see has to be finite. The D values of a head are consecutive; the other strides may be any of whole 16 bytes (slices of
+    a grouped projection, transposed heads, expanded batches)."""
+    for t, what in ((q, "q"), (k, "k"), (v, "v")):
+        _op(t, "cross_attention: " + what)
+        if t.dim() != 4:
+            raise RuntimeError(f"cross_attention: {what} is (B, L, heads, D), got {tuple(t.shape)}")
+        if t.dtype != q.dtype:
+            raise RuntimeError(f"cross_attention: q, k, v have one type, got {q.dtype} and {t.dtype}")
+    B, Lq, H, D = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise RuntimeError(f"cross_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not belong together")
+    Lk, Hk = k.shape[1], k.shape[2]
+    if D % 8 or not 8 <= D <= 128:
+        raise RuntimeError(f"cross_attention: a head has a multiple of 8 values, at most 128; got {D}")
+    if Hk < 1 or H < 1 or H % Hk:
+        raise RuntimeError(f"cross_attention: {H} query heads do not divide over {Hk} state heads")
+    if B < 1 or Lq < 1:
+        raise RuntimeError(f"cross_attention: at least one query, got {tuple(q.shape)}")
+    for t, what in ((q, "q"), (k, "k"), (v, "v")):
+        step = 16 // t.element_size()
+        if t.stride(3) != 1 or any(s % step for s in _strides3(t)) or t.data_ptr() % 16:
+            raise RuntimeError(f"cross_attention: {what} needs consecutive head values and rows on 16-byte boundaries, got strides {t.stride()} "
+                               f"at address {t.data_ptr() % 16} modulo 16 (.contiguous() first)")
+    if lengths is not None and (_op(lengths, "cross_attention: lengths", torch.int32).shape != (B,) or not lengths.is_contiguous()):
+        raise RuntimeError(f"cross_attention: lengths is a contiguous ({B},) tensor, got {tuple(lengths.shape)}, strides {lengths.stride()}")
+    if mask is not None:
+        if _op(mask, "cross_attention: mask", torch.bool).dim() != 3 or mask.shape[0] not in (1, B) or mask.shape[1] not in (1, Lq) or mask.shape[2] != Lk:
+            raise RuntimeError(f"cross_attention: mask is ({B} or 1, {Lq} or 1, {Lk}) bool, got {tuple(mask.shape)}")
+        if Lk > 1 and mask.stride(2) != 1:
+            raise RuntimeError("cross_attention: the mask's last dimension has to be consecutive (.contiguous() first)")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    _same_device(q, k, v, lengths, mask)
+    if _wants_grad(q, k, v):
+        return CrossAttentionFn.apply(q, k, v, lengths, mask, scale)
+    return _cross_attention_fwd(q, k, v, lengths, mask, scale, False)[0]
+
+
+def _embedding_fwd(weight, tokens, scale, padding_idx, op_dtype):
+    V, D = weight.shape
+    out = torch.empty(tokens.shape + (D,), dtype=op_dtype, device=weight.device)
+    _lib.call("l2i_embedding_fwd", weight.data_ptr(), _code(weight.dtype), tokens.data_ptr(), out.data_ptr(), _code(op_dtype), tokens.numel(), V, D,
+              scale, padding_idx, _stream())
+    return out
+
+
+class EmbeddingFn(Function):
+    @staticmethod
+    def forward(ctx, weight, tokens, scale, padding_idx, op_dtype):
+        ctx.save_for_backward(tokens)
+        ctx.cfg = (weight.shape, weight.dtype, scale, padding_idx)
+        return _embedding_fwd(weight, tokens, scale, padding_idx, op_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (tokens,) = ctx.saved_tensors
+        (V, D), dtype, scale, padding_idx = ctx.cfg
+        dy = dy.contiguous()
+        dw = torch.empty((V, D), dtype=dtype, device=dy.device)
+        ws, wp, wn = _scratch(dy.device, "l2i_embedding_bwd_scratch", tokens.numel(), D)
+        _lib.call("l2i_embedding_bwd", tokens.data_ptr(), dy.data_ptr(), _code(dy.dtype), dw.data_ptr(), _code(dtype), tokens.numel(), V, D, scale,
+                  padding_idx, wp, wn, _stream())
+        return dw, None, None, None, None
+
+
+def embedding(weight, tokens, scale=1.0, padding_idx=-1, op_dtype=None):
+    """scale * weight[tokens]: rows of a (V, D) table, f32 or bf16, for integer tokens of any shape -> tokens.shape + (D,) in op_dtype (default: the
+    table's). A token outside [0, V), or equal to padding_idx (-1: none), gives zeros and no gradient. The gradient is a dense (V, D) tensor, each
+    row added up in f32 in the order of the tokens' positions: the same bits on every run."""
+    _op(weight, "embedding: weight")
+    op_dtype = _op_dtype(op_dtype, weight.dtype, "embedding")
+    if weight.dim() != 2 or weight.numel() == 0 or weight.shape[0] > 0x7fffff00 or weight.shape[1] > 65536:
+        raise RuntimeError(f"embedding: weight is (V, D) with V < 2^31 - 256 and D <= 65536, got {tuple(weight.shape)}")
+    if not weight.is_contiguous():
+        raise RuntimeError(f"embedding: weight has to be contiguous, got strides {weight.stride()}")
+    if _op(tokens, "embedding: tokens", torch.int64, torch.int32).numel() > 0x7fffffff - 2048:
+        raise RuntimeError(f"embedding: fewer than 2^31 - 2048 tokens, got {tokens.numel()}")
+    if not isinstance(padding_idx, int) or not -1 <= padding_idx < weight.shape[0]:
+        raise RuntimeError(f"embedding: padding_idx is -1 (none) or a row of the table, got {padding_idx}")
+    _same_device(weight, tokens)
+    tokens = tokens.contiguous()
+    if tokens.dtype != torch.int64:
+        tokens = tokens.to(torch.int64)
+    if _wants_grad(weight):
+        return EmbeddingFn.apply(weight, tokens, float(scale), padding_idx, op_dtype)
+    return _embedding_fwd(weight, tokens, float(scale), padding_idx, op_dtype)
+
+
+def _dropout_raw(x, residual, out, rng, used, threshold, scale, layer):
+    _lib.call("l2i_dropout", x.data_ptr(), _code(x.dtype), _p(residual), out.data_ptr(), _code(out.dtype), rng.data_ptr(), _p(used), x.numel(),
+              threshold, scale, layer, _stream())
+    return out
+
+
+class DropoutFn(Function):
+    @staticmethod
+    def forward(ctx, x, residual, rng, threshold, scale, layer, op_dtype):
+        used = torch.empty_like(rng)
+        ctx.save_for_backward(used)
+        ctx.cfg = (x.dtype, threshold, scale, layer)
+        return _dropout_raw(x, residual, torch.empty(x.shape, dtype=op_dtype, device=x.device), rng, used, threshold, scale, layer)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (used,) = ctx.saved_tensors
+        dtype, threshold, scale, layer = ctx.cfg
+        dx = None
+        if ctx.needs_input_grad[0]:
+            g = dy.contiguous()
+            dx = _dropout_raw(g, None, torch.empty(g.shape, dtype=dtype, device=g.device), used, None, threshold, scale, layer)
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None, None
+
+
+def dropout(x, p, rng, residual=None, layer=0, op_dtype=None):
+    """residual + (x / (1 - p) where a draw keeps the element, 0 elsewhere): elementwise dropout with probability p, in one pass, whose mask is
+    a function of (rng, layer, element) and is never stored. rng: (2,) int64 on the device, [seed, offset]; the same pair gives the same mask.
+    Advance the offset between steps (rng[1] += 1, also inside a captured graph) and give each dropout of a step a `layer` of its own; the
+    backward pass uses the pair that the forward read. x: any shape, f32 or bf16; residual: x's shape in the result's type. op_dtype: the
+    result's type (default: the residual's, else x's)."""
+    _op(x, "dropout: x")
+    if residual is not None:
+        _op(residual, "dropout: residual")
+    op_dtype = _op_dtype(op_dtype, x.dtype if residual is None else residual.dtype, "dropout")
+    if not 0.0 <= p <= 1.0:
+        raise RuntimeError(f"dropout: p lies in [0, 1], got {p}")
+    if not isinstance(layer, int) or not 0 <= layer < 1 << 31:
+        raise RuntimeError(f"dropout: layer is an integer in [0, 2^31), got {layer!r}")
+    if _op(rng, "dropout: rng", torch.int64).shape != (2,) or not rng.is_contiguous():
+        raise RuntimeError(f"dropout: rng is a contiguous (2,) tensor, got {tuple(rng.shape)}, strides {rng.stride()}")
+    if not x.is_contiguous() or (residual is not None and not residual.is_contiguous()):
+        raise RuntimeError("dropout: x and residual have to be contiguous")
+    if x.numel() > 1 << 34:
+        raise RuntimeError(f"dropout: at most 2^34 elements, got {x.numel()}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != op_dtype):
+        raise RuntimeError(f"dropout: residual has x's shape and the result's type, got {tuple(residual.shape)} {residual.dtype} for "
+                           f"{tuple(x.shape)} {op_dtype}")
+    _same_device(x, residual, rng)
+    threshold, scale = round(p * 2.0 ** 32), 1.0 / (1.0 - p) if p < 1.0 else 0.0
+    if _wants_grad(x, residual):
+        return DropoutFn.apply(x, residual, rng, threshold, scale, layer, op_dtype)
+    return _dropout_raw(x, residual, torch.empty(x.shape, dtype=op_dtype, device=x.device), rng, None, threshold, scale, layer)
