@@ -5,59 +5,116 @@
 //   backward, dz = dy act'(z):
 //     dbeta_c = sum dz;  dgamma_c = sum dz xh;  dx = rstd (gamma dz - (S1 + xh S2) / n),  S1 = sum gamma dz, S2 = sum gamma dz xh over the group
 //
-// Bound by bytes. The map is cut in NCH chunks of rows (pixels) per image. The first launch leaves every chunk's moments (mean and sum of
-// squared deviations per group: sums around a value of the chunk itself, so that a mean far from zero costs no digits), the second joins
-// them in chunk order and writes the result; in the backward pass the first leaves the group sums and the channel rows that
-// l2i's ordered fold adds into dgamma / dbeta. Statistics are f32; nothing is accumulated by atomics.
+// Bound by bytes. Two forms:
+//   resident: a workgroup holds all pixels of a slab of whole groups (at least 64 contiguous bytes a pixel) in registers: one launch, every
+//     value read once; used where a slab is at most 32768 values (maps up to 32 x 32 of the wide layers).
+//   split: the map is cut in NCH chunks of rows (pixels) per image. The first launch leaves every chunk's moments (mean and sum of squared
+//     deviations per group: sums around a value of the chunk itself, so that a mean far from zero costs no digits), the second joins
+//     them in a fixed order and writes the result, reading the map a second time -- from the chunk that was read last backwards, on the
+//     XCD that read it, so that L2 and the Infinity Cache still hold what is read first.
+// In the backward pass the sums are S1, S2 per group and rows of (sum dz xh | sum dz) per channel, which the ordered fold adds into dgamma / dbeta (in
+// workgroups of their own at the end of the second launch). Statistics are f32; nothing is accumulated by atomics.
 #include "common.h"
 
 struct GnArgs {
     const void* x; const float* gamma; const float* beta; void* y;
     float* mean; float* rstd;             // [B][G]
     const void* dy; void* dx;
-    float* part;                          // forward: [B][NCH][G] (mean, M2); backward: [B][NCH][G] (S1, S2)
+    float* part;                          // split: [B][NCH][G] (mean, M2), backward (S1, S2)
     float* cpart;                         // backward: [B][NCH][2 Cp] rows of (sum dz xh | sum dz)
     long long HW; long long rows;         // rows per chunk
     int B, C, Cp, G, cg, nch, act;
+    int Cs, slabs, tw, nr;                // resident: channels of a slab, slabs per image, threads along the channels and along the rows
     float eps;
 };
 
-// act'(z) * dy, and act(z)
-__device__ __forceinline__ float gn_act(float z, int act) {
-    if (act == 1) return fmaxf(z, 0.f);
-    if (act == 2) return z / (1.f + __expf(-z));
+// With d = x - mean and A = rstd gamma: z = A d + beta, and every kernel sees a value through d, so that its channel costs three registers.
+// silu: s = 1 / (1 + 2^(-z log2 e)) by the hardware's exp2 and reciprocal (relative 2^-21), silu' = s + z (s - s^2).
+#define GN_LOG2E 1.44269504088896340736f
+__device__ __forceinline__ float gn_sig(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -GN_LOG2E)); }
+template <int ACT> __device__ __forceinline__ float gn_act(float z) {
+    if (ACT == 1) return fmaxf(z, 0.f);
+    if (ACT == 2) return z * gn_sig(z);
     return z;
 }
-__device__ __forceinline__ float gn_dact(float z, float dy, int act) {
-    if (act == 1) return z > 0.f ? dy : 0.f;
-    if (act == 2) { const float s = 1.f / (1.f + __expf(-z)); return dy * s * (1.f + z * (1.f - s)); }
+template <int ACT> __device__ __forceinline__ float gn_dact(float z, float dy) {
+    if (ACT == 1) return z > 0.f ? dy : 0.f;
+    if (ACT == 2) { const float s = gn_sig(z); return dy * fmaf(z, fmaf(-s, s, s), s); }
     return dy;
 }
 
-template <typename T, int V> __device__ __forceinline__ void gn_load(const T* p, float (&v)[V]) {
-    if constexpr (V == 4) Op4<T>::load(p, v);
-    else v[0] = OpT<T>::to(p[0]);
-}
+// V consecutive values as they lie in memory
+template <typename T, int V> struct GnVec {
+    static constexpr int N = V * (int)sizeof(T) / 16;   // 16-byte pieces; 0: one 8-byte piece (bf16 x 4); V = 1: one value
+    uint4 r[N ? N : 1];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (V == 1) r[0].x = sizeof(T) == 4 ? __float_as_uint((float)OpT<T>::to(p[0])) : (unsigned)__float_as_uint(OpT<T>::to(p[0]));
+        else if constexpr (N == 0) { const uint2 u = *reinterpret_cast<const uint2*>(p); r[0].x = u.x; r[0].y = u.y; }
+        else
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+    __device__ __forceinline__ void get(float (&v)[V]) const {
+        if constexpr (V == 1) v[0] = __uint_as_float(r[0].x);
+        else {
+            const unsigned* w = reinterpret_cast<const unsigned*>(r);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if constexpr (sizeof(T) == 4) v[e] = __uint_as_float(w[e]);
+                else v[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+            }
+        }
+    }
+};
 template <typename T, int V> __device__ __forceinline__ void gn_store(T* p, const float (&v)[V]) {
-    if constexpr (V == 4) Op4<T>::store(p, v);
-    else p[0] = OpT<T>::from(v[0]);
+    if constexpr (V == 1) p[0] = OpT<T>::from(v[0]);
+    else if constexpr (sizeof(T) == 2 && V == 8) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(f2bf2(v[0], v[1]), f2bf2(v[2], v[3]), f2bf2(v[4], v[5]), f2bf2(v[6], v[7]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) { const float q[4] = {v[i], v[i + 1], v[i + 2], v[i + 3]}; Op4<T>::store(p + i, q); }
+    }
 }
 
-// Column mapping shared by the four kernels: a workgroup covers all C channels of its rows in tiles of tw = min(C / V, 256) vectors; tw threads
-// stand along the channels, 256 / tw along the rows.
-#define GN_COLS(V)                                                                                                   \
+// f(e, channel c + e, its group): one division for the V channels of a thread
+template <int V, typename F> __device__ __forceinline__ void gn_each(int c, int cg, F f) {
+    int g = c / cg, rem = c - g * cg;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        f(e, c + e, g);
+        if (++rem == cg) { rem = 0; ++g; }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ split form
+// A workgroup covers all C channels of its rows in tiles of tw = min(C / V, 256) vectors; tw threads stand along the channels, 256 / tw along
+// the rows. REV: the chunks from the last to the first, each on the XCD (workgroup number modulo 8) that the other order gives it.
+#define GN_COLS(V, REV)                                                                                              \
     const int cv = p.C / (V), tw = cv < 256 ? cv : 256, nr = 256 / tw, tx = (int)threadIdx.x % tw, ty = (int)threadIdx.x / tw; \
-    const int b = blockIdx.y, ch = blockIdx.x;                                                                       \
+    int id = blockIdx.x;                                                                                             \
+    const int total8 = p.B * p.nch & ~7;                                                                             \
+    if ((REV) && id < total8) id = total8 - 8 - (id & ~7) + (id & 7);                                                \
+    const int b = id / p.nch, ch = id - b * p.nch;                                                                   \
     const long long r0 = ch * p.rows, r1 = r0 + p.rows < p.HW ? r0 + p.rows : p.HW;                                   \
     const size_t img = (size_t)b * p.HW * p.C;
+// rows r0 + ty, + nr, ... of the chunk: LOAD(k, r) puts row r into slot k, four rows in flight, then USE(k, r)
+#define GN_ROWS(LOAD, USE)                                                                                           \
+    do {                                                                                                             \
+        long long r = r0 + ty;                                                                                       \
+        for (; r + 3 * nr < r1; r += 4 * nr) {                                                                       \
+            LOAD(0, r) LOAD(1, r + nr) LOAD(2, r + 2 * nr) LOAD(3, r + 3 * nr)                                       \
+            USE(0, r) USE(1, r + nr) USE(2, r + 2 * nr) USE(3, r + 3 * nr)                                           \
+        }                                                                                                            \
+        for (; r < r1; r += nr) { LOAD(0, r) USE(0, r) }                                                             \
+    } while (0)
 
 template <typename T, int V>
 __global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) float sm[];   // [C] means, [C] squared deviations, [256][2 V] row lanes
     float *cm = sm, *cq = sm + p.Cp, *red = cq + p.Cp;
-    GN_COLS(V)
+    GN_COLS(V, false)
     const T* x = reinterpret_cast<const T*>(p.x) + img;
-    const float n = (float)(r1 - r0);
+    const float n = (float)(r1 - r0), rn = 1.f / n;
     for (int t0 = 0; t0 < cv; t0 += tw) {
         const int c = (t0 + tx) * V;
         const bool on = ty < nr && t0 + tx < cv;
@@ -65,28 +122,28 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) { s[e] = 0.f; q[e] = 0.f; k[e] = 0.f; }
         if (on) {
-            gn_load<T, V>(x + (size_t)r0 * p.C + c, k);
-            for (long long r = r0 + ty; r < r1; r += nr) {
-                float v[V];
-                gn_load<T, V>(x + (size_t)r * p.C + c, v);
-#pragma unroll
-                for (int e = 0; e < V; ++e) { const float d = v[e] - k[e]; s[e] += d; q[e] += d * d; }
-            }
+            GnVec<T, V> a[4];
+            a[0].load(x + (size_t)r0 * p.C + c);
+            a[0].get(k);
+#define GN_L(K, R) a[K].load(x + (size_t)(R) * p.C + c);
+#define GN_U(K, R) { float v[V]; a[K].get(v); _Pragma("unroll") for (int e = 0; e < V; ++e) { const float d = v[e] - k[e]; s[e] += d; q[e] = fmaf(d, d, q[e]); } }
+            GN_ROWS(GN_L, GN_U);
+#undef GN_U
         }
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < V; ++e) { red[threadIdx.x * 2 * V + e] = s[e]; red[threadIdx.x * 2 * V + V + e] = q[e]; }
+        for (int e = 0; e < V; ++e) { red[e * 512 + threadIdx.x] = s[e]; red[e * 512 + 256 + threadIdx.x] = q[e]; }
         __syncthreads();
-        if (ty == 0 && t0 + tx < cv) {
-            for (int j = 1; j < nr; ++j)
-#pragma unroll
-                for (int e = 0; e < V; ++e) { s[e] += red[(j * tw + tx) * 2 * V + e]; q[e] += red[(j * tw + tx) * 2 * V + V + e]; }
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float m = s[e] / n;
-                cm[c + e] = k[e] + m;
-                cq[c + e] = q[e] - s[e] * m;
-            }
+        // channel sums over the row lanes: thread (channel of the tile)
+        for (int i = threadIdx.x; i < tw * V; i += 256) {
+            const int e = i / tw, tt = i - e * tw;
+            if (t0 + tt >= cv) continue;
+            float ss = 0.f, qq = 0.f;
+            for (int j = 0; j < nr; ++j) { ss += red[e * 512 + j * tw + tt]; qq += red[e * 512 + 256 + j * tw + tt]; }
+            const int cc = (t0 + tt) * V + e;
+            const float m = ss * rn;
+            cm[cc] = OpT<T>::to(x[(size_t)r0 * p.C + cc]) + m;
+            cq[cc] = qq - ss * m;
         }
     }
     __syncthreads();
@@ -95,31 +152,45 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs p) {
         for (int c = g * p.cg; c < (g + 1) * p.cg; ++c) m += cm[c];
         m /= (float)p.cg;
         for (int c = g * p.cg; c < (g + 1) * p.cg; ++c) { const float d = cm[c] - m; m2 += cq[c] + n * d * d; }
-        float* o = p.part + (((size_t)b * p.nch + ch) * p.G + g) * 2;
-        o[0] = m; o[1] = m2;
+        *reinterpret_cast<float2*>(p.part + (((size_t)b * p.nch + ch) * p.G + g) * 2) = make_float2(m, m2);
     }
 }
 
-template <typename TI, typename TO, int V>
+// L = 256 / (power of two >= G) lanes a group (at least one) walk the chunks; their sums meet in a butterfly of fixed order
+#define GN_LANES                                                                                                     \
+    int L = 1;                                                                                                       \
+    while (L < 64 && 2 * L * p.G <= 256) L <<= 1;                                                                    \
+    const int gl = (int)threadIdx.x & (L - 1), gs = 256 / L;
+
+template <typename TI, typename TO, int V, int ACT>
 __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) float sm[];   // [G] mean, [G] rstd
     float *gm = sm, *gr = sm + p.G;
-    GN_COLS(V)
-    for (int g = threadIdx.x; g < p.G; g += 256) {
-        const float* q = p.part + ((size_t)b * p.nch * p.G + g) * 2;
-        float m = 0.f, m2 = 0.f;
-        for (int i = 0; i < p.nch; ++i) {
-            const long long ra = i * p.rows, rb = ra + p.rows < p.HW ? ra + p.rows : p.HW;
-            m += q[(size_t)i * p.G * 2] * ((float)(rb - ra) / (float)p.HW);
+    GN_COLS(V, true)
+    {
+        GN_LANES
+        const float cgf = (float)p.cg, N = (float)p.HW * cgf;
+        for (int g0 = 0; g0 < p.G; g0 += gs) {
+            const int g = g0 + (int)threadIdx.x / L;
+            float m0 = 0.f, s = 0.f, q = 0.f;
+            if (g < p.G) {
+                const float2* src = reinterpret_cast<const float2*>(p.part) + (size_t)b * p.nch * p.G + g;
+                m0 = src[0].x;   // the first chunk's mean as the origin of the sums
+                for (int i = gl; i < p.nch; i += L) {
+                    const float2 a = src[(size_t)i * p.G];
+                    const long long ra = i * p.rows, rb = ra + p.rows < p.HW ? ra + p.rows : p.HW;
+                    const float nn = (float)(rb - ra) * cgf, d = a.x - m0;
+                    s = fmaf(nn, d, s);
+                    q += fmaf(nn * d, d, a.y);
+                }
+            }
+            for (int o = 1; o < L; o <<= 1) { s += __shfl_xor(s, o, 64); q += __shfl_xor(q, o, 64); }
+            if (g < p.G && gl == 0) {
+                const float dm = s / N, m = m0 + dm, rs = 1.f / sqrtf(fmaxf(q - s * dm, 0.f) / N + p.eps);
+                gm[g] = m; gr[g] = rs;
+                if (ch == 0) { p.mean[(size_t)b * p.G + g] = m; p.rstd[(size_t)b * p.G + g] = rs; }
+            }
         }
-        for (int i = 0; i < p.nch; ++i) {
-            const long long ra = i * p.rows, rb = ra + p.rows < p.HW ? ra + p.rows : p.HW;
-            const float d = q[(size_t)i * p.G * 2] - m;
-            m2 += q[(size_t)i * p.G * 2 + 1] + d * d * (float)(rb - ra) * (float)p.cg;
-        }
-        const float rs = 1.f / sqrtf(fmaxf(m2, 0.f) / ((float)p.HW * (float)p.cg) + p.eps);
-        gm[g] = m; gr[g] = rs;
-        if (ch == 0) { p.mean[(size_t)b * p.G + g] = m; p.rstd[(size_t)b * p.G + g] = rs; }
     }
     __syncthreads();
     const TI* x = reinterpret_cast<const TI*>(p.x) + img;
@@ -127,93 +198,94 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs p) {
     if (ty >= nr) return;
     for (int t0 = 0; t0 + tx < cv; t0 += tw) {
         const int c = (t0 + tx) * V;
-        float m[V], a[V], o[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const int g = (c + e) / p.cg;
+        float m[V], a_[V], o[V];
+        gn_each<V>(c, p.cg, [&](int e, int ce, int g) {
             m[e] = gm[g];
-            a[e] = gr[g] * (p.gamma ? p.gamma[c + e] : 1.f);
-            o[e] = p.beta ? p.beta[c + e] : 0.f;
-        }
-        for (long long r = r0 + ty; r < r1; r += nr) {
-            float v[V];
-            gn_load<TI, V>(x + (size_t)r * p.C + c, v);
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = gn_act((v[e] - m[e]) * a[e] + o[e], p.act);
-            gn_store<TO, V>(y + (size_t)r * p.C + c, v);
-        }
+            a_[e] = gr[g] * (p.gamma ? p.gamma[ce] : 1.f);
+            o[e] = p.beta ? p.beta[ce] : 0.f;
+        });
+        GnVec<TI, V> a[4];
+#define GN_U(K, R) { float v[V]; a[K].get(v); _Pragma("unroll") for (int e = 0; e < V; ++e) v[e] = gn_act<ACT>(fmaf(v[e] - m[e], a_[e], o[e])); \
+                     gn_store<TO, V>(y + (size_t)(R) * p.C + c, v); }
+        GN_ROWS(GN_L, GN_U);
+#undef GN_U
+#undef GN_L
     }
 }
 
-template <typename TI, typename TO, int V>
+#define GN_L2(K, R) { a[K].load(x + (size_t)(R) * p.C + c); d[K].load(dy + (size_t)(R) * p.C + c); }
+template <typename TI, typename TO, int V, int ACT>
 __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs p) {
-    extern __shared__ __attribute__((aligned(16))) float sm[];   // [C] sum dz xh, [C] sum dz, [256][2 V]
+    extern __shared__ __attribute__((aligned(16))) float sm[];   // [C] sum dz xh, [C] sum dz, [V][2][256]
     float *ca = sm, *cb = sm + p.Cp, *red = cb + p.Cp;
-    GN_COLS(V)
+    GN_COLS(V, false)
     const TI* x = reinterpret_cast<const TI*>(p.x) + img;
     const TO* dy = reinterpret_cast<const TO*>(p.dy) + img;
+    float* o = p.cpart + ((size_t)b * p.nch + ch) * 2 * p.Cp;
     for (int t0 = 0; t0 < cv; t0 += tw) {
         const int c = (t0 + tx) * V;
-        const bool on = ty < nr && t0 + tx < cv;
         float sa[V], sb[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) { sa[e] = 0.f; sb[e] = 0.f; }
-        if (on) {
-            float m[V], rs[V], ga[V], be[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int g = (c + e) / p.cg;
-                m[e] = p.mean[(size_t)b * p.G + g]; rs[e] = p.rstd[(size_t)b * p.G + g];
-                ga[e] = p.gamma ? p.gamma[c + e] : 1.f; be[e] = p.beta ? p.beta[c + e] : 0.f;
-            }
-            for (long long r = r0 + ty; r < r1; r += nr) {
-                float v[V], d[V];
-                gn_load<TI, V>(x + (size_t)r * p.C + c, v);
-                gn_load<TO, V>(dy + (size_t)r * p.C + c, d);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float xh = (v[e] - m[e]) * rs[e], dz = gn_dact(xh * ga[e] + be[e], d[e], p.act);
-                    sa[e] += dz * xh; sb[e] += dz;
-                }
-            }
+        if (ty < nr && t0 + tx < cv) {
+            float m[V], A[V], be[V];
+            gn_each<V>(c, p.cg, [&](int e, int ce, int g) {
+                m[e] = p.mean[(size_t)b * p.G + g];
+                A[e] = p.rstd[(size_t)b * p.G + g] * (p.gamma ? p.gamma[ce] : 1.f); be[e] = p.beta ? p.beta[ce] : 0.f;
+            });
+            GnVec<TI, V> a[4];
+            GnVec<TO, V> d[4];
+#define GN_U(K, R) { float v[V], w[V]; a[K].get(v); d[K].get(w); _Pragma("unroll") for (int e = 0; e < V; ++e) { \
+                     const float dd = v[e] - m[e], dz = gn_dact<ACT>(fmaf(dd, A[e], be[e]), w[e]); sa[e] = fmaf(dz, dd, sa[e]); sb[e] += dz; } }
+            GN_ROWS(GN_L2, GN_U);
+#undef GN_U
         }
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < V; ++e) { red[threadIdx.x * 2 * V + e] = sa[e]; red[threadIdx.x * 2 * V + V + e] = sb[e]; }
+        for (int e = 0; e < V; ++e) { red[e * 512 + threadIdx.x] = sa[e]; red[e * 512 + 256 + threadIdx.x] = sb[e]; }
         __syncthreads();
-        if (ty == 0 && t0 + tx < cv) {
-            for (int j = 1; j < nr; ++j)
-#pragma unroll
-                for (int e = 0; e < V; ++e) { sa[e] += red[(j * tw + tx) * 2 * V + e]; sb[e] += red[(j * tw + tx) * 2 * V + V + e]; }
-            float* o = p.cpart + ((size_t)b * p.nch + ch) * 2 * p.Cp;
-#pragma unroll
-            for (int e = 0; e < V; ++e) { ca[c + e] = sa[e]; cb[c + e] = sb[e]; o[c + e] = sa[e]; o[p.Cp + c + e] = sb[e]; }
+        for (int i = threadIdx.x; i < tw * V; i += 256) {
+            const int e = i / tw, tt = i - e * tw;
+            if (t0 + tt >= cv) continue;
+            float s = 0.f, q = 0.f;
+            for (int j = 0; j < nr; ++j) { s += red[e * 512 + j * tw + tt]; q += red[e * 512 + 256 + j * tw + tt]; }
+            const int cc = (t0 + tt) * V + e;
+            s *= p.rstd[(size_t)b * p.G + cc / p.cg];   // (the sums ran over dz d)
+            ca[cc] = s; cb[cc] = q; o[cc] = s; o[p.Cp + cc] = q;
         }
     }
-    if (threadIdx.x < p.Cp - p.C) {   // (padding columns of the partial rows)
-        float* o = p.cpart + ((size_t)b * p.nch + ch) * 2 * p.Cp + p.C + threadIdx.x;
-        o[0] = 0.f; o[p.Cp] = 0.f;
-    }
+    if (threadIdx.x < p.Cp - p.C) { o[p.C + threadIdx.x] = 0.f; o[p.Cp + p.C + threadIdx.x] = 0.f; }   // (padding columns of the partial rows)
     __syncthreads();
     for (int g = threadIdx.x; g < p.G; g += 256) {
         float s1 = 0.f, s2 = 0.f;
         for (int c = g * p.cg; c < (g + 1) * p.cg; ++c) { const float ga = p.gamma ? p.gamma[c] : 1.f; s1 += ga * cb[c]; s2 += ga * ca[c]; }
-        float* o = p.part + (((size_t)b * p.nch + ch) * p.G + g) * 2;
-        o[0] = s1; o[1] = s2;
+        *reinterpret_cast<float2*>(p.part + (((size_t)b * p.nch + ch) * p.G + g) * 2) = make_float2(s1, s2);
     }
 }
 
-template <typename TI, typename TO, int V>
-__global__ __launch_bounds__(256) void gn_bwd_apply_kernel(GnArgs p) {
-    extern __shared__ __attribute__((aligned(16))) float sm[];   // [G] S1 / n, [G] S2 / n
+// workgroups behind the chunks fold the channel rows into dgamma / dbeta (f.src null: none)
+template <typename TI, typename TO, int V, int ACT>
+__global__ __launch_bounds__(256) void gn_bwd_apply_kernel(GnArgs p, RowsFoldArgs f) {
+    extern __shared__ __attribute__((aligned(16))) float sm[];   // [G] S1 / n, [G] S2 / n; the fold's 256 float4
+    if ((int)blockIdx.x >= p.B * p.nch) {
+        rows_fold2_body(f, (int)blockIdx.x - p.B * p.nch, 0, reinterpret_cast<float4*>(sm));
+        return;
+    }
     float *g1 = sm, *g2 = sm + p.G;
-    GN_COLS(V)
-    const float rn = 1.f / ((float)p.HW * (float)p.cg);
-    for (int g = threadIdx.x; g < p.G; g += 256) {
-        const float* q = p.part + ((size_t)b * p.nch * p.G + g) * 2;
-        float s1 = 0.f, s2 = 0.f;
-        for (int i = 0; i < p.nch; ++i) { s1 += q[(size_t)i * p.G * 2]; s2 += q[(size_t)i * p.G * 2 + 1]; }
-        g1[g] = s1 * rn; g2[g] = s2 * rn;
+    GN_COLS(V, true)
+    {
+        GN_LANES
+        const float rn = 1.f / ((float)p.HW * (float)p.cg);
+        for (int g0 = 0; g0 < p.G; g0 += gs) {
+            const int g = g0 + (int)threadIdx.x / L;
+            float s1 = 0.f, s2 = 0.f;
+            if (g < p.G) {
+                const float2* src = reinterpret_cast<const float2*>(p.part) + (size_t)b * p.nch * p.G + g;
+                for (int i = gl; i < p.nch; i += L) { const float2 a = src[(size_t)i * p.G]; s1 += a.x; s2 += a.y; }
+            }
+            for (int o = 1; o < L; o <<= 1) { s1 += __shfl_xor(s1, o, 64); s2 += __shfl_xor(s2, o, 64); }
+            if (g < p.G && gl == 0) { g1[g] = s1 * rn; g2[g] = s2 * rn; }
+        }
     }
     __syncthreads();
     const TI* x = reinterpret_cast<const TI*>(p.x) + img;
@@ -222,33 +294,184 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(GnArgs p) {
     if (ty >= nr) return;
     for (int t0 = 0; t0 + tx < cv; t0 += tw) {
         const int c = (t0 + tx) * V;
-        float m[V], rs[V], ga[V], be[V], s1[V], s2[V];
+        float m[V], A[V], be[V], s1[V], s2[V];   // dx = A dz - rstd S1 / n - d rstd^2 S2 / n
+        gn_each<V>(c, p.cg, [&](int e, int ce, int g) {
+            const float rs = p.rstd[(size_t)b * p.G + g];
+            m[e] = p.mean[(size_t)b * p.G + g];
+            A[e] = rs * (p.gamma ? p.gamma[ce] : 1.f); be[e] = p.beta ? p.beta[ce] : 0.f;
+            s1[e] = rs * g1[g]; s2[e] = rs * rs * g2[g];
+        });
+        GnVec<TI, V> a[4];
+        GnVec<TO, V> d[4];
+#define GN_U(K, R) { float v[V], w[V]; a[K].get(v); d[K].get(w); _Pragma("unroll") for (int e = 0; e < V; ++e) { \
+                     const float dd = v[e] - m[e], dz = gn_dact<ACT>(fmaf(dd, A[e], be[e]), w[e]); \
+                     v[e] = fmaf(A[e], dz, -fmaf(dd, s2[e], s1[e])); } gn_store<TI, V>(dx + (size_t)(R) * p.C + c, v); }
+        GN_ROWS(GN_L2, GN_U);
+#undef GN_U
+    }
+}
+#undef GN_L2
+
+// ------------------------------------------------------------------------------------------------ resident form
+// Thread (ty, tx) holds rows ty, ty + nr, ... (at most GN_R) of V channels of the slab. Sums over the slab's groups: row lanes meet in a tree in
+// LDS (fixed order), a wave adds a group's channels.
+#define GN_R 4
+template <int V>
+__device__ __forceinline__ void gn_channel_sums(const GnArgs& p, int cs, int tx, int ty, bool on, const float (&s)[V], float* red /* [nr][cs] */, float* out /* [cs] */) {
+    __syncthreads();
+    if (on)
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const int g = (c + e) / p.cg;
-            m[e] = p.mean[(size_t)b * p.G + g]; rs[e] = p.rstd[(size_t)b * p.G + g];
-            ga[e] = p.gamma ? p.gamma[c + e] : 1.f; be[e] = p.beta ? p.beta[c + e] : 0.f;
-            s1[e] = g1[g]; s2[e] = g2[g];
+        for (int e = 0; e < V; ++e) red[ty * cs + tx * V + e] = s[e];
+    int st = 1;
+    while (2 * st < p.nr) st <<= 1;
+    for (; st >= 1; st >>= 1) {
+        __syncthreads();
+        if (on && ty < st && ty + st < p.nr)
+#pragma unroll
+            for (int e = 0; e < V; ++e) red[ty * cs + tx * V + e] += red[(ty + st) * cs + tx * V + e];
+    }
+    if (on && ty == 0)
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[tx * V + e] = red[tx * V + e];
+    __syncthreads();
+}
+#define GN_RES(V)                                                                                                    \
+    const int b = blockIdx.x / p.slabs, slab = blockIdx.x - b * p.slabs, c0 = slab * p.Cs, cs = p.C - c0 < p.Cs ? p.C - c0 : p.Cs; \
+    const int tx = (int)threadIdx.x % p.tw, ty = (int)threadIdx.x / p.tw, c = c0 + tx * (V), g0 = c0 / p.cg, ng = cs / p.cg; \
+    const bool on = ty < p.nr && tx * (V) < cs;                                                                      \
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;                                \
+    const size_t base = ((size_t)b * p.HW + ty) * p.C + c, step = (size_t)p.nr * p.C;
+
+template <typename TI, typename TO, int V, int ACT, int THR>
+__global__ __launch_bounds__(THR) void gn_res_kernel(GnArgs p) {
+    extern __shared__ __attribute__((aligned(16))) float sm[];   // [nr][Cs], [Cs] channel sums, [2][Cs] per-group results
+    float *red = sm, *chan = sm + p.nr * p.Cs, *gres = chan + p.Cs;
+    GN_RES(V)
+    const TI* x = reinterpret_cast<const TI*>(p.x) + base;
+    GnVec<TI, V> a[GN_R];
+    float s[V], v[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < GN_R; ++k) if (on && ty + k * p.nr < p.HW) a[k].load(x + k * step);
+#pragma unroll
+    for (int k = 0; k < GN_R; ++k)
+        if (on && ty + k * p.nr < p.HW) {
+            a[k].get(v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e] += v[e];
         }
-        for (long long r = r0 + ty; r < r1; r += nr) {
-            float v[V], d[V];
-            gn_load<TI, V>(x + (size_t)r * p.C + c, v);
-            gn_load<TO, V>(dy + (size_t)r * p.C + c, d);
+    const float rn = 1.f / ((float)p.HW * (float)p.cg);
+    gn_channel_sums<V>(p, cs, tx, ty, on, s, red, chan);
+    for (int g = wave; g < ng; g += nw) {
+        float t = 0.f;
+        for (int i = lane; i < p.cg; i += 64) t += chan[g * p.cg + i];
+        t = wave_sum(t);
+        if (lane == 0) gres[g] = t * rn;
+    }
+    __syncthreads();
+    float m[V], r[V];
+    gn_each<V>(on ? c : c0, p.cg, [&](int e, int, int g) { m[e] = gres[g - g0]; s[e] = 0.f; });
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float xh = (v[e] - m[e]) * rs[e], dz = gn_dact(xh * ga[e] + be[e], d[e], p.act);
-                v[e] = rs[e] * (ga[e] * dz - (s1[e] + xh * s2[e]));
-            }
-            gn_store<TI, V>(dx + (size_t)r * p.C + c, v);
+    for (int k = 0; k < GN_R; ++k)
+        if (on && ty + k * p.nr < p.HW) {
+            a[k].get(v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) { const float d = v[e] - m[e]; s[e] = fmaf(d, d, s[e]); }
+        }
+    gn_channel_sums<V>(p, cs, tx, ty, on, s, red, chan);
+    for (int g = wave; g < ng; g += nw) {
+        float t = 0.f;
+        for (int i = lane; i < p.cg; i += 64) t += chan[g * p.cg + i];
+        t = wave_sum(t);
+        if (lane == 0) {
+            const float rs = 1.f / sqrtf(t * rn + p.eps);
+            p.mean[(size_t)b * p.G + g0 + g] = gres[g]; p.rstd[(size_t)b * p.G + g0 + g] = rs;
+            gres[p.Cs + g] = rs;
         }
     }
+    __syncthreads();
+    if (!on) return;
+    TO* y = reinterpret_cast<TO*>(p.y) + base;
+    gn_each<V>(c, p.cg, [&](int e, int ce, int g) { r[e] = gres[p.Cs + g - g0] * (p.gamma ? p.gamma[ce] : 1.f); s[e] = p.beta ? p.beta[ce] : 0.f; });
+#pragma unroll
+    for (int k = 0; k < GN_R; ++k)
+        if (ty + k * p.nr < p.HW) {
+            a[k].get(v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = gn_act<ACT>(fmaf(v[e] - m[e], r[e], s[e]));
+            gn_store<TO, V>(y + k * step, v);
+        }
+}
+
+template <typename TI, typename TO, int V, int ACT, int THR>
+__global__ __launch_bounds__(THR) void gn_res_bwd_kernel(GnArgs p) {
+    extern __shared__ __attribute__((aligned(16))) float sm[];   // [nr][Cs], [2][Cs] channel sums, [2][Cs] per-group results
+    float *red = sm, *ra = sm + p.nr * p.Cs, *rb = ra + p.Cs, *gres = rb + p.Cs;
+    GN_RES(V)
+    const TI* x = reinterpret_cast<const TI*>(p.x) + base;
+    const TO* dy = reinterpret_cast<const TO*>(p.dy) + base;
+    GnVec<TI, V> a[GN_R];
+    GnVec<TO, V> d[GN_R];
+#pragma unroll
+    for (int k = 0; k < GN_R; ++k) if (on && ty + k * p.nr < p.HW) { a[k].load(x + k * step); d[k].load(dy + k * step); }
+    float m[V], rs[V], A[V], be[V], sa[V], sb[V], v[V], w[V];
+    gn_each<V>(on ? c : c0, p.cg, [&](int e, int ce, int g) {
+        m[e] = p.mean[(size_t)b * p.G + g]; rs[e] = p.rstd[(size_t)b * p.G + g];
+        A[e] = rs[e] * (p.gamma ? p.gamma[ce] : 1.f); be[e] = p.beta ? p.beta[ce] : 0.f;
+        sa[e] = 0.f; sb[e] = 0.f;
+    });
+#pragma unroll
+    for (int k = 0; k < GN_R; ++k)
+        if (on && ty + k * p.nr < p.HW) {
+            a[k].get(v); d[k].get(w);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float dd = v[e] - m[e], dz = gn_dact<ACT>(fmaf(dd, A[e], be[e]), w[e]);
+                sa[e] = fmaf(dz, dd, sa[e]); sb[e] += dz;
+            }
+        }
+#pragma unroll
+    for (int e = 0; e < V; ++e) sa[e] *= rs[e];   // (sum dz d -> sum dz xh)
+    gn_channel_sums<V>(p, cs, tx, ty, on, sa, red, ra);
+    gn_channel_sums<V>(p, cs, tx, ty, on, sb, red, rb);
+    float* o = p.cpart + (size_t)b * 2 * p.Cp;
+    for (int i = threadIdx.x; i < cs; i += blockDim.x) { o[c0 + i] = ra[i]; o[p.Cp + c0 + i] = rb[i]; }
+    if (c0 + cs == p.C && (int)threadIdx.x < p.Cp - p.C) { o[p.C + threadIdx.x] = 0.f; o[p.Cp + p.C + threadIdx.x] = 0.f; }
+    if (!p.dx) return;   // (uniform over the launch)
+    const float rn = 1.f / ((float)p.HW * (float)p.cg);
+    for (int g = wave; g < ng; g += nw) {
+        float t1 = 0.f, t2 = 0.f;
+        for (int i = lane; i < p.cg; i += 64) {
+            const float gg = p.gamma ? p.gamma[c0 + g * p.cg + i] : 1.f;
+            t1 += gg * rb[g * p.cg + i]; t2 += gg * ra[g * p.cg + i];
+        }
+        t1 = wave_sum(t1); t2 = wave_sum(t2);
+        if (lane == 0) { gres[g] = t1 * rn; gres[p.Cs + g] = t2 * rn; }
+    }
+    __syncthreads();
+    if (!on) return;
+    TI* dx = reinterpret_cast<TI*>(p.dx) + base;
+    gn_each<V>(c, p.cg, [&](int e, int, int g) { sa[e] = rs[e] * gres[g - g0]; sb[e] = rs[e] * rs[e] * gres[p.Cs + g - g0]; });
+#pragma unroll
+    for (int k = 0; k < GN_R; ++k)
+        if (ty + k * p.nr < p.HW) {
+            a[k].get(v); d[k].get(w);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float dd = v[e] - m[e], dz = gn_dact<ACT>(fmaf(dd, A[e], be[e]), w[e]);
+                v[e] = fmaf(A[e], dz, -fmaf(dd, sb[e], sa[e]));
+            }
+            gn_store<TI, V>(dx + k * step, v);
+        }
 }
 
 // ------------------------------------------------------------------------------------------------ entry points
 #define GN_MAX_C 4096
-// chunks per image: 1024 workgroups over the chip, at least 8 rows of 256 vectors each
+// chunks per image: 512 workgroups over the chip (two a CU; 1024 cost 10 us more on four launches over 64 x 64 x 128 x 32 images in bf16, the same in
+// f32: what stands in front of a workgroup's loop is paid less often), at least 8192 values each
 static int gn_chunks(int B, long long HW, int C) {
-    long long want = (1024 + B - 1) / B, most = (HW * C + 8191) / 8192;
+    long long want = (512 + B - 1) / B, most = (HW * C + 8191) / 8192;
     if (want > most) want = most;
     if (want > HW) want = HW;
     if (want > 256) want = 256;
@@ -261,8 +484,33 @@ extern "C" int l2i_group_norm_scratch(int B, long long HW, int C, int G, int bwd
     if (!floats || gn_bad(B, HW, C, G, 0, 0, 0)) return L2I_ERR_ARG;
     const long long nch = gn_chunks(B, HW, C), Cp = (C + 3) & ~3;
     const long long rows = (long long)B * nch;
-    *floats = ((rows * G * 2 + 3) & ~3LL) + (bwd ? rows * 2 * Cp + (rows > L2I_FOLD_DIRECT ? rows_fold_tmp_floats((int)rows, 2 * (int)Cp, 1) : 0) : 0);
+    *floats = ((rows * G * 2 + 3) & ~3LL) + (bwd ? rows * 2 * Cp + (rows > L2I_FOLD_DIRECT ? rows_fold_tmp_floats((int)rows, (int)Cp, 1) : 0) : 0);
     return L2I_OK;
+}
+static int gn_vec(const GnArgs& a, int in, int out) {   // values a vector: 8, 4 or 1, by the channel count and the addresses
+    for (int v = in && out ? 8 : 4; v >= 4; v >>= 1) {
+        const size_t mi = (in ? 2 * v : 16) - 1, mo = (out ? 2 * v : 16) - 1;
+        if (a.C % v == 0 && !(((size_t)a.x | (size_t)a.dx) & mi) && !(((size_t)a.y | (size_t)a.dy) & mo)) return v;
+    }
+    return 1;
+}
+// resident form: the threads of a workgroup, 0 where a slab does not fit (or nothing is gained: V = 1)
+static int gn_resident(GnArgs& a, int v, int in, int out) {
+    if (v == 1) return 0;
+    const int es = in && out ? 2 : 4;
+    int cs = a.cg;
+    while (cs < a.C && (cs % v || cs * es < 64)) cs += a.cg;   // whole groups, whole vectors, 64 bytes of a pixel
+    if (cs > a.C) cs = a.C;
+    a.Cs = cs; a.slabs = (a.C + cs - 1) / cs; a.tw = cs / v;
+    if (cs % v || a.tw > 256) return 0;
+    for (int thr = 256; thr <= 1024; thr <<= 1) {
+        const int nr = thr / a.tw;
+        if ((long long)nr * GN_R >= a.HW) {
+            a.nr = nr < a.HW ? nr : (int)a.HW;
+            return ((long long)a.nr * cs + 4 * cs) * 4 <= 64 * 1024 ? thr : 0;
+        }
+    }
+    return 0;
 }
 static void gn_setup(GnArgs& a, int B, long long HW, int C, int G, int act, float eps, float* scratch) {
     a.B = B; a.HW = HW; a.C = C; a.Cp = (C + 3) & ~3; a.G = G; a.cg = C / G; a.act = act; a.eps = eps;
@@ -272,29 +520,70 @@ static void gn_setup(GnArgs& a, int B, long long HW, int C, int G, int act, floa
     a.part = scratch;
     a.cpart = scratch + ((((long long)B * a.nch * G * 2) + 3) & ~3LL);
 }
-template <typename TI, typename TO, int V>
-static void gn_fwd_launch(const GnArgs& a, hipStream_t s) {
-    const dim3 grid(a.nch, a.B);
+template <typename TI, typename TO, int V, int ACT>
+static void gn_fwd_launch(GnArgs& a, int thr, hipStream_t s) {
+    if constexpr (V > 1) {
+        if (thr) {
+            const size_t lds = sizeof(float) * ((size_t)a.nr * a.Cs + 3 * a.Cs);
+            const dim3 grid(a.B * a.slabs);
+            if (thr == 256) hipLaunchKernelGGL((gn_res_kernel<TI, TO, V, ACT, 256>), grid, dim3(256), lds, s, a);
+            else if (thr == 512) hipLaunchKernelGGL((gn_res_kernel<TI, TO, V, ACT, 512>), grid, dim3(512), lds, s, a);
+            else hipLaunchKernelGGL((gn_res_kernel<TI, TO, V, ACT, 1024>), grid, dim3(1024), lds, s, a);
+            return;
+        }
+    }
+    const dim3 grid(a.nch * a.B);
     hipLaunchKernelGGL((gn_stats_kernel<TI, V>), grid, dim3(256), sizeof(float) * (2 * a.Cp + 512 * V), s, a);
-    hipLaunchKernelGGL((gn_apply_kernel<TI, TO, V>), grid, dim3(256), sizeof(float) * 2 * a.G, s, a);
+    hipLaunchKernelGGL((gn_apply_kernel<TI, TO, V, ACT>), grid, dim3(256), sizeof(float) * 2 * a.G, s, a);
 }
-template <typename TI, typename TO, int V>
-static void gn_bwd_launch(const GnArgs& a, hipStream_t s) {
-    const dim3 grid(a.nch, a.B);
-    hipLaunchKernelGGL((gn_bwd_sums_kernel<TI, TO, V>), grid, dim3(256), sizeof(float) * (2 * a.Cp + 512 * V), s, a);
-    if (a.dx) hipLaunchKernelGGL((gn_bwd_apply_kernel<TI, TO, V>), grid, dim3(256), sizeof(float) * 2 * a.G, s, a);
+template <typename TI, typename TO, int V, int ACT>
+static void gn_bwd_launch(GnArgs& a, int thr, hipStream_t s, float* dgamma, float* dbeta) {
+    int rows = a.B * a.nch;
+    bool folded = !dgamma && !dbeta;
+    if constexpr (V > 1) {
+        if (thr) {
+            const size_t lds = sizeof(float) * ((size_t)a.nr * a.Cs + 4 * a.Cs);
+            const dim3 grid(a.B * a.slabs);
+            if (thr == 256) hipLaunchKernelGGL((gn_res_bwd_kernel<TI, TO, V, ACT, 256>), grid, dim3(256), lds, s, a);
+            else if (thr == 512) hipLaunchKernelGGL((gn_res_bwd_kernel<TI, TO, V, ACT, 512>), grid, dim3(512), lds, s, a);
+            else hipLaunchKernelGGL((gn_res_bwd_kernel<TI, TO, V, ACT, 1024>), grid, dim3(1024), lds, s, a);
+            rows = a.B;
+        }
+    }
+    RowsFoldArgs f = {};
+    if (!folded && rows <= L2I_FOLD_DIRECT) f = rows_fold_args4(a.cpart, rows, 2 * a.Cp, 1, dgamma, dbeta, nullptr, nullptr, a.Cp, a.C, 0, 0, nullptr, 2 * a.Cp);
+    if (!thr) {
+        hipLaunchKernelGGL((gn_bwd_sums_kernel<TI, TO, V, ACT>), dim3(rows), dim3(256), sizeof(float) * (2 * a.Cp + 512 * V), s, a);
+        if (a.dx) {
+            const size_t lds = sizeof(float) * 2 * a.G;
+            hipLaunchKernelGGL((gn_bwd_apply_kernel<TI, TO, V, ACT>), dim3(rows + (f.src ? f.nbx : 0)), dim3(256), lds < 4096 ? 4096 : lds, s, a, f);
+            folded = folded || f.src;
+        }
+    }
+    if (!folded) {
+        if (f.src) hipLaunchKernelGGL(rows_fold2_kernel, dim3(f.nbx), dim3(256), 0, s, f);
+        else {
+            float* tmp = a.cpart + (size_t)rows * 2 * a.Cp;
+            if (dgamma) rows_fold(a.cpart, rows, a.Cp, 1, dgamma, nullptr, a.C, 0, 0, tmp, s, nullptr, 2 * a.Cp);
+            if (dbeta) rows_fold(a.cpart + a.Cp, rows, a.Cp, 1, dbeta, nullptr, a.C, 0, 0, tmp, s, nullptr, 2 * a.Cp);
+        }
+    }
 }
-static bool gn_vec(const GnArgs& a, int in, int out) {
-    const size_t mi = in ? 7 : 15, mo = out ? 7 : 15;
-    return a.C % 4 == 0 && !(((size_t)a.x | (size_t)a.dx) & mi) && !(((size_t)a.y | (size_t)a.dy) & mo);
-}
-#define GN_DISPATCH(FN)                                                                                              \
+#define GN_ACTS(FN, TI, TO, V, ...)                                                                                  \
     do {                                                                                                             \
-        const bool vec = gn_vec(a, x_dtype, y_dtype);                                                                \
-        if (x_dtype == 0 && y_dtype == 0) { if (vec) FN<float, float, 4>(a, s); else FN<float, float, 1>(a, s); }     \
-        else if (x_dtype == 0) { if (vec) FN<float, bf16_t, 4>(a, s); else FN<float, bf16_t, 1>(a, s); }              \
-        else if (y_dtype == 0) { if (vec) FN<bf16_t, float, 4>(a, s); else FN<bf16_t, float, 1>(a, s); }              \
-        else { if (vec) FN<bf16_t, bf16_t, 4>(a, s); else FN<bf16_t, bf16_t, 1>(a, s); }                              \
+        if (act == 0) FN<TI, TO, V, 0>(__VA_ARGS__); else if (act == 1) FN<TI, TO, V, 1>(__VA_ARGS__); else FN<TI, TO, V, 2>(__VA_ARGS__); \
+    } while (0)
+#define GN_VECS(FN, TI, TO, ...)                                                                                     \
+    do {                                                                                                             \
+        if (vec == 8) GN_ACTS(FN, TI, TO, 8, __VA_ARGS__); else if (vec == 4) GN_ACTS(FN, TI, TO, 4, __VA_ARGS__); else GN_ACTS(FN, TI, TO, 1, __VA_ARGS__); \
+    } while (0)
+#define GN_DISPATCH(FN, ...)                                                                                         \
+    do {                                                                                                             \
+        const int vec = gn_vec(a, x_dtype, y_dtype), thr = gn_resident(a, vec, x_dtype, y_dtype);                    \
+        if (x_dtype == 0 && y_dtype == 0) GN_VECS(FN, float, float, a, thr, __VA_ARGS__);                            \
+        else if (x_dtype == 0) GN_VECS(FN, float, bf16_t, a, thr, __VA_ARGS__);                                      \
+        else if (y_dtype == 0) GN_VECS(FN, bf16_t, float, a, thr, __VA_ARGS__);                                      \
+        else GN_VECS(FN, bf16_t, bf16_t, a, thr, __VA_ARGS__);                                                       \
     } while (0)
 
 extern "C" int l2i_group_norm_fwd(const void* x, int x_dtype, const float* gamma, const float* beta, void* y, int y_dtype, float* mean, float* rstd,
@@ -306,7 +595,7 @@ extern "C" int l2i_group_norm_fwd(const void* x, int x_dtype, const float* gamma
     a.x = x; a.gamma = gamma; a.beta = beta; a.y = y; a.mean = mean; a.rstd = rstd;
     gn_setup(a, B, HW, C, G, act, eps, scratch);
     hipStream_t s = (hipStream_t)stream;
-    GN_DISPATCH(gn_fwd_launch);
+    GN_DISPATCH(gn_fwd_launch, s);
     return l2i_check_launch();
 }
 extern "C" int l2i_group_norm_bwd(const void* x, int x_dtype, const float* gamma, const float* beta, const float* mean, const float* rstd, const void* dy,
@@ -319,12 +608,6 @@ extern "C" int l2i_group_norm_bwd(const void* x, int x_dtype, const float* gamma
     a.x = x; a.gamma = gamma; a.beta = beta; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd); a.dy = dy; a.dx = dx;
     gn_setup(a, B, HW, C, G, act, 0.f, scratch);
     hipStream_t s = (hipStream_t)stream;
-    GN_DISPATCH(gn_bwd_launch);
-    if (dgamma || dbeta) {
-        const int rows = a.B * a.nch;
-        float* tmp = a.cpart + (size_t)rows * 2 * a.Cp;
-        if (dgamma) rows_fold(a.cpart, rows, a.Cp, 1, dgamma, nullptr, C, 0, 0, tmp, s, nullptr, 2 * a.Cp);
-        if (dbeta) rows_fold(a.cpart + a.Cp, rows, a.Cp, 1, dbeta, nullptr, C, 0, 0, tmp, s, nullptr, 2 * a.Cp);
-    }
+    GN_DISPATCH(gn_bwd_launch, s, dgamma, dbeta);
     return l2i_check_launch();
 }
