@@ -513,7 +513,7 @@ int l2i_cross_attention_bwd(const void* q, const void* k, const void* v, int dty
  * bwd: dw [V][D] (written, every row) = scale * sum of the dy rows of each token, in f32, in the order of their positions. */
 int l2i_embedding_fwd(const void* weight, int w_dtype, const long long* tokens, void* out, int out_dtype, long long n, int V, int D,
                       float scale, int padding_idx, void* stream);
-int l2i_embedding_bwd_scratch(long long n, int D, long long* floats);
+int l2i_embedding_bwd_scratch(long long n, int V, int D, long long* floats);
 int l2i_embedding_bwd(const long long* tokens, const void* dy, int dy_dtype, void* dw, int dw_dtype, long long n, int V, int D, float scale,
                       int padding_idx, float* scratch, long long scratch_floats, void* stream);
 

@@ -92,7 +92,7 @@ SIGNATURES = {
     "l2i_cross_attention_bwd": [_p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll,
                                 _ll, _ll, _f, _p, _ll, _p],
     "l2i_embedding_fwd": [_p, _i, _p, _p, _i, _ll, _i, _i, _f, _i, _p],
-    "l2i_embedding_bwd_scratch": [_ll, _i, _p],
+    "l2i_embedding_bwd_scratch": [_ll, _i, _i, _p],
     "l2i_embedding_bwd": [_p, _p, _i, _p, _i, _ll, _i, _i, _f, _i, _p, _ll, _p],
     "l2i_dropout": [_p, _i, _p, _p, _i, _p, _p, _ll, _ll, _f, _i, _p],
     "l2i_psp_stages_fwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _i, _f, _f, _p],

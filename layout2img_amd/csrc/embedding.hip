@@ -6,7 +6,7 @@
 // Lookup: bound by bytes (a row read, a row written). Gradient: V rows of D values are written, most of them zeros for a large
 // vocabulary, and n rows of dy are read once in the order of their tokens: (token, position) pairs are sorted stably, so that the rows
 // of a token are added in the order of their positions, by ONE writer -- no float atomics, the same bits on every run.
-#include "common.h"
+#include "vec.h"
 
 // ------------------------------------------------------------------------------------------------ lookup
 struct EmbArgs {
@@ -15,7 +15,7 @@ struct EmbArgs {
     int tx;   // lanes along a row: a power of two
 };
 
-template <typename TI, typename TO, bool VEC>
+template <typename TI, typename TO, int V>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(EmbArgs p) {
     const int tx = threadIdx.x & (p.tx - 1), ty = threadIdx.x / p.tx, rows = 256 / p.tx;
     const long long i = (long long)blockIdx.x * rows + ty;
@@ -24,55 +24,66 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(EmbArgs p) {
     const bool there = t >= 0 && t < p.V && t != p.pad;
     const TI* src = reinterpret_cast<const TI*>(p.w) + (size_t)(there ? t : 0) * p.D;
     TO* dst = reinterpret_cast<TO*>(p.out) + (size_t)i * p.D;
-    constexpr int E = VEC ? 4 : 1;
-    for (int c = tx * E; c < p.D; c += p.tx * E) {
-        if (VEC) {
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            if (there) Op4<TI>::load(src + c, v);
+    for (int c = tx * V; c < p.D; c += p.tx * V) {
+        Vec<TI, V> a;
+        float v[V];
+        a.load(src + c);
+        a.get(v);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = there ? v[e] * p.scale : 0.f;
-            Op4<TO>::store(dst + c, v);
-        } else {
-            dst[c] = OpT<TO>::from(there ? OpT<TI>::to(src[c]) * p.scale : 0.f);
-        }
+        for (int e = 0; e < V; ++e) v[e] = there ? v[e] * p.scale : 0.f;
+        vec_store<TO, V>(dst + c, v);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ sort
 // The rank of pair i is the number of pairs in front of it: those with a smaller key, and those with the same key at a smaller position.
-// Counting it directly is n^2 comparisons and one launch. A workgroup ranks 64 pairs: each of its four waves counts over a quarter of
-// every tile of 1024 keys that the workgroup stages in LDS.
+// Counting it directly is n^2 comparisons and one launch (29 us at 16384 pairs, where the radix sort's six launches take 35). A workgroup ranks 64 pairs: each of its NW waves counts over its share of every
+// tile of 256 NW keys that the workgroup stages in LDS (four waves up to 2048 pairs, sixteen above: four a SIMD hide the LDS reads).
+// The sort's first launch also marks every row of dW as absent (range[v] = (-1, 0)); the next kernel fills in the tokens that occur.
 __device__ __forceinline__ int emb_key(long long t, int V, int pad) { return (t >= 0 && t < V && t != pad) ? (int)t : V; }
+__device__ __forceinline__ void emb_clear(int2* range, int V) {
+    for (long long v = (long long)blockIdx.x * blockDim.x + threadIdx.x; v < V; v += (long long)gridDim.x * blockDim.x) range[v] = make_int2(-1, 0);
+}
 
-__global__ __launch_bounds__(256) void embedding_rank_kernel(const long long* __restrict__ tok, int n, int V, int pad, int* __restrict__ skey, int* __restrict__ spos) {
-    __shared__ __attribute__((aligned(16))) int keys[1024];
-    __shared__ int cnt[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
+template <int NW>
+__global__ __launch_bounds__(NW * 64) void embedding_rank_kernel(const long long* __restrict__ tok, int n, int V, int pad, int* __restrict__ skey,
+                                                                 int* __restrict__ spos, int2* __restrict__ range) {
+    __shared__ __attribute__((aligned(16))) int keys[256 * NW];
+    __shared__ int cnt[NW][64];
+    emb_clear(range, V);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i0 = blockIdx.x * 64, i = i0 + lane;
+    if (i0 >= n) return;   // (a workgroup that only clears)
     const int me = i < n ? emb_key(tok[i], V, pad) : 0x7fffffff;
-    int rank = 0;
-    for (int base = 0; base < n; base += 1024) {
+    int c0 = 0, c1 = 0, c2 = 0, c3 = 0;
+    for (int base = 0; base < n; base += 256 * NW) {
+        const int m = min(256 * NW, n - base), q4 = (m + 4 * NW - 1) / (4 * NW);   // groups of four keys a wave
         __syncthreads();
-        for (int k = threadIdx.x; k < 1024; k += 256) keys[k] = base + k < n ? emb_key(tok[base + k], V, pad) : 0x7fffffff;
+        for (int k = threadIdx.x; k < 4 * NW * q4; k += 64 * NW) keys[k] = k < m ? emb_key(tok[base + k], V, pad) : 0x7fffffff;
         __syncthreads();
-        const int b0 = base + wave * 256;
-        const int4* q = reinterpret_cast<const int4*>(keys + wave * 256);
-        if (b0 + 256 <= i - lane) {          // all in front of this workgroup's pairs: equal keys count
-            for (int k = 0; k < 64; ++k) { const int4 a = q[k]; rank += (a.x <= me) + (a.y <= me) + (a.z <= me) + (a.w <= me); }
-        } else if (b0 >= i - lane + 64) {    // all behind them
-            for (int k = 0; k < 64; ++k) { const int4 a = q[k]; rank += (a.x < me) + (a.y < me) + (a.z < me) + (a.w < me); }
+        const int b0 = base + wave * 4 * q4;
+        const int4* q = reinterpret_cast<const int4*>(keys + wave * 4 * q4);
+        if (b0 + 4 * q4 <= i0) {          // all in front of this workgroup's pairs: equal keys count
+#pragma unroll 8
+            for (int k = 0; k < q4; ++k) { const int4 a = q[k]; c0 += a.x <= me; c1 += a.y <= me; c2 += a.z <= me; c3 += a.w <= me; }
+        } else if (b0 >= i0 + 64) {       // all behind them
+#pragma unroll 8
+            for (int k = 0; k < q4; ++k) { const int4 a = q[k]; c0 += a.x < me; c1 += a.y < me; c2 += a.z < me; c3 += a.w < me; }
         } else {
-            for (int k = 0; k < 64; ++k) {
+#pragma unroll 4
+            for (int k = 0; k < q4; ++k) {
                 const int4 a = q[k];
                 const int j = b0 + 4 * k;
-                rank += (a.x < me || (a.x == me && j < i)) + (a.y < me || (a.y == me && j + 1 < i)) + (a.z < me || (a.z == me && j + 2 < i)) +
-                        (a.w < me || (a.w == me && j + 3 < i));
+                c0 += a.x < me || (a.x == me && j < i); c1 += a.y < me || (a.y == me && j + 1 < i);
+                c2 += a.z < me || (a.z == me && j + 2 < i); c3 += a.w < me || (a.w == me && j + 3 < i);
             }
         }
     }
-    cnt[wave][lane] = rank;
+    cnt[wave][lane] = (c0 + c1) + (c2 + c3);
     __syncthreads();
     if (wave == 0 && i < n) {
-        const int r = cnt[0][lane] + cnt[1][lane] + cnt[2][lane] + cnt[3][lane];
+        int r = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) r += cnt[w][lane];
         skey[r] = me;
         spos[r] = i;
     }
@@ -80,16 +91,17 @@ __global__ __launch_bounds__(256) void embedding_rank_kernel(const long long* __
 
 // Above EMB_RANK_MAX pairs: a stable radix sort, eight bits a pass from the lowest, three launches a pass. A workgroup owns 2048
 // consecutive pairs, a wave 512 of them; hist[digit][workgroup] counts, its exclusive scan is where each workgroup's pairs of a digit go.
-#define EMB_RANK_MAX 8192
+#define EMB_RANK_MAX 16384
 #define EMB_TILE 2048
 struct EmbSortArgs {
-    const long long* tok; const int* kin; const int* pin; int* kout; int* pout; int* hist;
+    const long long* tok; const int* kin; const int* pin; int* kout; int* pout; int* hist; int2* range;   // range: first pass only
     int n, V, pad, shift, nblk;
 };
 __device__ __forceinline__ int emb_sort_key(const EmbSortArgs& p, int i) { return p.tok ? emb_key(p.tok[i], p.V, p.pad) : p.kin[i]; }
 
 __global__ __launch_bounds__(256) void embedding_hist_kernel(EmbSortArgs p) {
     __shared__ int h[256];
+    if (p.range) emb_clear(p.range, p.V);
     h[threadIdx.x] = 0;
     __syncthreads();
     for (int k = threadIdx.x; k < EMB_TILE; k += 256) {
@@ -161,89 +173,131 @@ __global__ __launch_bounds__(256) void embedding_scatter_kernel(EmbSortArgs p) {
 }
 
 // ------------------------------------------------------------------------------------------------ gradient rows
-// The sorted pairs are cut in chunks of EMB_CHUNK. A chunk whose pairs all carry one token is added up by embedding_part_kernel (so that
-// a token which half of the batch carries is summed by many workgroups); embedding_rows_kernel owns the rows of dW, adds the partial rows
-// of the chunks inside a token's range and the single rows at its two ends, and writes the row -- zeros where the range is empty.
-#define EMB_CHUNK 32
-#define EMB_VROWS 16   // rows of dW per workgroup
+// The sorted pairs are cut in chunks. embedding_part_kernel walks a chunk: the tokens that lie in it as a whole are finished there (their
+// row of dW is written), the run that came in from the chunk before and the run that goes on in the next are left as partial rows, so that
+// every chunk costs the same however skewed the tokens are. embedding_rows_kernel owns the other rows of dW: it adds a token's partial
+// rows in chunk order, or writes zeros where the token does not occur.
+#define EMB_VROWS 8   // rows of dW per workgroup
 struct EmbBwdArgs {
-    const int* skey; const int* spos; const void* dy; float* part; void* dw;
-    int n, V, D; float scale;
-    int tx;
+    const int* skey; const int* spos; int2* range /* [V]: a token's pairs [x, y); x = -1: none */; const void* dy;
+    float* part /* [chunks][2][D]: come in, go on */; void* dw;
+    int n, V, D, chunk, nch; float scale;
+    int tx;   // lanes along a row: a power of two
 };
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void emb_add(const T* __restrict__ src, float (&s)[4]) {
-    if (VEC) {
-        float v[4];
-        Op4<T>::load(src, v);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += v[e];
-    } else {
-        s[0] += OpT<T>::to(src[0]);
-    }
-}
-
-template <typename TO, bool VEC>
+template <typename TO, typename TW, int V>
 __global__ __launch_bounds__(256) void embedding_part_kernel(EmbBwdArgs p) {
-    const int c0 = blockIdx.x, base = c0 * EMB_CHUNK;   // (whole chunks only)
-    const int k = p.skey[base];
-    if (k >= p.V || k != p.skey[base + EMB_CHUNK - 1]) return;
-    constexpr int E = VEC ? 4 : 1;
-    for (int c = threadIdx.x * E; c < p.D; c += 256 * E) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-        for (int j = 0; j < EMB_CHUNK; ++j) emb_add<TO, VEC>(reinterpret_cast<const TO*>(p.dy) + (size_t)p.spos[base + j] * p.D + c, s);
-        float* d = p.part + (size_t)c0 * p.D + c;
-        if (VEC) *reinterpret_cast<float4*>(d) = make_float4(s[0], s[1], s[2], s[3]);
-        else *d = s[0];
+    const int tx = threadIdx.x & (p.tx - 1), c = blockIdx.x * (256 / p.tx) + threadIdx.x / p.tx;
+    if (c >= p.nch) return;
+    const int base = c * p.chunk, m = min(p.chunk, p.n - base);
+    const int before = base > 0 ? p.skey[base - 1] : -1, behind = base + m < p.n ? p.skey[base + m] : -1;
+    const TO* dy = reinterpret_cast<const TO*>(p.dy);
+    for (int col = tx * V; col < p.D; col += p.tx * V) {
+        float s[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] = 0.f;
+        bool in = p.skey[base] == before;
+        int prev = before;
+        for (int j0 = 0; j0 < m; j0 += 8) {
+            Vec<TO, V> a[8];
+            int key[9];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int at = base + min(j0 + j, m - 1);
+                key[j] = p.skey[at];
+                a[j].load(dy + (size_t)p.spos[at] * p.D + col);
+            }
+            key[8] = j0 + 8 < m ? p.skey[base + j0 + 8] : -1;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (j0 + j >= m) break;
+                float v[V];
+                a[j].get(v);
+#pragma unroll
+                for (int e = 0; e < V; ++e) s[e] += v[e];
+                const bool last = j0 + j == m - 1;
+                const int next = last ? behind : key[j + 1];
+                if (tx == 0 && col == 0 && key[j] < p.V) {
+                    if (prev != key[j]) p.range[key[j]].x = base + j0 + j;
+                    if (next != key[j]) p.range[key[j]].y = base + j0 + j + 1;
+                }
+                prev = key[j];
+                if (next == key[j] && !last) continue;
+                // the run ends here, or the chunk does
+                if (key[j] < p.V) {
+                    if (in || next == key[j]) {
+                        vec_store<float, V>(p.part + ((size_t)c * 2 + (in ? 0 : 1)) * p.D + col, s);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < V; ++e) s[e] *= p.scale;
+                        vec_store<TW, V>(reinterpret_cast<TW*>(p.dw) + (size_t)key[j] * p.D + col, s);
+                    }
+                }
+                in = false;
+#pragma unroll
+                for (int e = 0; e < V; ++e) s[e] = 0.f;
+            }
+        }
     }
 }
 
-// the first sorted pair whose key is >= v: every lane of the wave probes, 64 places a step
-__device__ __forceinline__ int emb_lower_bound(const int* __restrict__ skey, int n, int v) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, hi = n;   // the answer lies in [lo, hi]
-    while (lo < hi) {
-        const int step = (hi - lo + 63) / 64;
-        const long long at = (long long)lo + (long long)step * (lane + 1) - 1;   // the last pair of the lane's piece
-        const bool below = at < hi && skey[at] < v;
-        const int full = __popcll(__ballot(below));                              // pieces that lie below v as a whole
-        lo = lo + full * step < hi ? lo + full * step : hi;
-        hi = lo + step - 1 < hi ? lo + step - 1 : hi;
-    }
-    return lo;
-}
-
-template <typename TO, typename TW, bool VEC>
+template <typename TW, int V>
 __global__ __launch_bounds__(256) void embedding_rows_kernel(EmbBwdArgs p) {
-    __shared__ int first[EMB_VROWS + 1];
-    const int v0 = blockIdx.x * EMB_VROWS, wave = threadIdx.x >> 6;
-    for (int r = wave; r <= EMB_VROWS; r += 4) {
-        const int a = emb_lower_bound(p.skey, p.n, min(v0 + r, p.V));
-        if ((threadIdx.x & 63) == 0) first[r] = a;
+    __shared__ int ra[EMB_VROWS], rk[EMB_VROWS];   // first chunk of a row and chunks it runs through; 0: absent, 1: finished
+    __shared__ float red[256 * V];
+    const int v0 = blockIdx.x * EMB_VROWS, nv = min(EMB_VROWS, p.V - v0);
+    if ((int)threadIdx.x < nv) {
+        const int2 a = p.n ? p.range[v0 + threadIdx.x] : make_int2(-1, 0);
+        ra[threadIdx.x] = a.x / p.chunk;
+        rk[threadIdx.x] = a.x < 0 ? 0 : (a.y - 1) / p.chunk - a.x / p.chunk + 1;
     }
     __syncthreads();
     const int tx = threadIdx.x & (p.tx - 1), ty = threadIdx.x / p.tx, nr = 256 / p.tx;
-    constexpr int E = VEC ? 4 : 1;
-    const TO* dy = reinterpret_cast<const TO*>(p.dy);
-    for (int r = ty; r < EMB_VROWS && v0 + r < p.V; r += nr) {
-        const int a = first[r], b = first[r + 1];
-        const int ca = (a + EMB_CHUNK - 1) / EMB_CHUNK, cb = b / EMB_CHUNK;   // whole chunks inside [a, b): [ca, cb)
-        TW* dst = reinterpret_cast<TW*>(p.dw) + (size_t)(v0 + r) * p.D;
-        for (int c = tx * E; c < p.D; c += p.tx * E) {
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
-            if (ca < cb) {
-                for (int j = a; j < ca * EMB_CHUNK; ++j) emb_add<TO, VEC>(dy + (size_t)p.spos[j] * p.D + c, s);
-                for (int j = ca; j < cb; ++j) emb_add<float, VEC>(p.part + (size_t)j * p.D + c, s);
-                for (int j = cb * EMB_CHUNK; j < b; ++j) emb_add<TO, VEC>(dy + (size_t)p.spos[j] * p.D + c, s);
-            } else {
-                for (int j = a; j < b; ++j) emb_add<TO, VEC>(dy + (size_t)p.spos[j] * p.D + c, s);
-            }
+    TW* dw = reinterpret_cast<TW*>(p.dw) + (size_t)v0 * p.D;
+    float s[V];
+    auto add = [&](int ca, int c, int j0, int k, int step) {   // partial rows j0, j0 + step, ... of k from chunk ca on: the first went on from its chunk, the others came in
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] *= p.scale;
-            if (VEC) Op4<TW>::store(dst + c, s);
-            else dst[c] = OpT<TW>::from(s[0]);
+        for (int e = 0; e < V; ++e) s[e] = 0.f;
+#pragma unroll 8
+        for (int j = j0; j < k; j += step) {
+            Vec<float, V> t;
+            float v[V];
+            t.load(p.part + ((size_t)(ca + j) * 2 + (j == 0 ? 1 : 0)) * p.D + c);
+            t.get(v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e] += v[e];
+        }
+    };
+    auto put = [&](int r, int c) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] *= p.scale;
+        vec_store<TW, V>(dw + (size_t)r * p.D + c, s);
+    };
+    bool many = false;
+    for (int r = 0; r < nv; ++r) many = many || rk[r] > 32;
+    for (int r = ty; r < nv; r += nr) {
+        const int k = rk[r];
+        if (k == 1 || k > 32) continue;
+        for (int c = tx * V; c < p.D; c += p.tx * V) { add(ra[r], c, 0, k, 1); put(r, c); }
+    }
+    if (!many) return;
+    for (int r = 0; r < nv; ++r) {   // a token of many chunks: the whole workgroup, every nr-th partial row a lane, joined in lane order
+        const int k = rk[r];
+        if (k <= 32) continue;
+        for (int c0 = 0; c0 < p.D; c0 += p.tx * V) {
+            const int c = c0 + tx * V;
+            if (c < p.D) add(ra[r], c, ty, k, nr);
+            __syncthreads();
+            if (c < p.D)
+#pragma unroll
+                for (int e = 0; e < V; ++e) red[e * 256 + threadIdx.x] = s[e];
+            __syncthreads();
+            if (ty == 0 && c < p.D) {
+                for (int j = 1; j < nr && j < k; ++j)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) s[e] += red[e * 256 + j * p.tx + tx];
+                put(r, c);
+            }
         }
     }
 }
@@ -256,11 +310,12 @@ static int emb_lanes(int D, int E) {
 }
 template <typename TI, typename TO>
 static void emb_fwd_launch(EmbArgs a, hipStream_t s) {
-    const bool vec = a.D % 4 == 0 && !((size_t)a.w & (4 * sizeof(TI) - 1)) && !((size_t)a.out & (4 * sizeof(TO) - 1));
-    a.tx = emb_lanes(a.D, vec ? 4 : 1);
-    const unsigned grid = (unsigned)((a.n + 256 / a.tx - 1) / (256 / a.tx));
-    if (vec) hipLaunchKernelGGL((embedding_fwd_kernel<TI, TO, true>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((embedding_fwd_kernel<TI, TO, false>), dim3(grid), dim3(256), 0, s, a);
+    const int v = vec_width(a.D, a.w, sizeof(TI) == 2, a.out, sizeof(TO) == 2);
+    a.tx = emb_lanes(a.D, v);
+    const dim3 grid((unsigned)((a.n + 256 / a.tx - 1) / (256 / a.tx)));
+    if (v == 8) hipLaunchKernelGGL((embedding_fwd_kernel<TI, TO, 8>), grid, dim3(256), 0, s, a);
+    else if (v == 4) hipLaunchKernelGGL((embedding_fwd_kernel<TI, TO, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((embedding_fwd_kernel<TI, TO, 1>), grid, dim3(256), 0, s, a);
 }
 extern "C" int l2i_embedding_fwd(const void* weight, int w_dtype, const long long* tokens, void* out, int out_dtype, long long n, int V, int D,
                                  float scale, int padding_idx, void* stream) {
@@ -275,38 +330,41 @@ extern "C" int l2i_embedding_fwd(const void* weight, int w_dtype, const long lon
     return l2i_check_launch();
 }
 
-// scratch, in ints: sorted keys and positions [n] each, a second pair of them and the histogram when the radix sort runs, then the partial rows
+// scratch, in ints: sorted keys and positions [n] each, the tokens' ranges [V][2], a second pair of them and the histogram when the radix sort runs, then the partial rows
+static int emb_chunk(long long n) { return n <= 2048 ? 8 : n <= 65536 ? 32 : 128; }   // few pairs: more workgroups; many: fewer partial rows
 static long long emb_al(long long ints) { return (ints + 3) & ~3LL; }
 static long long emb_hist_ints(long long n) { return 256 * ((n + EMB_TILE - 1) / EMB_TILE); }
-extern "C" int l2i_embedding_bwd_scratch(long long n, int D, long long* floats) {
-    if (!floats || n < 0 || n > 0x7fffffffLL || D < 1) return L2I_ERR_ARG;
-    *floats = emb_al(n) * (n > EMB_RANK_MAX ? 4 : 2) + (n > EMB_RANK_MAX ? emb_al(emb_hist_ints(n)) : 0) + (n / EMB_CHUNK) * (long long)D;
+extern "C" int l2i_embedding_bwd_scratch(long long n, int V, int D, long long* floats) {
+    if (!floats || n < 0 || n > 0x7fffffffLL || V < 1 || V > 0x7fffff00 || D < 1 || D > 65536) return L2I_ERR_ARG;
+    *floats = emb_al(2LL * V) + emb_al(n) * (n > EMB_RANK_MAX ? 4 : 2) + (n > EMB_RANK_MAX ? emb_al(emb_hist_ints(n)) : 0) + (n + emb_chunk(n) - 1) / emb_chunk(n) * 2 * (long long)D;
     return L2I_OK;
 }
 
+template <typename TO, typename TW, int V>
+static void emb_bwd_kernels(EmbBwdArgs a, hipStream_t s) {
+    a.tx = emb_lanes(a.D, V);
+    const unsigned grid = (unsigned)((a.V + EMB_VROWS - 1) / EMB_VROWS), per = 256 / a.tx;
+    if (a.n) hipLaunchKernelGGL((embedding_part_kernel<TO, TW, V>), dim3((a.nch + per - 1) / per), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((embedding_rows_kernel<TW, V>), dim3(grid), dim3(256), 0, s, a);
+}
 template <typename TO, typename TW>
-static void emb_bwd_launch(EmbBwdArgs a, hipStream_t s) {
-    const bool vec = a.D % 4 == 0 && !((size_t)a.dy & (4 * sizeof(TO) - 1)) && !((size_t)a.dw & (4 * sizeof(TW) - 1));
-    a.tx = emb_lanes(a.D, vec ? 4 : 1);
-    const unsigned grid = (unsigned)((a.V + EMB_VROWS - 1) / EMB_VROWS), nch = (unsigned)(a.n / EMB_CHUNK);
-    if (vec) {
-        if (nch) hipLaunchKernelGGL((embedding_part_kernel<TO, true>), dim3(nch), dim3(256), 0, s, a);
-        hipLaunchKernelGGL((embedding_rows_kernel<TO, TW, true>), dim3(grid), dim3(256), 0, s, a);
-    } else {
-        if (nch) hipLaunchKernelGGL((embedding_part_kernel<TO, false>), dim3(nch), dim3(256), 0, s, a);
-        hipLaunchKernelGGL((embedding_rows_kernel<TO, TW, false>), dim3(grid), dim3(256), 0, s, a);
-    }
+static void emb_bwd_launch(const EmbBwdArgs& a, hipStream_t s) {
+    const int v = vec_width(a.D, a.dy, sizeof(TO) == 2, a.dw, sizeof(TW) == 2);
+    if (v == 8) emb_bwd_kernels<TO, TW, 8>(a, s);
+    else if (v == 4) emb_bwd_kernels<TO, TW, 4>(a, s);
+    else emb_bwd_kernels<TO, TW, 1>(a, s);
 }
 extern "C" int l2i_embedding_bwd(const long long* tokens, const void* dy, int dy_dtype, void* dw, int dw_dtype, long long n, int V, int D, float scale,
                                  int padding_idx, float* scratch, long long scratch_floats, void* stream) {
     if (n < 0 || n > 0x7fffffffLL - EMB_TILE || V < 1 || V > 0x7fffff00 || D < 1 || D > 65536 || (dy_dtype | dw_dtype) & ~1) return L2I_ERR_ARG;
     if (!dw || (n && (!tokens || !dy || !scratch || ((size_t)scratch & 15)))) return L2I_ERR_ARG;
     long long need = 0;
-    if (l2i_embedding_bwd_scratch(n, D, &need) != L2I_OK || (n && scratch_floats < need)) return L2I_ERR_ARG;
+    if (l2i_embedding_bwd_scratch(n, V, D, &need) != L2I_OK || (n && scratch_floats < need)) return L2I_ERR_ARG;
     hipStream_t s = (hipStream_t)stream;
     int* skey = reinterpret_cast<int*>(scratch);
     int* spos = skey + emb_al(n);
-    int* end = spos + emb_al(n);
+    int2* range = reinterpret_cast<int2*>(spos + emb_al(n));
+    int* end = reinterpret_cast<int*>(range) + emb_al(2LL * V);
     if (n > EMB_RANK_MAX) {
         int *k2 = end, *p2 = k2 + emb_al(n), *hist = p2 + emb_al(n);
         end = hist + emb_al(emb_hist_ints(n));
@@ -320,16 +378,21 @@ extern "C" int l2i_embedding_bwd(const long long* tokens, const void* dy, int dy
             a.tok = q == 0 ? tokens : nullptr;
             a.kin = to_first ? k2 : skey; a.pin = q == 0 ? nullptr : (to_first ? p2 : spos);
             a.kout = to_first ? skey : k2; a.pout = to_first ? spos : p2;
-            a.shift = 8 * q;
+            a.shift = 8 * q; a.range = q == 0 ? range : nullptr;
             hipLaunchKernelGGL(embedding_hist_kernel, dim3(a.nblk), dim3(256), 0, s, a);
             hipLaunchKernelGGL(embedding_scan_kernel, dim3(1), dim3(1024), 0, s, hist, 256 * a.nblk);
             hipLaunchKernelGGL(embedding_scatter_kernel, dim3(a.nblk), dim3(256), 0, s, a);
         }
     } else if (n) {
-        hipLaunchKernelGGL(embedding_rank_kernel, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, s, tokens, (int)n, V, padding_idx, skey, spos);
+        int grid = (int)((n + 63) / 64);
+        const int clear = V / 8192 < 256 ? V / 8192 : 256;
+        if (grid < clear) grid = clear;
+        if (n <= 2048) hipLaunchKernelGGL((embedding_rank_kernel<4>), dim3(grid), dim3(256), 0, s, tokens, (int)n, V, padding_idx, skey, spos, range);
+        else hipLaunchKernelGGL((embedding_rank_kernel<16>), dim3(grid), dim3(1024), 0, s, tokens, (int)n, V, padding_idx, skey, spos, range);
     }
     EmbBwdArgs b;
-    b.skey = skey; b.spos = spos; b.dy = dy; b.part = reinterpret_cast<float*>(end); b.dw = dw; b.n = (int)n; b.V = V; b.D = D; b.scale = scale; b.tx = 0;
+    b.skey = skey; b.spos = spos; b.range = range; b.dy = dy; b.part = reinterpret_cast<float*>(end); b.dw = dw; b.n = (int)n; b.V = V; b.D = D; b.scale = scale; b.tx = 0;
+    b.chunk = emb_chunk(n); b.nch = (int)((n + b.chunk - 1) / b.chunk);
     if (dy_dtype == 0) { if (dw_dtype == 0) emb_bwd_launch<float, float>(b, s); else emb_bwd_launch<float, bf16_t>(b, s); }
     else { if (dw_dtype == 0) emb_bwd_launch<bf16_t, float>(b, s); else emb_bwd_launch<bf16_t, bf16_t>(b, s); }
     return l2i_check_launch();

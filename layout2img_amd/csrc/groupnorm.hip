@@ -14,7 +14,7 @@
 //     XCD that read it, so that L2 and the Infinity Cache still hold what is read first.
 // In the backward pass the sums are S1, S2 per group and rows of (sum dz xh | sum dz) per channel, which the ordered fold adds into dgamma / dbeta (in
 // workgroups of their own at the end of the second launch). Statistics are f32; nothing is accumulated by atomics.
-#include "common.h"
+#include "vec.h"
 
 struct GnArgs {
     const void* x; const float* gamma; const float* beta; void* y;
@@ -41,39 +41,6 @@ template <int ACT> __device__ __forceinline__ float gn_dact(float z, float dy) {
     if (ACT == 1) return z > 0.f ? dy : 0.f;
     if (ACT == 2) { const float s = gn_sig(z); return dy * fmaf(z, fmaf(-s, s, s), s); }
     return dy;
-}
-
-// V consecutive values as they lie in memory
-template <typename T, int V> struct GnVec {
-    static constexpr int N = V * (int)sizeof(T) / 16;   // 16-byte pieces; 0: one 8-byte piece (bf16 x 4); V = 1: one value
-    uint4 r[N ? N : 1];
-    __device__ __forceinline__ void load(const T* p) {
-        if constexpr (V == 1) r[0].x = sizeof(T) == 4 ? __float_as_uint((float)OpT<T>::to(p[0])) : (unsigned)__float_as_uint(OpT<T>::to(p[0]));
-        else if constexpr (N == 0) { const uint2 u = *reinterpret_cast<const uint2*>(p); r[0].x = u.x; r[0].y = u.y; }
-        else
-#pragma unroll
-            for (int i = 0; i < N; ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
-    }
-    __device__ __forceinline__ void get(float (&v)[V]) const {
-        if constexpr (V == 1) v[0] = __uint_as_float(r[0].x);
-        else {
-            const unsigned* w = reinterpret_cast<const unsigned*>(r);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                if constexpr (sizeof(T) == 4) v[e] = __uint_as_float(w[e]);
-                else v[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
-            }
-        }
-    }
-};
-template <typename T, int V> __device__ __forceinline__ void gn_store(T* p, const float (&v)[V]) {
-    if constexpr (V == 1) p[0] = OpT<T>::from(v[0]);
-    else if constexpr (sizeof(T) == 2 && V == 8) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(f2bf2(v[0], v[1]), f2bf2(v[2], v[3]), f2bf2(v[4], v[5]), f2bf2(v[6], v[7]));
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i += 4) { const float q[4] = {v[i], v[i + 1], v[i + 2], v[i + 3]}; Op4<T>::store(p + i, q); }
-    }
 }
 
 // f(e, channel c + e, its group): one division for the V channels of a thread
@@ -122,7 +89,7 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) { s[e] = 0.f; q[e] = 0.f; k[e] = 0.f; }
         if (on) {
-            GnVec<T, V> a[4];
+            Vec<T, V> a[4];
             a[0].load(x + (size_t)r0 * p.C + c);
             a[0].get(k);
 #define GN_L(K, R) a[K].load(x + (size_t)(R) * p.C + c);
@@ -204,9 +171,9 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs p) {
             a_[e] = gr[g] * (p.gamma ? p.gamma[ce] : 1.f);
             o[e] = p.beta ? p.beta[ce] : 0.f;
         });
-        GnVec<TI, V> a[4];
+        Vec<TI, V> a[4];
 #define GN_U(K, R) { float v[V]; a[K].get(v); _Pragma("unroll") for (int e = 0; e < V; ++e) v[e] = gn_act<ACT>(fmaf(v[e] - m[e], a_[e], o[e])); \
-                     gn_store<TO, V>(y + (size_t)(R) * p.C + c, v); }
+                     vec_store<TO, V>(y + (size_t)(R) * p.C + c, v); }
         GN_ROWS(GN_L, GN_U);
 #undef GN_U
 #undef GN_L
@@ -233,8 +200,8 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs p) {
                 m[e] = p.mean[(size_t)b * p.G + g];
                 A[e] = p.rstd[(size_t)b * p.G + g] * (p.gamma ? p.gamma[ce] : 1.f); be[e] = p.beta ? p.beta[ce] : 0.f;
             });
-            GnVec<TI, V> a[4];
-            GnVec<TO, V> d[4];
+            Vec<TI, V> a[4];
+            Vec<TO, V> d[4];
 #define GN_U(K, R) { float v[V], w[V]; a[K].get(v); d[K].get(w); _Pragma("unroll") for (int e = 0; e < V; ++e) { \
                      const float dd = v[e] - m[e], dz = gn_dact<ACT>(fmaf(dd, A[e], be[e]), w[e]); sa[e] = fmaf(dz, dd, sa[e]); sb[e] += dz; } }
             GN_ROWS(GN_L2, GN_U);
@@ -301,11 +268,11 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(GnArgs p, RowsFoldArg
             A[e] = rs * (p.gamma ? p.gamma[ce] : 1.f); be[e] = p.beta ? p.beta[ce] : 0.f;
             s1[e] = rs * g1[g]; s2[e] = rs * rs * g2[g];
         });
-        GnVec<TI, V> a[4];
-        GnVec<TO, V> d[4];
+        Vec<TI, V> a[4];
+        Vec<TO, V> d[4];
 #define GN_U(K, R) { float v[V], w[V]; a[K].get(v); d[K].get(w); _Pragma("unroll") for (int e = 0; e < V; ++e) { \
                      const float dd = v[e] - m[e], dz = gn_dact<ACT>(fmaf(dd, A[e], be[e]), w[e]); \
-                     v[e] = fmaf(A[e], dz, -fmaf(dd, s2[e], s1[e])); } gn_store<TI, V>(dx + (size_t)(R) * p.C + c, v); }
+                     v[e] = fmaf(A[e], dz, -fmaf(dd, s2[e], s1[e])); } vec_store<TI, V>(dx + (size_t)(R) * p.C + c, v); }
         GN_ROWS(GN_L2, GN_U);
 #undef GN_U
     }
@@ -348,7 +315,7 @@ __global__ __launch_bounds__(THR) void gn_res_kernel(GnArgs p) {
     float *red = sm, *chan = sm + p.nr * p.Cs, *gres = chan + p.Cs;
     GN_RES(V)
     const TI* x = reinterpret_cast<const TI*>(p.x) + base;
-    GnVec<TI, V> a[GN_R];
+    Vec<TI, V> a[GN_R];
     float s[V], v[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) s[e] = 0.f;
@@ -400,7 +367,7 @@ __global__ __launch_bounds__(THR) void gn_res_kernel(GnArgs p) {
             a[k].get(v);
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] = gn_act<ACT>(fmaf(v[e] - m[e], r[e], s[e]));
-            gn_store<TO, V>(y + k * step, v);
+            vec_store<TO, V>(y + k * step, v);
         }
 }
 
@@ -411,8 +378,8 @@ __global__ __launch_bounds__(THR) void gn_res_bwd_kernel(GnArgs p) {
     GN_RES(V)
     const TI* x = reinterpret_cast<const TI*>(p.x) + base;
     const TO* dy = reinterpret_cast<const TO*>(p.dy) + base;
-    GnVec<TI, V> a[GN_R];
-    GnVec<TO, V> d[GN_R];
+    Vec<TI, V> a[GN_R];
+    Vec<TO, V> d[GN_R];
 #pragma unroll
     for (int k = 0; k < GN_R; ++k) if (on && ty + k * p.nr < p.HW) { a[k].load(x + k * step); d[k].load(dy + k * step); }
     float m[V], rs[V], A[V], be[V], sa[V], sb[V], v[V], w[V];
@@ -462,7 +429,7 @@ __global__ __launch_bounds__(THR) void gn_res_bwd_kernel(GnArgs p) {
                 const float dd = v[e] - m[e], dz = gn_dact<ACT>(fmaf(dd, A[e], be[e]), w[e]);
                 v[e] = fmaf(A[e], dz, -fmaf(dd, sb[e], sa[e]));
             }
-            gn_store<TI, V>(dx + k * step, v);
+            vec_store<TI, V>(dx + k * step, v);
         }
 }
 
@@ -486,13 +453,6 @@ extern "C" int l2i_group_norm_scratch(int B, long long HW, int C, int G, int bwd
     const long long rows = (long long)B * nch;
     *floats = ((rows * G * 2 + 3) & ~3LL) + (bwd ? rows * 2 * Cp + (rows > L2I_FOLD_DIRECT ? rows_fold_tmp_floats((int)rows, (int)Cp, 1) : 0) : 0);
     return L2I_OK;
-}
-static int gn_vec(const GnArgs& a, int in, int out) {   // values a vector: 8, 4 or 1, by the channel count and the addresses
-    for (int v = in && out ? 8 : 4; v >= 4; v >>= 1) {
-        const size_t mi = (in ? 2 * v : 16) - 1, mo = (out ? 2 * v : 16) - 1;
-        if (a.C % v == 0 && !(((size_t)a.x | (size_t)a.dx) & mi) && !(((size_t)a.y | (size_t)a.dy) & mo)) return v;
-    }
-    return 1;
 }
 // resident form: the threads of a workgroup, 0 where a slab does not fit (or nothing is gained: V = 1)
 static int gn_resident(GnArgs& a, int v, int in, int out) {
@@ -579,7 +539,7 @@ static void gn_bwd_launch(GnArgs& a, int thr, hipStream_t s, float* dgamma, floa
     } while (0)
 #define GN_DISPATCH(FN, ...)                                                                                         \
     do {                                                                                                             \
-        const int vec = gn_vec(a, x_dtype, y_dtype), thr = gn_resident(a, vec, x_dtype, y_dtype);                    \
+        const int vec = vec_width(a.C, (const void*)((size_t)a.x | (size_t)a.dx), x_dtype, (const void*)((size_t)a.y | (size_t)a.dy), y_dtype), thr = gn_resident(a, vec, x_dtype, y_dtype);                    \
         if (x_dtype == 0 && y_dtype == 0) GN_VECS(FN, float, float, a, thr, __VA_ARGS__);                            \
         else if (x_dtype == 0) GN_VECS(FN, float, bf16_t, a, thr, __VA_ARGS__);                                      \
         else if (y_dtype == 0) GN_VECS(FN, bf16_t, float, a, thr, __VA_ARGS__);                                      \

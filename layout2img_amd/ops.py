@@ -2253,7 +2253,7 @@ class EmbeddingFn(Function):
         (V, D), dtype, scale, padding_idx = ctx.cfg
         dy = dy.contiguous()
         dw = torch.empty((V, D), dtype=dtype, device=dy.device)
-        ws, wp, wn = _scratch(dy.device, "l2i_embedding_bwd_scratch", tokens.numel(), D)
+        ws, wp, wn = _scratch(dy.device, "l2i_embedding_bwd_scratch", tokens.numel(), V, D)
         _lib.call("l2i_embedding_bwd", tokens.data_ptr(), dy.data_ptr(), _code(dy.dtype), dw.data_ptr(), _code(dtype), tokens.numel(), V, D, scale,
                   padding_idx, wp, wn, _stream())
         return dw, None, None, None, None
