@@ -13,7 +13,11 @@
 // movement, because the sum over keys may run in any order as long as V is read in the same one: bf16 V^T comes from LDS by
 // the transposing read (ds_read_b64_tr_b16), f32 V by plain reads. Probabilities enter P V (and dS the gradient products) rounded to bf16 in
 // the bf16 kernels (relative 2^-9, as small as the rounding of the inputs); maxima, sums, S, D and all accumulators are f32.
-#include "common.h"
+//
+// What bounds it: with 64 values a head, a wave's 32 x 64 scores cost 16 MFMAs (512 cycles) and 32 exponentials a lane with what surrounds
+// them (about 900 cycles), so the vector unit; tiles therefore come to LDS by LDS-DMA (no registers, no instructions of the waves), two
+// buffers deep, and the rescaling of the accumulators waits until the maximum has grown by 2^8.
+#include "igemm.h"
 #include <type_traits>
 
 typedef __attribute__((ext_vector_type(8))) __bf16 b16x8_t;
@@ -28,18 +32,17 @@ struct XaArgs {
     const int* len; const unsigned char* mask;
     long long qb, ql, qh, kb, kl, kh, vb, vl, vh, mb, mq;   // strides in elements (mask: bytes; mq = 0: one mask row for all queries)
     int B, Lq, Lk, Hk, G, D, R, ns;
-    float scale, c;                           // c = scale log2(e)
+    float scale, c;                           // c = |scale| log2(e); a negative scale turns the sign of one operand of S
 };
 
 // ---- LDS tiles: rows of CH 16-byte chunks, chunk c of row r at place c ^ f(r): 16 rows at one chunk (row reads) and 4 rows x 4 chunks
 // (transposing reads) each fall on 16 different 16-byte bank groups
-template <int CH> __device__ __forceinline__ int xa_at(int row, int chunk) {
-    int f;
-    if constexpr (CH == 4) f = (row >> 2) & 3;
-    else if constexpr (CH == 8) f = (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
-    else f = ((row & 3) << 2) | ((row >> 2) & 3);
-    return (row * CH + (chunk ^ f)) * 16;
+template <int CH> __device__ __forceinline__ int xa_swz(int row) {
+    if constexpr (CH == 4) return (row >> 2) & 3;
+    else if constexpr (CH == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    else return ((row & 3) << 2) | ((row >> 2) & 3);
 }
+template <int CH> __device__ __forceinline__ int xa_at(int row, int chunk) { return (row * CH + (chunk ^ xa_swz<CH>(row))) * 16; }
 
 // ---- acc[a's row][b's row] += a . b over one step of dims (bf16: 16, f32: 8): a, b = the lane's 16-byte chunk 2 s + lane / 32 of its row
 __device__ __forceinline__ void xa_dot(f32x16_t& acc, const uint4& a, const uint4& b, bf16_t) {
@@ -50,6 +53,14 @@ __device__ __forceinline__ void xa_dot(f32x16_t& acc, const uint4& a, const uint
     acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), acc, 0, 0, 0);
     acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), acc, 0, 0, 0);
     acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), acc, 0, 0, 0);
+}
+// acc[tile row row0 + ..][b's row] = sum over all dims
+template <typename T, int CH> __device__ __forceinline__ void xa_rows_dot(f32x16_t& acc, const char* tile, int row0, const uint4 (&b)[CH / 2]) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int s = 0; s < CH / 2; ++s) xa_dot(acc, *reinterpret_cast<const uint4*>(tile + xa_at<CH>(row0 + (lane & 31), 2 * s + h)), b[s], T());
 }
 
 // ---- acc[d][lane] += sum over 32 tile rows i of tile[row0 + i][d] p_i(lane); p: an accumulator (register r of a lane = row 8 (r / 4) + 4 (lane / 32) + r % 4)
@@ -102,35 +113,39 @@ __device__ __forceinline__ int xa_len(const XaArgs& p, int b) {
     return n < 0 ? 0 : (n < p.Lk ? n : p.Lk);
 }
 
-// a tile of NR rows x CH chunks on its way to LDS through registers; row(i) -> pointer to the row's first element or null (zeros)
-template <typename T, int CH, int NR> struct XaStage {
-    static constexpr int N = NR * CH / 256;
-    uint4 r[N];
-    template <typename F> __device__ __forceinline__ void load(int D, F row) {
+// ---- tiles of NR rows x CH chunks to LDS by LDS-DMA. Thread i of TH fills places i, i + TH, ...: place (row, pos) takes chunk pos ^ f(row) of
+// its row; what does not exist (rows that `rows` refuses, chunks behind D) is read out of range, which writes zeros.
+#define XA_OOB 0x80000000u
+#define XA_SPAN 0x7fffffffu   // bytes a tile's rows may span: checked on the host
+template <typename T, int CH, int NR, int TH> struct XaDma {
+    static constexpr int N = NR * CH / TH;
+    unsigned off[N];   // byte offset of the place's chunk from the tile's first row
+    __device__ __forceinline__ static int row(int i) { return (int)((threadIdx.x % TH + TH * i) / CH); }
+    __device__ __forceinline__ static int chunk(int i) { return (int)((threadIdx.x % TH + TH * i) % CH) ^ xa_swz<CH>(row(i)); }
+    __device__ __forceinline__ void init(long long stride, int D) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int idx = threadIdx.x + 256 * i, chunk = idx % CH;
-            const T* src = row(idx / CH);
-            r[i] = make_uint4(0, 0, 0, 0);
-            if (src && chunk * (16 / (int)sizeof(T)) < D) r[i] = *reinterpret_cast<const uint4*>(src + chunk * (16 / (int)sizeof(T)));
-        }
+        for (int i = 0; i < N; ++i) off[i] = chunk(i) * 16 < D * (int)sizeof(T) ? (unsigned)(row(i) * stride * (int)sizeof(T)) + chunk(i) * 16 : XA_OOB;
     }
-    __device__ __forceinline__ void store(char* tile) const {
+    template <typename F> __device__ __forceinline__ void issue(const T* base, unsigned lds, F rows) const {   // base, lds: the same for all lanes
+        const u32x4_t r = make_rsrc(base, XA_SPAN);
+        const unsigned at = lds + (TH == 64 ? 0 : (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024));
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int idx = threadIdx.x + 256 * i;
-            *reinterpret_cast<uint4*>(tile + xa_at<CH>(idx / CH, idx % CH)) = r[i];
-        }
+        for (int i = 0; i < N; ++i) buf_load_lds16(r, rows(row(i)) ? off[i] : XA_OOB, at + i * TH * 16);
     }
+    __device__ __forceinline__ void issue(const T* base, unsigned lds) const { issue(base, lds, [](int) { return true; }); }
 };
-// the lane's chunks of a row as a product operand
-template <typename T, int CH> __device__ __forceinline__ void xa_row_frag(uint4 (&f)[CH / 2], const T* src, int D) {
+template <int N> __device__ __forceinline__ void xa_wait_dma() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// the lane's chunks of a row as a product operand; neg: with the other sign
+template <typename T, int CH> __device__ __forceinline__ void xa_row_frag(uint4 (&f)[CH / 2], const T* src, int D, bool neg = false) {
     const int h = (threadIdx.x & 63) >> 5;
+    const unsigned flip = neg ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
 #pragma unroll
     for (int s = 0; s < CH / 2; ++s) {
         const int e = (2 * s + h) * (16 / (int)sizeof(T));
         f[s] = make_uint4(0, 0, 0, 0);
         if (src && e < D) f[s] = *reinterpret_cast<const uint4*>(src + e);
+        f[s].x ^= flip; f[s].y ^= flip; f[s].z ^= flip; f[s].w ^= flip;
     }
 }
 // live bits of four consecutive keys j .. j + 3 of a mask row of Lk bytes (none is read outside the row)
@@ -162,105 +177,157 @@ __device__ __forceinline__ unsigned xa_live(unsigned kbits, const unsigned char*
     return m;
 }
 __device__ __forceinline__ float xa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }   // (below 2^-126: 0)
+// x where bit e of live is set, else `other` (both by bits: two instructions)
+__device__ __forceinline__ float xa_pick(unsigned live, int e, float x, unsigned other) {
+    const unsigned m = (unsigned)((int)(live << (31 - e)) >> 31);
+    return __uint_as_float((__float_as_uint(x) & m) | (other & ~m));
+}
+#define XA_NINF 0xff800000u
 // Between a matrix instruction and the first read of its result no branch may join: the compiler's wait count there follows one of the joining
 // paths only. Live bits are therefore made in front of the products, masked and unmasked tiles are separate straight bodies, and behind a
 // loop of products this wait stands.
 __device__ __forceinline__ void xa_settle() { asm volatile("s_nop 15\n\ts_nop 7" ::: "memory"); }
 
+// the states of one (image, state head): where they are and which of them live
+template <typename T> struct XaStates {
+    const T *k, *v;
+    const unsigned char* mb;   // the image's mask or null
+    int len; bool kmask;       // kmask: one mask row for all queries
+    __device__ __forceinline__ XaStates(const XaArgs& p, int b, int hk) {
+        k = reinterpret_cast<const T*>(p.k) + b * p.kb + hk * p.kh;
+        v = reinterpret_cast<const T*>(p.v) + b * p.vb + hk * p.vh;
+        mb = p.mask ? p.mask + b * p.mb : nullptr;
+        len = xa_len(p, b);
+        kmask = mb && p.mq == 0;
+    }
+    __device__ __forceinline__ bool live(int j) const { return j < len && (!kmask || mb[j]); }
+};
+
 // ------------------------------------------------------------------------------------------------ forward
-// WQ = 4: four waves x 32 rows, every wave reads all 64 keys of a tile. WQ = 1: 32 rows (a single token, a few), the four waves each take
-// 32 of the tile's 128 keys with a softmax of their own and are joined at the end. ns > 1: the tiles of states are cut in ns ranges,
-// joined by xa_join_kernel.
+// WQ = 4: four waves x 32 rows share tiles of 64 keys (one barrier a tile). WQ = 1: 32 rows (a single token, a few), every wave has tiles of 32
+// keys of its own in its own part of LDS, no barrier in the loop, and a softmax of its own; the four are joined at the end. ns > 1: the tiles of states
+// are cut in ns ranges, joined by xa_join_kernel.
+template <typename T, int DP, int WQ> struct XaFwdTile {
+    static constexpr int CH = DP * (int)sizeof(T) / 16, KT = WQ == 4 ? 64 : 32, TH = WQ == 4 ? 256 : 64;
+    static constexpr int BYTES = KT * CH * 16;                                    // of K; V behind it
+    static constexpr int NBUF = 4 * BYTES * (WQ == 4 ? 1 : 4) <= 128 * 1024 ? 2 : 1;
+    static constexpr int LDS = 2 * BYTES * NBUF * (WQ == 4 ? 1 : 4);
+    static constexpr int TOTAL = WQ == 4 ? LDS : (LDS > 512 * DP ? LDS : 512 * DP) + 1024;
+};
 template <typename T, int DP, int WQ>
-__global__ __launch_bounds__(256) void xa_fwd_kernel(XaArgs p, int nqt, int total) {
-    constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, KW = WQ == 4 ? 64 : 32, KT = KW * (4 / WQ), QT = 32 * WQ;
+__global__ __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : (sizeof(T) == 4 ? 2 : 3)) void xa_fwd_kernel(XaArgs p, int nqt, int total) {
+    using Tile = XaFwdTile<T, DP, WQ>;
+    constexpr int CH = Tile::CH, ND = DP / 32, S = CH / 2, KT = Tile::KT, TH = Tile::TH, QT = 32 * WQ, NBUF = Tile::NBUF, STEP = WQ == 4 ? 1 : 4;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    char *ks = smem, *vs = smem + KT * CH * 16;
     const int id = xa_tile_id(total);
     if (id >= total) return;
     const int bh = id / (nqt * p.ns), rest = id - bh * nqt * p.ns, split = rest / nqt, qt = rest - split * nqt;
     const int b = bh / p.Hk, hk = bh - b * p.Hk;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int r = qt * QT + (WQ == 4 ? wave * 32 : 0) + (lane & 31);
     const int iq = r < p.R ? xa_row_query(p, r) : 0, head = hk * p.G + (r < p.R ? r - iq * p.G : 0);
-    const int len = xa_len(p, b), nt = (len + KT - 1) / KT, per = (nt + p.ns - 1) / p.ns;
-    const int t0 = split * per, t1 = min(nt, t0 + per);
+    const XaStates<T> st(p, b, hk);
+    const int nt = (st.len + KT - 1) / KT, per = (nt + p.ns - 1) / p.ns;
+    const int t0 = split * per + (WQ == 4 ? 0 : wave), t1 = min(nt, split * per + per);
+    const unsigned char* mrow = st.mb && !st.kmask ? st.mb + (long long)iq * p.mq : nullptr;   // (null or not: the same for the whole launch)
+    char* tiles = smem + (WQ == 4 ? 0 : wave * 2 * Tile::BYTES * NBUF);
+    const unsigned lds = lds_addr_of(tiles);
+    XaDma<T, CH, KT, TH> dk, dv;
+    dk.init(p.kl, p.D);
+    dv.init(p.vl, p.D);
+    auto issue = [&](int t, int buf) {
+        const T *kp = st.k + (long long)t * KT * p.kl, *vp = st.v + (long long)t * KT * p.vl;
+        const unsigned at = lds + buf * 2 * Tile::BYTES;
+        if (st.kmask || (t + 1) * KT > st.len) {
+            auto rows = [&](int i) { return st.live(t * KT + i); };
+            dk.issue(kp, at, rows);
+            dv.issue(vp, at + Tile::BYTES, rows);
+        } else {
+            dk.issue(kp, at);
+            dv.issue(vp, at + Tile::BYTES);
+        }
+    };
+    if (t0 < t1) issue(t0, 0);
     uint4 qf[S];
-    xa_row_frag<T, CH>(qf, r < p.R ? reinterpret_cast<const T*>(p.q) + b * p.qb + (long long)iq * p.ql + head * p.qh : nullptr, p.D);
-    const T* kp = reinterpret_cast<const T*>(p.k) + b * p.kb + hk * p.kh;
-    const T* vp = reinterpret_cast<const T*>(p.v) + b * p.vb + hk * p.vh;
-    const unsigned char* mb = p.mask ? p.mask + b * p.mb : nullptr;
-    const bool kmask = mb && p.mq == 0;
-    const unsigned char* mrow = mb && !kmask ? mb + (long long)iq * p.mq : nullptr;   // (null or not: the same for the whole launch)
-    auto krow = [&](int t) { return [=](int i) -> const T* { const int j = t * KT + i; return j < len && (!kmask || mb[j]) ? kp + j * p.kl : nullptr; }; };
-    auto vrow = [&](int t) { return [=](int i) -> const T* { const int j = t * KT + i; return j < len && (!kmask || mb[j]) ? vp + j * p.vl : nullptr; }; };
-    XaStage<T, CH, KT> sk, sv;
+    xa_row_frag<T, CH>(qf, r < p.R ? reinterpret_cast<const T*>(p.q) + b * p.qb + (long long)iq * p.ql + head * p.qh : nullptr, p.D, p.scale < 0.f);
     f32x16_t oacc[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) oacc[d][e] = 0.f;
     float m = -INFINITY, l = 0.f;
-    if (t0 < t1) { sk.load(p.D, krow(t0)); sv.load(p.D, vrow(t0)); }
-    for (int t = t0; t < t1; ++t) {
-        __syncthreads();
-        sk.store(ks); sv.store(vs);
-        __syncthreads();
-        if (t + 1 < t1) { sk.load(p.D, krow(t + 1)); sv.load(p.D, vrow(t + 1)); }
-        const int row0 = WQ == 4 ? 0 : wave * 32, j0 = t * KT + row0;
-        const int jl = j0 + lane;
-        const unsigned long long kbits = __ballot(lane < KW && jl < len && (!kmask || mb[jl]));
-        auto body = [&](auto masked) {
-            f32x16_t sc[KW / 32];
-            unsigned live[KW / 32];
-            if constexpr (decltype(masked)::value) {
+    int buf = 0;
+    for (int t = t0; t < t1; t += STEP) {
+        const int jl = t * KT + lane;
+        const unsigned long long kbits = __ballot(lane < KT && st.live(jl));
+        const bool all = !mrow && kbits == (KT == 64 ? ~0ull : 0xffffffffull);
+        unsigned live[KT / 32];
+        if (!all)
 #pragma unroll
-                for (int kb = 0; kb < KW / 32; ++kb) live[kb] = xa_live((unsigned)(kbits >> (32 * kb)), mrow, j0 + 32 * kb, p.Lk);
-            }
+            for (int kb = 0; kb < KT / 32; ++kb) live[kb] = xa_live((unsigned)(kbits >> (32 * kb)), mrow, t * KT + 32 * kb, p.Lk);
+        if (WQ == 4) {
+            xa_wait_dma<0>();
+            __syncthreads();
+            if (t + STEP < t1) issue(t + STEP, buf ^ 1);
+        } else if (NBUF == 2 && t + STEP < t1) {
+            issue(t + STEP, buf ^ 1);
+            xa_wait_dma<2 * XaDma<T, CH, KT, TH>::N>();
+        } else {
+            xa_wait_dma<0>();
+        }
+        const char *ks = tiles + buf * 2 * Tile::BYTES, *vs = ks + Tile::BYTES;
+        auto body = [&](auto masked) {
+            f32x16_t sc[KT / 32];
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb) xa_rows_dot<T, CH>(sc[kb], ks, kb * 32, qf);
             float tm = -INFINITY;
 #pragma unroll
-            for (int kb = 0; kb < KW / 32; ++kb) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) sc[kb][e] = 0.f;
-#pragma unroll
-                for (int s = 0; s < S; ++s) xa_dot(sc[kb], *reinterpret_cast<const uint4*>(ks + xa_at<CH>(row0 + kb * 32 + (lane & 31), 2 * s + h)), qf[s], T());
-            }
-#pragma unroll
-            for (int kb = 0; kb < KW / 32; ++kb)
+            for (int kb = 0; kb < KT / 32; ++kb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    sc[kb][e] *= p.c;
-                    if constexpr (decltype(masked)::value) sc[kb][e] = (live[kb] >> e) & 1 ? sc[kb][e] : -INFINITY;
+                    if constexpr (decltype(masked)::value) sc[kb][e] = xa_pick(live[kb], e, sc[kb][e], XA_NINF);
                     tm = fmaxf(tm, sc[kb][e]);
                 }
             tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
-            const float mn = fmaxf(m, tm), ref = mn == -INFINITY ? 0.f : mn, al = xa_exp2(m - ref);
-            m = mn;
-            l *= al;
+            tm = tm == -INFINITY ? tm : tm * p.c;   // (c may be 0)
+            if (__ballot(tm > m + 8.f || (m == -INFINITY && tm > m))) {   // the reference moves only when it has to: scores stay below 2^8
+                const float mn = fmaxf(m, tm), al = xa_exp2(m - (mn == -INFINITY ? 0.f : mn));
+                m = mn;
+                l *= al;
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
+                for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) oacc[d][e] *= al;
+                    for (int e = 0; e < 16; ++e) oacc[d][e] *= al;
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int kb = 0; kb < KW / 32; ++kb) {
+            for (int kb = 0; kb < KT / 32; ++kb) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) { sc[kb][e] = xa_exp2(sc[kb][e] - ref); l += sc[kb][e]; }
-                xa_tdot<CH, ND>(oacc, vs, row0 + kb * 32, sc[kb], T());
+                for (int e = 0; e < 16; ++e) {
+                    float x = fmaf(sc[kb][e], p.c, -ref);
+                    if constexpr (decltype(masked)::value) x = xa_pick(live[kb], e, x, XA_NINF);
+                    sc[kb][e] = xa_exp2(x);
+                    l += sc[kb][e];
+                }
+                xa_tdot<CH, ND>(oacc, vs, kb * 32, sc[kb], T());
             }
         };
-        if (!mrow && kbits == (KW == 64 ? ~0ull : 0xffffffffull)) body(std::false_type());
+        if (all) body(std::false_type());
         else body(std::true_type());
+        if (NBUF == 2) buf ^= 1;
+        else if (WQ == 4) __syncthreads();
+        if (NBUF == 1 && WQ == 1 && t + STEP < t1) issue(t + STEP, 0);
     }
     xa_settle();
     l += __shfl_xor(l, 32, 64);
     if constexpr (WQ == 1) {   // the four waves' softmaxes, in wave order
-        float* ob = reinterpret_cast<float*>(smem);                       // [4][DP][32]
-        float* st = reinterpret_cast<float*>(smem + 2 * KT * CH * 16);    // [4][32] max, [4][32] sum
+        float* ob = reinterpret_cast<float*>(smem);                                  // [4][DP][32]
+        float* stt = reinterpret_cast<float*>(smem + Tile::TOTAL - 1024);            // [4][32] max, [4][32] sum
         __syncthreads();
-        if (lane < 32) { st[wave * 32 + lane] = m; st[128 + wave * 32 + lane] = l; }
+        if (lane < 32) { stt[wave * 32 + lane] = m; stt[128 + wave * 32 + lane] = l; }
         __syncthreads();
         const int n = lane & 31;
-        const float mn = fmaxf(fmaxf(st[n], st[32 + n]), fmaxf(st[64 + n], st[96 + n])), ref = mn == -INFINITY ? 0.f : mn;
+        const float mn = fmaxf(fmaxf(stt[n], stt[32 + n]), fmaxf(stt[64 + n], stt[96 + n])), ref = mn == -INFINITY ? 0.f : mn;
         const float al = xa_exp2(m - ref);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -268,7 +335,7 @@ __global__ __launch_bounds__(256) void xa_fwd_kernel(XaArgs p, int nqt, int tota
             for (int e = 0; e < 16; ++e) ob[(wave * DP + d * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + n] = oacc[d][e] * al;
         l = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) l += st[128 + w * 32 + n] * xa_exp2(st[w * 32 + n] - ref);
+        for (int w = 0; w < 4; ++w) l += stt[128 + w * 32 + n] * xa_exp2(stt[w * 32 + n] - ref);
         m = mn;
         __syncthreads();
         if (wave >= ND) return;   // wave d joins block d of the dims
@@ -337,10 +404,9 @@ __global__ __launch_bounds__(256) void xa_join_kernel(XaArgs p) {
 // ------------------------------------------------------------------------------------------------ backward: dq (and D)
 // Four waves x 32 rows, tiles of 64 keys, as the forward; also leaves D for the kernel behind it.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void xa_dq_kernel(XaArgs p, int nqt, int total) {
-    constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, KT = 64;
+__global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_dq_kernel(XaArgs p, int nqt, int total) {
+    constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, KT = 64, BYTES = KT * CH * 16;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    char *ks = smem, *vs = smem + KT * CH * 16;
     const int id = xa_tile_id(total);
     if (id >= total) return;
     const int bh = id / nqt, qt = id - bh * nqt, b = bh / p.Hk, hk = bh - b * p.Hk;
@@ -348,10 +414,29 @@ __global__ __launch_bounds__(256) void xa_dq_kernel(XaArgs p, int nqt, int total
     const int r = qt * 128 + wave * 32 + (lane & 31);
     const bool on = r < p.R;
     const int iq = on ? xa_row_query(p, r) : 0, head = hk * p.G + (on ? r - iq * p.G : 0);
-    const int len = xa_len(p, b), nt = (len + KT - 1) / KT;
+    const XaStates<T> st(p, b, hk);
+    const int nt = p.dq ? (st.len + KT - 1) / KT : 0;
     const size_t orow = (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D;
+    const unsigned char* mrow = st.mb && !st.kmask ? st.mb + (long long)iq * p.mq : nullptr;
+    const unsigned lds = lds_addr_of(smem);
+    XaDma<T, CH, KT, 256> dk, dv;
+    dk.init(p.kl, p.D);
+    dv.init(p.vl, p.D);
+    auto issue = [&](int t, int buf) {
+        const T *kp = st.k + (long long)t * KT * p.kl, *vp = st.v + (long long)t * KT * p.vl;
+        const unsigned at = lds + buf * 2 * BYTES;
+        if (st.kmask || (t + 1) * KT > st.len) {
+            auto rows = [&](int i) { return st.live(t * KT + i); };
+            dk.issue(kp, at, rows);
+            dv.issue(vp, at + BYTES, rows);
+        } else {
+            dk.issue(kp, at);
+            dv.issue(vp, at + BYTES);
+        }
+    };
+    if (nt) issue(0, 0);
     uint4 qf[S], gf[S];
-    xa_row_frag<T, CH>(qf, on ? reinterpret_cast<const T*>(p.q) + b * p.qb + (long long)iq * p.ql + head * p.qh : nullptr, p.D);
+    xa_row_frag<T, CH>(qf, on ? reinterpret_cast<const T*>(p.q) + b * p.qb + (long long)iq * p.ql + head * p.qh : nullptr, p.D, p.scale < 0.f);
     xa_row_frag<T, CH>(gf, on ? reinterpret_cast<const T*>(p.g) + orow : nullptr, p.D);
     float dl = 0.f;
     {
@@ -369,55 +454,42 @@ __global__ __launch_bounds__(256) void xa_dq_kernel(XaArgs p, int nqt, int total
     }
     const float ls = on ? p.lse[(size_t)bh * p.R + r] : INFINITY;
     if (on && h == 0) p.delta[(size_t)bh * p.R + r] = dl;
-    if (!p.dq) return;   // (uniform over the launch)
-    const T* kp = reinterpret_cast<const T*>(p.k) + b * p.kb + hk * p.kh;
-    const T* vp = reinterpret_cast<const T*>(p.v) + b * p.vb + hk * p.vh;
-    const unsigned char* mb = p.mask ? p.mask + b * p.mb : nullptr;
-    const bool kmask = mb && p.mq == 0;
-    const unsigned char* mrow = mb && !kmask ? mb + (long long)iq * p.mq : nullptr;   // (null or not: the same for the whole launch)
-    auto krow = [&](int t) { return [=](int i) -> const T* { const int j = t * KT + i; return j < len && (!kmask || mb[j]) ? kp + j * p.kl : nullptr; }; };
-    auto vrow = [&](int t) { return [=](int i) -> const T* { const int j = t * KT + i; return j < len && (!kmask || mb[j]) ? vp + j * p.vl : nullptr; }; };
-    XaStage<T, CH, KT> sk, sv;
     f32x16_t acc[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
-    if (nt) { sk.load(p.D, krow(0)); sv.load(p.D, vrow(0)); }
     for (int t = 0; t < nt; ++t) {
-        __syncthreads();
-        sk.store(ks); sv.store(vs);
-        __syncthreads();
-        if (t + 1 < nt) { sk.load(p.D, krow(t + 1)); sv.load(p.D, vrow(t + 1)); }
         const int jl = t * KT + lane;
-        const unsigned long long kbits = __ballot(jl < len && (!kmask || mb[jl]));
+        const unsigned long long kbits = __ballot(st.live(jl));
+        const bool all = !mrow && kbits == ~0ull;
+        unsigned live[2];
+        if (!all)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) live[kb] = xa_live((unsigned)(kbits >> (32 * kb)), mrow, t * KT + 32 * kb, p.Lk);
+        xa_wait_dma<0>();
+        __syncthreads();
+        if (t + 1 < nt) issue(t + 1, (t + 1) & 1);
+        const char *ks = smem + (t & 1) * 2 * BYTES, *vs = ks + BYTES;
         auto body = [&](auto masked) {
-#pragma unroll
+#pragma unroll 1
             for (int kb = 0; kb < 2; ++kb) {
-                unsigned live = 0;
-                if constexpr (decltype(masked)::value) live = xa_live((unsigned)(kbits >> (32 * kb)), mrow, t * KT + 32 * kb, p.Lk);
                 f32x16_t sc, dp;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) { sc[e] = 0.f; dp[e] = 0.f; }
-#pragma unroll
-                for (int s = 0; s < S; ++s) {
-                    const int at = xa_at<CH>(kb * 32 + (lane & 31), 2 * s + h);
-                    xa_dot(sc, *reinterpret_cast<const uint4*>(ks + at), qf[s], T());
-                    xa_dot(dp, *reinterpret_cast<const uint4*>(vs + at), gf[s], T());
-                }
+                xa_rows_dot<T, CH>(sc, ks, kb * 32, qf);
+                xa_rows_dot<T, CH>(dp, vs, kb * 32, gf);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    sc[e] = xa_exp2(sc[e] * p.c - ls) * (dp[e] - dl);
-                    if constexpr (decltype(masked)::value) sc[e] = (live >> e) & 1 ? sc[e] : 0.f;
+                    sc[e] = xa_exp2(fmaf(sc[e], p.c, -ls)) * (dp[e] - dl);
+                    if constexpr (decltype(masked)::value) sc[e] = xa_pick(kb ? live[1] : live[0], e, sc[e], 0u);
                 }
                 xa_tdot<CH, ND>(acc, ks, kb * 32, sc, T());
             }
         };
-        if (!mrow && kbits == ~0ull) body(std::false_type());
+        if (all) body(std::false_type());
         else body(std::true_type());
     }
     xa_settle();
-    if (!on) return;
+    if (!on || !p.dq) return;
     T* o = reinterpret_cast<T*>(p.dq) + orow;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -430,128 +502,127 @@ __global__ __launch_bounds__(256) void xa_dq_kernel(XaArgs p, int nqt, int total
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
-// A lane owns one key. WK = 4: four waves x 32 keys, every wave reads all 64 rows of a tile of queries. WK = 1: 32 keys, the waves each
-// take 32 of the tile's 128 rows and are joined at the end. ns > 1: the rows are cut in ns ranges, added in range order by xa_fold_kernel.
-template <typename T, int DP, int WK>
-__global__ __launch_bounds__(256) void xa_dkv_kernel(XaArgs p, int nkt, int total) {
-    constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, RW = WK == 4 ? 64 : 32, RT = RW * (4 / WK);
+// A lane owns one key: four waves x 32 keys, every wave reads all 64 rows of a tile of queries and their gradients. ns > 1: the rows are cut in ns
+// ranges, added in range order by xa_fold_kernel.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_dkv_kernel(XaArgs p, int nkt, int total) {
+    constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, RT = 64, BYTES = RT * CH * 16;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    char *qs = smem, *gs = smem + RT * CH * 16;
-    float* lss = reinterpret_cast<float*>(smem + 2 * RT * CH * 16);   // [RT] lse, [RT] D, [RT] query of the row
-    float* dls = lss + RT;
-    int* iqs = reinterpret_cast<int*>(dls + RT);
+    float* rowv = reinterpret_cast<float*>(smem + 4 * BYTES);   // two of: [RT] lse, [RT] D, [RT] query of the row
     const int id = xa_tile_id(total);
     if (id >= total) return;
     const int bh = id / (nkt * p.ns), rest = id - bh * nkt * p.ns, kt = rest / p.ns, split = rest - kt * p.ns;
     const int b = bh / p.Hk, hk = bh - b * p.Hk;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int key = kt * 32 * WK + (WK == 4 ? wave * 32 : 0) + (lane & 31);
-    const int len = xa_len(p, b);
-    const unsigned char* mb = p.mask ? p.mask + b * p.mb : nullptr;
-    const bool kmask = mb && p.mq == 0, klive = key < len && (!kmask || mb[key]);
-    const bool qmask = mb && !kmask;
-    const int nt = kt * 32 * WK < len ? (p.R + RT - 1) / RT : 0, per = (nt + p.ns - 1) / p.ns;
+    const int key = kt * 128 + wave * 32 + (lane & 31);
+    const XaStates<T> st(p, b, hk);
+    const bool klive = st.live(key), qmask = st.mb && !st.kmask;
+    const int nt = kt * 128 < st.len ? (p.R + RT - 1) / RT : 0, per = (nt + p.ns - 1) / p.ns;
     const int t0 = split * per, t1 = min(nt, t0 + per);
-    uint4 kf[S], vf[S];
-    xa_row_frag<T, CH>(kf, klive ? reinterpret_cast<const T*>(p.k) + b * p.kb + hk * p.kh + key * p.kl : nullptr, p.D);
-    xa_row_frag<T, CH>(vf, klive ? reinterpret_cast<const T*>(p.v) + b * p.vb + hk * p.vh + key * p.vl : nullptr, p.D);
+    const unsigned lds = lds_addr_of(smem);
     const T* qp = reinterpret_cast<const T*>(p.q) + b * p.qb + hk * p.G * p.qh;
     const T* gp = reinterpret_cast<const T*>(p.g) + ((size_t)b * p.Lq * p.Hk + hk) * p.G * p.D;
-    auto qrow = [&](int t) { return [=](int i) -> const T* {
-        const int r = t * RT + i;
-        if (r >= p.R) return nullptr;
-        const int iq = xa_row_query(p, r);
-        return qp + (long long)iq * p.ql + (r - iq * p.G) * p.qh; }; };
-    auto grow = [&](int t) { return [=](int i) -> const T* {
-        const int r = t * RT + i;
-        if (r >= p.R) return nullptr;
-        const int iq = xa_row_query(p, r);
-        return gp + ((size_t)iq * p.Hk * p.G + (r - iq * p.G)) * p.D; }; };
-    XaStage<T, CH, RT> sq, sg;
+    const long long gl = (long long)p.Hk * p.G * p.D;   // a query's step in g
+    XaDma<T, CH, RT, 256> dq, dg;
+    dq.init(p.ql, p.D);
+    dg.init(gl, p.D);
+    const float rG = 1.f / (float)p.G;
+    float nls = INFINITY, ndl = 0.f;
+    int niq = 0;
+    auto issue = [&](int t, int buf) {
+        const int r0 = t * RT, left = p.R - r0;
+        const unsigned at = lds + buf * 2 * BYTES;
+        if (p.G == 1) {
+            const T *a = qp + (long long)r0 * p.ql, *c = gp + (long long)r0 * gl;
+            if (left >= RT) { dq.issue(a, at); dg.issue(c, at + BYTES); }
+            else {
+                auto rows = [&](int i) { return i < left; };
+                dq.issue(a, at, rows);
+                dg.issue(c, at + BYTES, rows);
+            }
+        } else {   // row r0 + i = head (g0 + i) % G of query iq0 + (g0 + i) / G
+            const int iq0 = (int)((unsigned)r0 / (unsigned)p.G), g0 = r0 - iq0 * p.G;
+            XaDma<T, CH, RT, 256> a, c;
+#pragma unroll
+            for (int i = 0; i < a.N; ++i) {
+                const int rr = g0 + a.row(i), di = (int)(((float)rr + 0.5f) * rG), gg = rr - di * p.G, ck = a.chunk(i) * 16;
+                const bool ok = ck < p.D * (int)sizeof(T) && a.row(i) < left;
+                a.off[i] = ok ? (unsigned)((di * p.ql + gg * p.qh) * (int)sizeof(T)) + ck : XA_OOB;
+                c.off[i] = ok ? (unsigned)((di * gl + gg * p.D) * (int)sizeof(T)) + ck : XA_OOB;
+            }
+            a.issue(qp + (long long)iq0 * p.ql, at);
+            c.issue(gp + (long long)iq0 * gl, at + BYTES);
+        }
+        if (threadIdx.x < RT) {
+            const bool on = (int)threadIdx.x < left;
+            const size_t row = (size_t)bh * p.R + r0 + (on ? threadIdx.x : 0);
+            nls = on ? p.lse[row] : INFINITY;   // (a row behind the last: probabilities 0)
+            ndl = on ? p.delta[row] : 0.f;
+            niq = on ? xa_row_query(p, r0 + threadIdx.x) : 0;
+        }
+    };
+    if (t0 < t1) issue(t0, 0);
+    uint4 kf[S], vf[S];
+    xa_row_frag<T, CH>(kf, klive ? st.k + key * p.kl : nullptr, p.D, p.scale < 0.f);
+    xa_row_frag<T, CH>(vf, klive ? st.v + key * p.vl : nullptr, p.D);
     f32x16_t dk[ND], dv[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) { dk[d][e] = 0.f; dv[d][e] = 0.f; }
-    if (t0 < t1) { sq.load(p.D, qrow(t0)); sg.load(p.D, grow(t0)); }
+    const bool all = !qmask && __ballot(klive) == ~0ull;
+    int buf = 0;
     for (int t = t0; t < t1; ++t) {
+        float* rv = rowv + buf * 3 * RT;
+        if (threadIdx.x < RT) { rv[threadIdx.x] = nls; rv[RT + threadIdx.x] = ndl; reinterpret_cast<int*>(rv)[2 * RT + threadIdx.x] = niq; }
+        xa_wait_dma<0>();
         __syncthreads();
-        sq.store(qs); sg.store(gs);
-        if (threadIdx.x < RT) {
-            const int r = t * RT + threadIdx.x;
-            const bool on = r < p.R;
-            lss[threadIdx.x] = on ? p.lse[(size_t)bh * p.R + r] : INFINITY;   // (a row behind the last: probabilities 0)
-            dls[threadIdx.x] = on ? p.delta[(size_t)bh * p.R + r] : 0.f;
-            iqs[threadIdx.x] = on ? xa_row_query(p, r) : 0;
-        }
-        __syncthreads();
-        if (t + 1 < t1) { sq.load(p.D, qrow(t + 1)); sg.load(p.D, grow(t + 1)); }
+        if (t + 1 < t1) issue(t + 1, buf ^ 1);
+        const char *qs = smem + buf * 2 * BYTES, *gs = qs + BYTES;
         auto body = [&](auto masked) {
-#pragma unroll
-            for (int rb = 0; rb < RW / 32; ++rb) {
-                const int row0 = (WK == 4 ? 0 : wave * 32) + rb * 32;
-                unsigned live = klive ? 0xffffu : 0u;
+#pragma unroll 1
+            for (int row0 = 0; row0 < RT; row0 += 32) {
+                unsigned live = 0;
                 if constexpr (decltype(masked)::value) {
+                    live = klive ? 0xffffu : 0u;
                     if (qmask && klive) {
                         live = 0;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) live |= (mb[(long long)iqs[row0 + 8 * (e >> 2) + 4 * h + (e & 3)] * p.mq + key] != 0 ? 1u : 0u) << e;
+                        for (int e = 0; e < 16; ++e)
+                            live |= (st.mb[(long long)reinterpret_cast<const int*>(rv)[2 * RT + row0 + 8 * (e >> 2) + 4 * h + (e & 3)] * p.mq + key] != 0 ? 1u : 0u) << e;
                     }
                 }
                 f32x16_t pr, ds;
+                xa_rows_dot<T, CH>(pr, qs, row0, kf);
+                xa_rows_dot<T, CH>(ds, gs, row0, vf);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) { pr[e] = 0.f; ds[e] = 0.f; }
+                for (int a = 0; a < 4; ++a) {
+                    const float4 ls = *reinterpret_cast<const float4*>(rv + row0 + 8 * a + 4 * h), dl = *reinterpret_cast<const float4*>(rv + RT + row0 + 8 * a + 4 * h);
+                    const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dd[4] = {dl.x, dl.y, dl.z, dl.w};
 #pragma unroll
-                for (int s = 0; s < S; ++s) {
-                    const int at = xa_at<CH>(row0 + (lane & 31), 2 * s + h);
-                    xa_dot(pr, *reinterpret_cast<const uint4*>(qs + at), kf[s], T());
-                    xa_dot(ds, *reinterpret_cast<const uint4*>(gs + at), vf[s], T());
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int row = row0 + 8 * (e >> 2) + 4 * h + (e & 3);
-                    pr[e] = xa_exp2(pr[e] * p.c - lss[row]);
-                    ds[e] = pr[e] * (ds[e] - dls[row]);
-                    if constexpr (decltype(masked)::value) {
-                        pr[e] = (live >> e) & 1 ? pr[e] : 0.f;
-                        ds[e] = (live >> e) & 1 ? ds[e] : 0.f;
+                    for (int i = 0; i < 4; ++i) {
+                        const int e = 4 * a + i;
+                        pr[e] = xa_exp2(fmaf(pr[e], p.c, -lv[i]));
+                        if constexpr (decltype(masked)::value) pr[e] = xa_pick(live, e, pr[e], 0u);
+                        ds[e] = pr[e] * (ds[e] - dd[i]);
+                        if constexpr (decltype(masked)::value) ds[e] = xa_pick(live, e, ds[e], 0u);
                     }
                 }
                 xa_tdot<CH, ND>(dv, gs, row0, pr, T());
                 xa_tdot<CH, ND>(dk, qs, row0, ds, T());
             }
         };
-        if (!qmask && __ballot(klive) == ~0ull) body(std::false_type());
+        if (all) body(std::false_type());
         else body(std::true_type());
+        buf ^= 1;
     }
     xa_settle();
-    if constexpr (WK == 1) {   // the four waves' rows, in wave order; wave d keeps block d of the dims
-        float* ob = reinterpret_cast<float*>(smem);   // [4][DP][32]
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            __syncthreads();
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) ob[(wave * DP + d * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + (lane & 31)] = which ? dv[d][e] : dk[d][e];
-            __syncthreads();
-            if (wave < ND) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int dd = wave * 32 + 8 * (e >> 2) + 4 * h + (e & 3), n = lane & 31;
-                    const float s = (ob[dd * 32 + n] + ob[(DP + dd) * 32 + n]) + (ob[(2 * DP + dd) * 32 + n] + ob[(3 * DP + dd) * 32 + n]);
-                    if (which) dv[0][e] = s; else dk[0][e] = s;
-                }
-            }
-        }
-        if (wave >= ND) return;
-    }
     if (key >= p.Lk) return;
 #pragma unroll
-    for (int d = 0; d < (WK == 1 ? 1 : ND); ++d)
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
-            const int dd = (WK == 1 ? wave : d) * 32 + 8 * a + 4 * h;
+            const int dd = d * 32 + 8 * a + 4 * h;
             if (dd >= p.D) continue;
             const float vk[4] = {dk[d][4 * a] * p.scale, dk[d][4 * a + 1] * p.scale, dk[d][4 * a + 2] * p.scale, dk[d][4 * a + 3] * p.scale};
             const float vv[4] = {dv[d][4 * a], dv[d][4 * a + 1], dv[d][4 * a + 2], dv[d][4 * a + 3]};
@@ -592,17 +663,15 @@ static int xa_splits(long long tiles, long long nt) {
     if (ns > 64) ns = 64;
     return ns < 1 ? 1 : (int)ns;
 }
-struct XaPlan { int wq, nqt, ns, wk, nkt, nsb; };
+struct XaPlan { int wq, nqt, ns, nkt, nsb; };
 static XaPlan xa_plan(int B, long long R, int Lk, int Hk) {
     XaPlan q;
     q.wq = R <= 32 ? 1 : 4;
     q.nqt = (int)((R + 32 * q.wq - 1) / (32 * q.wq));
-    const int kt = q.wq == 4 ? 64 : 128;
+    const int kt = q.wq == 4 ? 64 : 128;   // keys a workgroup takes at a time
     q.ns = xa_splits((long long)B * Hk * q.nqt, (Lk + kt - 1) / kt);
-    q.wk = Lk <= 32 ? 1 : 4;
-    q.nkt = (Lk + 32 * q.wk - 1) / (32 * q.wk);
-    const int rt = q.wk == 4 ? 64 : 128;
-    q.nsb = xa_splits((long long)B * Hk * q.nkt, (R + rt - 1) / rt);
+    q.nkt = (Lk + 127) / 128;
+    q.nsb = xa_splits((long long)B * Hk * q.nkt, (R + 63) / 64);
     return q;
 }
 static bool xa_bad(int B, int Lq, int Lk, int Hk, int G, int D, int dtype) {
@@ -627,8 +696,8 @@ static unsigned xa_grid(long long total) { return (unsigned)((total + 7) / 8 * 8
 
 template <typename T, int DP, int WQ>
 static int xa_fwd_launch(const XaArgs& a, const XaPlan& q, hipStream_t s) {
-    const int kt = WQ == 4 ? 64 : 128, total = a.B * a.Hk * q.nqt * a.ns;
-    const size_t lds = (size_t)2 * kt * DP * sizeof(T) + (WQ == 1 ? 256 * sizeof(float) : 0);
+    const int total = a.B * a.Hk * q.nqt * a.ns;
+    const size_t lds = XaFwdTile<T, DP, WQ>::TOTAL;
     if (int e = xa_lds(xa_fwd_kernel<T, DP, WQ>, lds)) return e;
     hipLaunchKernelGGL((xa_fwd_kernel<T, DP, WQ>), dim3(xa_grid(total)), dim3(256), lds, s, a, q.nqt, total);
     return L2I_OK;
@@ -649,36 +718,31 @@ static int xa_fwd_type(const XaArgs& a, const XaPlan& q, hipStream_t s) {
 template <typename T, int DP>
 static int xa_bwd_launch(const XaArgs& a, const XaPlan& q, hipStream_t s) {
     const int nqt = (a.R + 127) / 128, tq = a.B * a.Hk * nqt, tk = a.B * a.Hk * q.nkt * a.ns;
-    const size_t lq = (size_t)2 * 64 * DP * sizeof(T);
+    const size_t lq = (size_t)4 * 64 * DP * sizeof(T), lk = lq + 6 * 64 * sizeof(float);
     if (int e = xa_lds(xa_dq_kernel<T, DP>, lq)) return e;
     hipLaunchKernelGGL((xa_dq_kernel<T, DP>), dim3(xa_grid(tq)), dim3(256), lq, s, a, nqt, tq);
     if (!a.dk || a.Lk == 0) return L2I_OK;
-    const int rt = q.wk == 4 ? 64 : 128;
-    const size_t lk = (size_t)2 * rt * DP * sizeof(T) + (size_t)rt * 12;
-    if (q.wk == 4) {
-        if (int e = xa_lds(xa_dkv_kernel<T, DP, 4>, lk)) return e;
-        hipLaunchKernelGGL((xa_dkv_kernel<T, DP, 4>), dim3(xa_grid(tk)), dim3(256), lk, s, a, q.nkt, tk);
-    } else {
-        if (int e = xa_lds(xa_dkv_kernel<T, DP, 1>, lk)) return e;
-        hipLaunchKernelGGL((xa_dkv_kernel<T, DP, 1>), dim3(xa_grid(tk)), dim3(256), lk, s, a, q.nkt, tk);
-    }
+    if (int e = xa_lds(xa_dkv_kernel<T, DP>, lk)) return e;
+    hipLaunchKernelGGL((xa_dkv_kernel<T, DP>), dim3(xa_grid(tk)), dim3(256), lk, s, a, q.nkt, tk);
     if (a.ns > 1) {
         const long long n = (long long)a.B * a.Hk * a.Lk * a.D;
         hipLaunchKernelGGL((xa_fold_kernel<T>), dim3((unsigned)((n / 4 + 255) / 256), 2), dim3(256), 0, s, a);
     }
     return L2I_OK;
 }
-// strides: 16-byte steps between any two rows, so that every row starts on a 16-byte boundary
-static bool xa_rows_ok(const void* t, long long sb, long long sl, long long sh, int dtype) {
-    const long long e = dtype ? 8 : 4;
-    return !((size_t)t & 15) && sb % e == 0 && sl % e == 0 && sh % e == 0 && sb >= 0 && sl >= 0 && sh >= 0;
+// strides: 16-byte steps between any two rows, so that every row starts on a 16-byte boundary; the rows of a tile (64 positions and the G heads
+// of a group) span less than 2^31 bytes
+static bool xa_rows_ok(const void* t, long long sb, long long sl, long long sh, int heads, int dtype) {
+    const long long e = dtype ? 8 : 4, most = 1LL << 31;
+    if (((size_t)t & 15) || sb % e || sl % e || sh % e || sb < 0 || sl < 0 || sh < 0) return false;
+    return sl < most / 512 && sh < most && 65 * sl * (16 / e) + heads * sh * (16 / e) + 1024 < most;
 }
 static void xa_setup(XaArgs& a, const void* q, const void* k, const void* v, const int* lengths, const unsigned char* mask, int B, int Lq, int Lk, int Hk,
                      int G, int D, long long qb, long long ql, long long qh, long long kb, long long kl, long long kh, long long vb, long long vl, long long vh,
                      long long mb, long long mq, float scale) {
     a.q = q; a.k = k; a.v = v; a.len = lengths; a.mask = mask; a.B = B; a.Lq = Lq; a.Lk = Lk; a.Hk = Hk; a.G = G; a.D = D; a.R = Lq * G;
     a.qb = qb; a.ql = ql; a.qh = qh; a.kb = kb; a.kl = kl; a.kh = kh; a.vb = vb; a.vl = vl; a.vh = vh; a.mb = mb; a.mq = mq;
-    a.scale = scale; a.c = scale * 1.44269504088896340736f;
+    a.scale = scale; a.c = fabsf(scale) * 1.44269504088896340736f;
 }
 extern "C" int l2i_cross_attention_fwd(const void* q, const void* k, const void* v, int dtype, const int* lengths, const unsigned char* mask, void* out,
                                        float* lse, int B, int Lq, int Lk, int Hk, int G, int D, long long qb, long long ql, long long qh, long long kb,
@@ -686,7 +750,7 @@ extern "C" int l2i_cross_attention_fwd(const void* q, const void* k, const void*
                                        float* scratch, long long scratch_floats, void* stream) {
     long long need = 0;
     if (xa_bad(B, Lq, Lk, Hk, G, D, dtype) || !q || !out || (Lk && (!k || !v)) || mb < 0 || mq < 0 || ((size_t)out & 15)) return L2I_ERR_ARG;
-    if (!xa_rows_ok(q, qb, ql, qh, dtype) || !xa_rows_ok(k, kb, kl, kh, dtype) || !xa_rows_ok(v, vb, vl, vh, dtype)) return L2I_ERR_ARG;
+    if (!xa_rows_ok(q, qb, ql, qh, G, dtype) || !xa_rows_ok(k, kb, kl, kh, 0, dtype) || !xa_rows_ok(v, vb, vl, vh, 0, dtype)) return L2I_ERR_ARG;
     if (l2i_cross_attention_scratch(B, Lq, Lk, Hk, G, D, 0, &need) != L2I_OK) return L2I_ERR_ARG;
     if (need && (!scratch || ((size_t)scratch & 15) || scratch_floats < need)) return L2I_ERR_ARG;
     XaArgs a = {};
@@ -704,7 +768,7 @@ extern "C" int l2i_cross_attention_bwd(const void* q, const void* k, const void*
     long long need = 0;
     if (xa_bad(B, Lq, Lk, Hk, G, D, dtype) || !q || !out || !lse || !dout || (Lk && (!k || !v)) || mb < 0 || mq < 0) return L2I_ERR_ARG;
     if ((dk == nullptr) != (dv == nullptr) || (((size_t)out | (size_t)dout | (size_t)dq | (size_t)dk | (size_t)dv) & 15)) return L2I_ERR_ARG;
-    if (!xa_rows_ok(q, qb, ql, qh, dtype) || !xa_rows_ok(k, kb, kl, kh, dtype) || !xa_rows_ok(v, vb, vl, vh, dtype)) return L2I_ERR_ARG;
+    if (!xa_rows_ok(q, qb, ql, qh, G, dtype) || !xa_rows_ok(k, kb, kl, kh, 0, dtype) || !xa_rows_ok(v, vb, vl, vh, 0, dtype)) return L2I_ERR_ARG;
     if (l2i_cross_attention_scratch(B, Lq, Lk, Hk, G, D, 1, &need) != L2I_OK || !scratch || ((size_t)scratch & 15) || scratch_floats < need) return L2I_ERR_ARG;
     XaArgs a = {};
     xa_setup(a, q, k, v, lengths, mask, B, Lq, Lk, Hk, G, D, qb, ql, qh, kb, kl, kh, vb, vl, vh, mb, mq, scale);
