@@ -497,7 +497,7 @@ int l2i_group_norm_bwd(const void* x, int x_dtype, const float* gamma, const flo
  * have to be finite. A query without a live key gives zeros (and no gradient).
  * out [B][Lq][Hk G][D] contiguous; lse [B][Hk][Lq G] (optional in fwd) is kept for bwd.
  * bwd: out, dout, dq [B][Lq][Hk G][D] and dk, dv [B][Lk][Hk][D] contiguous and 16-byte aligned; dq, and dk with dv, optional. */
-int l2i_cross_attention_scratch(int B, int Lq, int Lk, int Hk, int G, int D, int bwd, long long* floats);
+int l2i_cross_attention_scratch(int B, int Lq, int Lk, int Hk, int G, int D, int dtype, int bwd, long long* floats);
 int l2i_cross_attention_fwd(const void* q, const void* k, const void* v, int dtype, const int* lengths, const unsigned char* mask, void* out,
                             float* lse, int B, int Lq, int Lk, int Hk, int G, int D, long long qb, long long ql, long long qh, long long kb,
                             long long kl, long long kh, long long vb, long long vl, long long vh, long long mb, long long mq, float scale,

@@ -86,7 +86,7 @@ SIGNATURES = {
     "l2i_group_norm_scratch": [_i, _ll, _i, _i, _i, _p],
     "l2i_group_norm_fwd": [_p, _i, _p, _p, _p, _i, _p, _p, _i, _ll, _i, _i, _f, _i, _p, _ll, _p],
     "l2i_group_norm_bwd": [_p, _i, _p, _p, _p, _p, _p, _i, _p, _p, _p, _i, _ll, _i, _i, _i, _p, _ll, _p],
-    "l2i_cross_attention_scratch": [_i, _i, _i, _i, _i, _i, _i, _p],
+    "l2i_cross_attention_scratch": [_i, _i, _i, _i, _i, _i, _i, _i, _p],
     "l2i_cross_attention_fwd": [_p, _p, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _f,
                                 _p, _ll, _p],
     "l2i_cross_attention_bwd": [_p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll,

@@ -18,6 +18,7 @@
 // them (about 900 cycles), so the vector unit; tiles therefore come to LDS by LDS-DMA (no registers, no instructions of the waves), two
 // buffers deep, and the rescaling of the accumulators waits until the maximum has grown by 2^8.
 #include "igemm.h"
+#include <algorithm>
 #include <type_traits>
 
 typedef __attribute__((ext_vector_type(8))) __bf16 b16x8_t;
@@ -63,27 +64,33 @@ template <typename T, int CH> __device__ __forceinline__ void xa_rows_dot(f32x16
     for (int s = 0; s < CH / 2; ++s) xa_dot(acc, *reinterpret_cast<const uint4*>(tile + xa_at<CH>(row0 + (lane & 31), 2 * s + h)), b[s], T());
 }
 
+// ---- bf16: the lane's column of 8 tile rows as a product operand: column 32 db + lane % 32, rows row0 + 16 t + 4 h + {0 .. 3} and 8 further on --
+// the order in which an accumulator's registers 8 t .. 8 t + 7 hold its rows
+template <int CH> __device__ __forceinline__ b16x8_t xa_tr(const char* tile, int row0, int t, int db) {
+    const int lane = threadIdx.x & 63, h = lane >> 5, i = lane & 15, d16 = (lane >> 4) & 1;
+    const int ra = row0 + 16 * t + 4 * h + (i >> 2), chunk = db * 4 + d16 * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
+    typedef __attribute__((address_space(3))) s16x4_t lds4_t;
+    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t*)(tile + xa_at<CH>(ra, chunk) + sub));
+    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t*)(tile + xa_at<CH>(ra + 8, chunk) + sub));
+    bf16x8_t a;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { a[e] = lo[e]; a[4 + e] = hi[e]; }
+    return __builtin_bit_cast(b16x8_t, a);
+}
+template <int CH> __device__ __forceinline__ float xa_el(const char* tile, int row, int col) {   // f32: one value
+    return *reinterpret_cast<const float*>(tile + xa_at<CH>(row, col >> 2) + (col & 3) * 4);
+}
+
 // ---- acc[d][lane] += sum over 32 tile rows i of tile[row0 + i][d] p_i(lane); p: an accumulator (register r of a lane = row 8 (r / 4) + 4 (lane / 32) + r % 4)
 template <int CH, int ND>
 __device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, int row0, const f32x16_t& p, bf16_t) {
-    const int lane = threadIdx.x & 63, h = lane >> 5, i = lane & 15, d16 = (lane >> 4) & 1;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         uint4 pb;
         pb.x = f2bf2(p[8 * t], p[8 * t + 1]); pb.y = f2bf2(p[8 * t + 2], p[8 * t + 3]);
         pb.z = f2bf2(p[8 * t + 4], p[8 * t + 5]); pb.w = f2bf2(p[8 * t + 6], p[8 * t + 7]);
-        const int ra = row0 + 16 * t + 4 * h + (i >> 2);
 #pragma unroll
-        for (int db = 0; db < ND; ++db) {
-            const int chunk = db * 4 + d16 * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
-            typedef __attribute__((address_space(3))) s16x4_t lds4_t;
-            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t*)(tile + xa_at<CH>(ra, chunk) + sub));
-            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t*)(tile + xa_at<CH>(ra + 8, chunk) + sub));
-            bf16x8_t a;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { a[e] = lo[e]; a[4 + e] = hi[e]; }
-            acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8_t, a), __builtin_bit_cast(b16x8_t, pb), acc[db], 0, 0, 0);
-        }
+        for (int db = 0; db < ND; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa_tr<CH>(tile, row0, t, db), __builtin_bit_cast(b16x8_t, pb), acc[db], 0, 0, 0);
     }
 }
 template <int CH, int ND>
@@ -94,10 +101,40 @@ __device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, i
         const int row = row0 + 8 * (r >> 2) + 4 * h + (r & 3);
 #pragma unroll
         for (int db = 0; db < ND; ++db) {
-            const int col = db * 32 + (lane & 31);
-            const float a = *reinterpret_cast<const float*>(tile + xa_at<CH>(row, col >> 2) + (col & 3) * 4);
-            acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[db], 0, 0, 0);
+            acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(xa_el<CH>(tile, row, db * 32 + (lane & 31)), p[r], acc[db], 0, 0, 0);
         }
+    }
+}
+// ---- the same with p from a second tile of 32 rows x 32 columns (row i, column = lane): what an accumulator's transpose is, through LDS
+template <typename T> struct XaSquare {
+    static constexpr int CH = 32 * (int)sizeof(T) / 16, BYTES = 32 * CH * 16;
+    __device__ __forceinline__ static void store(char* tile, const f32x16_t& p) {   // column i of the lane's accumulator -> row `lane`
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const float v[4] = {p[4 * a], p[4 * a + 1], p[4 * a + 2], p[4 * a + 3]};
+            if constexpr (sizeof(T) == 2) Op4<bf16_t>::store(reinterpret_cast<bf16_t*>(tile + xa_at<CH>(lane & 31, a) + 8 * h), v);
+            else Op4<float>::store(reinterpret_cast<float*>(tile + xa_at<CH>(lane & 31, 2 * a + h)), v);
+        }
+        asm volatile("" ::: "memory");   // (the wave's own LDS accesses run in order; the compiler keeps them so)
+    }
+};
+template <int CH, int ND> __device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, const char* sq, bf16_t) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const b16x8_t pb = xa_tr<XaSquare<bf16_t>::CH>(sq, 0, t, 0);
+#pragma unroll
+        for (int db = 0; db < ND; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa_tr<CH>(tile, 0, t, db), pb, acc[db], 0, 0, 0);
+    }
+}
+template <int CH, int ND> __device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, const char* sq, float) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int row = 8 * (r >> 2) + 4 * h + (r & 3);
+        const float pb = xa_el<XaSquare<float>::CH>(sq, row, lane & 31);
+#pragma unroll
+        for (int db = 0; db < ND; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(xa_el<CH>(tile, row, db * 32 + (lane & 31)), pb, acc[db], 0, 0, 0);
     }
 }
 
@@ -202,6 +239,22 @@ template <typename T> struct XaStates {
     }
     __device__ __forceinline__ bool live(int j) const { return j < len && (!kmask || mb[j]); }
 };
+
+// NR rows from r0 on of the queries and of g, for groups of several heads: row r0 + i = head (g0 + i) % G of query iq0 + (g0 + i) / G
+template <typename T, int CH, int NR, int TH>
+__device__ __forceinline__ void xa_issue_heads(const XaArgs& p, const T* qp, const T* gp, long long gl, int r0, float rG, unsigned qat, unsigned gat) {
+    const int iq0 = (int)((unsigned)r0 / (unsigned)p.G), g0 = r0 - iq0 * p.G, left = p.R - r0;
+    XaDma<T, CH, NR, TH> a, c;
+#pragma unroll
+    for (int i = 0; i < a.N; ++i) {
+        const int rr = g0 + a.row(i), di = (int)(((float)rr + 0.5f) * rG), gg = rr - di * p.G, ck = a.chunk(i) * 16;
+        const bool ok = ck < p.D * (int)sizeof(T) && a.row(i) < left;
+        a.off[i] = ok ? (unsigned)((di * p.ql + gg * p.qh) * (int)sizeof(T)) + ck : XA_OOB;
+        c.off[i] = ok ? (unsigned)((di * gl + gg * p.D) * (int)sizeof(T)) + ck : XA_OOB;
+    }
+    a.issue(qp + (long long)iq0 * p.ql, qat);
+    c.issue(gp + (long long)iq0 * gl, gat);
+}
 
 // ------------------------------------------------------------------------------------------------ forward
 // WQ = 4: four waves x 32 rows share tiles of 64 keys (one barrier a tile). WQ = 1: 32 rows (a single token, a few), every wave has tiles of 32
@@ -540,18 +593,8 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_d
                 dq.issue(a, at, rows);
                 dg.issue(c, at + BYTES, rows);
             }
-        } else {   // row r0 + i = head (g0 + i) % G of query iq0 + (g0 + i) / G
-            const int iq0 = (int)((unsigned)r0 / (unsigned)p.G), g0 = r0 - iq0 * p.G;
-            XaDma<T, CH, RT, 256> a, c;
-#pragma unroll
-            for (int i = 0; i < a.N; ++i) {
-                const int rr = g0 + a.row(i), di = (int)(((float)rr + 0.5f) * rG), gg = rr - di * p.G, ck = a.chunk(i) * 16;
-                const bool ok = ck < p.D * (int)sizeof(T) && a.row(i) < left;
-                a.off[i] = ok ? (unsigned)((di * p.ql + gg * p.qh) * (int)sizeof(T)) + ck : XA_OOB;
-                c.off[i] = ok ? (unsigned)((di * gl + gg * p.D) * (int)sizeof(T)) + ck : XA_OOB;
-            }
-            a.issue(qp + (long long)iq0 * p.ql, at);
-            c.issue(gp + (long long)iq0 * gl, at + BYTES);
+        } else {
+            xa_issue_heads<T, CH, RT, 256>(p, qp, gp, gl, r0, rG, at, at + BYTES);
         }
         if (threadIdx.x < RT) {
             const bool on = (int)threadIdx.x < left;
@@ -652,6 +695,242 @@ __global__ __launch_bounds__(256) void xa_fold_kernel(XaArgs p) {
     Op4<T>::store(reinterpret_cast<T*>(blockIdx.y ? p.dv : p.dk) + (((size_t)b * p.Lk + key) * p.Hk + hk) * p.D + d, s);
 }
 
+// ------------------------------------------------------------------------------------------------ states that fit one tile
+// At most 32 states (a layout's objects): K and V stand in LDS for a whole workgroup, whose waves each walk row blocks of 32 on their own, with no
+// barrier. Bound by bytes: q and out forward; q, g and dq backward -- S, P and D = sum_j P_ij (g_i . v_j) are made from them in registers, so
+// that one launch gives dq and (through a transpose of P and dS in LDS) its rows' share of dk and dv.
+template <typename T, int DP> struct XaShort {
+    static constexpr int CH = DP * (int)sizeof(T) / 16, TILE = 32 * CH * 16;
+    static constexpr int SQ = XaSquare<T>::BYTES;
+    static constexpr int NBUF = 2 * TILE + 4 * (4 * TILE + 2 * SQ) <= 160 * 1024 ? 2 : 1;
+    static constexpr int WAVE = 2 * TILE * NBUF + 2 * SQ;             // of a wave, backward
+    static constexpr int BWD = 2 * TILE + 4 * WAVE;
+    static constexpr bool OK = BWD <= 160 * 1024;
+};
+template <typename T, int CH> __device__ __forceinline__ void xa_stage32(char* tile, const T* src, long long stride, int D, const XaStates<T>& st) {
+    for (int i = threadIdx.x; i < 32 * CH; i += 256) {
+        const int row = i / CH, chunk = i - row * CH;
+        uint4 a = make_uint4(0, 0, 0, 0);
+        if (chunk * 16 < D * (int)sizeof(T) && st.live(row)) a = *reinterpret_cast<const uint4*>(src + row * stride + chunk * (16 / (int)sizeof(T)));
+        *reinterpret_cast<uint4*>(tile + xa_at<CH>(row, chunk)) = a;
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 2 : 4) void xa_short_fwd_kernel(XaArgs p, int nwg, int total) {
+    constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    char *ks = smem, *vs = smem + 32 * CH * 16;
+    const int id = xa_tile_id(total);
+    if (id >= total) return;
+    const int bh = id / nwg, part = id - bh * nwg, b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+    const int nblk = (p.R + 31) / 32, step = 4 * nwg;
+    const XaStates<T> st(p, b, hk);
+    const unsigned kbits = (unsigned)__ballot(lane < 32 && st.live(lane));
+    const bool qmask = st.mb && !st.kmask, all = !qmask && kbits == 0xffffffffu;
+    uint4 nq[S];
+    unsigned nlive = 0;
+    auto fetch = [&](int blk) {   // the block's queries and their live keys, on the way while the block before is worked on
+        const int r = blk * 32 + (lane & 31), iq = r < p.R ? xa_row_query(p, r) : 0;
+        const T* src = r < p.R ? reinterpret_cast<const T*>(p.q) + b * p.qb + (long long)iq * p.ql + (hk * p.G + r - iq * p.G) * p.qh : nullptr;
+        xa_row_frag<T, CH>(nq, src, p.D, p.scale < 0.f);
+        nlive = xa_live(kbits, qmask ? st.mb + (long long)iq * p.mq : nullptr, 0, p.Lk);
+    };
+    int blk = part * 4 + wave;
+    if (blk < nblk) fetch(blk);
+    xa_stage32<T, CH>(ks, st.k, p.kl, p.D, st);
+    xa_stage32<T, CH>(vs, st.v, p.vl, p.D, st);
+    __syncthreads();
+    for (; blk < nblk; blk += step) {
+        uint4 qf[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) qf[s] = nq[s];
+        const unsigned live = nlive;
+        if (blk + step < nblk) fetch(blk + step);
+        f32x16_t sc, oacc[ND];
+        xa_rows_dot<T, CH>(sc, ks, 0, qf);
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { sc[e] = xa_pick(live, e, sc[e], XA_NINF); m = fmaxf(m, sc[e]); }
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const float ref = m == -INFINITY ? 0.f : m * p.c;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { sc[e] = xa_exp2(xa_pick(live, e, fmaf(sc[e], p.c, -ref), XA_NINF)); l += sc[e]; }
+        l += __shfl_xor(l, 32, 64);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) oacc[d][e] = 0.f;
+        xa_tdot<CH, ND>(oacc, vs, 0, sc, T());
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) oacc[d][e] *= inv;   // (here, in front of the branch below)
+        const int r = blk * 32 + (lane & 31);
+        if (r < p.R) {
+            const int iq = xa_row_query(p, r), head = hk * p.G + r - iq * p.G;
+            if (p.lse && h == 0) p.lse[(size_t)bh * p.R + r] = l > 0.f ? ref + log2f(l) : INFINITY;
+            T* o = reinterpret_cast<T*>(p.o) + (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const int dd = d * 32 + 8 * a + 4 * h;
+                    const float v[4] = {oacc[d][4 * a], oacc[d][4 * a + 1], oacc[d][4 * a + 2], oacc[d][4 * a + 3]};
+                    if (dd < p.D) Op4<T>::store(o + dd, v);
+                }
+        }
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : DP == 64 ? 2 : 3) void xa_short_bwd_kernel(XaArgs p, int nwg, int total) {
+    using Sh = XaShort<T, DP>;
+    constexpr int CH = Sh::CH, ND = DP / 32, S = CH / 2, NBUF = Sh::NBUF;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    char *ks = smem, *vs = smem + Sh::TILE;
+    const int id = xa_tile_id(total);
+    if (id >= total) return;
+    const int bh = id / nwg, part = id - bh * nwg, b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+    const int nblk = (p.R + 31) / 32, step = 4 * nwg;
+    char* mine = smem + 2 * Sh::TILE + wave * Sh::WAVE;      // q and g tiles, NBUF of each; P, dS
+    char *sp = mine + 2 * Sh::TILE * NBUF, *sd = sp + Sh::SQ;
+    const unsigned lds = lds_addr_of(mine);
+    const XaStates<T> st(p, b, hk);
+    const unsigned kbits = (unsigned)__ballot(lane < 32 && st.live(lane));
+    const bool qmask = st.mb && !st.kmask;
+    const T* qp = reinterpret_cast<const T*>(p.q) + b * p.qb + hk * p.G * p.qh;
+    const T* gp = reinterpret_cast<const T*>(p.g) + ((size_t)b * p.Lq * p.Hk + hk) * p.G * p.D;
+    const long long gl = (long long)p.Hk * p.G * p.D;   // a query's step in g
+    XaDma<T, CH, 32, 64> dq, dg;
+    dq.init(p.ql, p.D);
+    dg.init(gl, p.D);
+    const float rG = 1.f / (float)p.G;
+    auto issue = [&](int blk, int buf) {
+        const int r0 = blk * 32, left = p.R - r0;
+        const unsigned at = lds + buf * 2 * Sh::TILE;
+        if (p.G == 1) {
+            const T *a = qp + (long long)r0 * p.ql, *c = gp + (long long)r0 * gl;
+            if (left >= 32) { dq.issue(a, at); dg.issue(c, at + Sh::TILE); }
+            else {
+                auto rows = [&](int i) { return i < left; };
+                dq.issue(a, at, rows);
+                dg.issue(c, at + Sh::TILE, rows);
+            }
+        } else {
+            xa_issue_heads<T, CH, 32, 64>(p, qp, gp, gl, r0, rG, at, at + Sh::TILE);
+        }
+    };
+    int blk = part * 4 + wave, buf = 0;
+    if (blk < nblk) issue(blk, 0);
+    xa_stage32<T, CH>(ks, st.k, p.kl, p.D, st);
+    xa_stage32<T, CH>(vs, st.v, p.vl, p.D, st);
+    __syncthreads();
+    f32x16_t dk[ND], dv[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { dk[d][e] = 0.f; dv[d][e] = 0.f; }
+    for (; blk < nblk; blk += step) {
+        const int r = blk * 32 + (lane & 31);
+        const bool on = r < p.R;
+        const int iq = on ? xa_row_query(p, r) : 0;
+        const float ls = on ? p.lse[(size_t)bh * p.R + r] : INFINITY;   // (a row behind the last: probabilities 0)
+        const unsigned live = xa_live(kbits, qmask ? st.mb + (long long)iq * p.mq : nullptr, 0, p.Lk);
+        if (NBUF == 2 && blk + step < nblk) {
+            issue(blk + step, buf ^ 1);
+            xa_wait_dma<2 * XaDma<T, CH, 32, 64>::N>();
+        } else {
+            xa_wait_dma<0>();
+        }
+        const char *qs = mine + buf * 2 * Sh::TILE, *gs = qs + Sh::TILE;
+        uint4 qf[S], gf[S];
+        const unsigned flip = p.scale < 0.f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int at = xa_at<CH>(lane & 31, 2 * s + h);
+            qf[s] = *reinterpret_cast<const uint4*>(qs + at);
+            gf[s] = *reinterpret_cast<const uint4*>(gs + at);
+            qf[s].x ^= flip; qf[s].y ^= flip; qf[s].z ^= flip; qf[s].w ^= flip;
+        }
+        f32x16_t sc, dp, dqa[ND];
+        xa_rows_dot<T, CH>(sc, ks, 0, qf);
+        xa_rows_dot<T, CH>(dp, vs, 0, gf);
+        float dl = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            sc[e] = xa_pick(live, e, xa_exp2(fmaf(sc[e], p.c, -ls)), 0u);
+            dl = fmaf(sc[e], dp[e], dl);
+        }
+        dl += __shfl_xor(dl, 32, 64);
+        XaSquare<T>::store(sp, sc);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] *= dp[e] - dl;
+        XaSquare<T>::store(sd, sc);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dqa[d][e] = 0.f;
+        xa_tdot<CH, ND>(dqa, ks, 0, sc, T());
+        xa_tdot<CH, ND>(dv, gs, sp, T());
+        xa_tdot<CH, ND>(dk, qs, sd, T());
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dqa[d][e] *= p.scale;   // (here, in front of the branch below)
+        if (on && p.dq) {
+            T* o = reinterpret_cast<T*>(p.dq) + (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + hk * p.G + r - iq * p.G) * p.D;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const int dd = d * 32 + 8 * a + 4 * h;
+                    const float v[4] = {dqa[d][4 * a], dqa[d][4 * a + 1], dqa[d][4 * a + 2], dqa[d][4 * a + 3]};
+                    if (dd < p.D) Op4<T>::store(o + dd, v);
+                }
+        }
+        if (NBUF == 2) buf ^= 1;
+        else if (blk + step < nblk) issue(blk + step, 0);
+    }
+    xa_settle();
+    if (!p.dk) return;
+    // the four waves' shares, in wave order: [4][DP][32] f32 over the waves' tiles, dk then dv; wave d keeps block d of the dims
+    float* ob = reinterpret_cast<float*>(smem);
+    const int n = lane & 31;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) ob[(wave * DP + d * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + n] = which ? dv[d][e] : dk[d][e] * p.scale;
+        __syncthreads();
+        if (wave < ND && n < p.Lk) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int dd = wave * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+                v[e] = (ob[dd * 32 + n] + ob[(DP + dd) * 32 + n]) + (ob[(2 * DP + dd) * 32 + n] + ob[(3 * DP + dd) * 32 + n]);
+            }
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const int dd = wave * 32 + 8 * a + 4 * h;
+                if (dd >= p.D) continue;
+                const float w[4] = {v[4 * a], v[4 * a + 1], v[4 * a + 2], v[4 * a + 3]};
+                if (p.ns > 1) {
+                    const size_t all = (size_t)p.B * p.Hk * p.Lk * p.D;
+                    Op4<float>::store(p.part + (size_t)(which * p.ns + part) * all + ((size_t)bh * p.Lk + n) * p.D + dd, w);
+                } else {
+                    Op4<T>::store(reinterpret_cast<T*>(which ? p.dv : p.dk) + (((size_t)b * p.Lk + n) * p.Hk + hk) * p.D + dd, w);
+                }
+            }
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ entry points
 #define XA_WGS 512   // workgroups that fill the chip: 256 CUs, two each
 static int xa_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
@@ -663,15 +942,26 @@ static int xa_splits(long long tiles, long long nt) {
     if (ns > 64) ns = 64;
     return ns < 1 ? 1 : (int)ns;
 }
-struct XaPlan { int wq, nqt, ns, nkt, nsb; };
-static XaPlan xa_plan(int B, long long R, int Lk, int Hk) {
+struct XaPlan { int wq, nqt, ns, nkt, nsb, nwf, nwb; };   // nwf, nwb: workgroups an (image, state head) of the one-tile form has, 0: not that form
+static bool xa_short_fits(int dp, int dtype) {
+    return dtype ? (dp == 32 ? XaShort<bf16_t, 32>::OK : dp == 64 ? XaShort<bf16_t, 64>::OK : XaShort<bf16_t, 128>::OK)
+                 : (dp == 32 ? XaShort<float, 32>::OK : dp == 64 ? XaShort<float, 64>::OK : XaShort<float, 128>::OK);
+}
+static XaPlan xa_plan(int B, long long R, int Lk, int Hk, int D, int dtype) {
     XaPlan q;
+    const long long bh = (long long)B * Hk, groups = (R + 127) / 128;   // a workgroup's four waves take at least a block of 32 rows each
+    q.nwf = q.nwb = 0;
+    if (Lk <= 32 && xa_short_fits(xa_dp(D), dtype)) {
+        q.nwf = (int)std::min(groups, std::max(1LL, (2048 + bh - 1) / bh));
+        q.nwb = (int)std::min(groups, std::max(1LL, (1024 + bh - 1) / bh));
+    }
     q.wq = R <= 32 ? 1 : 4;
     q.nqt = (int)((R + 32 * q.wq - 1) / (32 * q.wq));
     const int kt = q.wq == 4 ? 64 : 128;   // keys a workgroup takes at a time
     q.ns = xa_splits((long long)B * Hk * q.nqt, (Lk + kt - 1) / kt);
     q.nkt = (Lk + 127) / 128;
-    q.nsb = xa_splits((long long)B * Hk * q.nkt, (R + 63) / 64);
+    q.nsb = q.nwb ? q.nwb : xa_splits((long long)B * Hk * q.nkt, (R + 63) / 64);
+    if (q.nwf) q.ns = 1;
     return q;
 }
 static bool xa_bad(int B, int Lq, int Lk, int Hk, int G, int D, int dtype) {
@@ -680,10 +970,10 @@ static bool xa_bad(int B, int Lq, int Lk, int Hk, int G, int D, int dtype) {
     // (rows, tiles and workgroups are counted in 32 bits; the offsets of rows in 64)
     return R > (1LL << 30) || Lk > (1 << 30) || (long long)B * Hk * ((R + 31) / 32) > (1LL << 28) || (long long)B * Hk * ((Lk + 31) / 32) > (1LL << 28);
 }
-extern "C" int l2i_cross_attention_scratch(int B, int Lq, int Lk, int Hk, int G, int D, int bwd, long long* floats) {
-    if (!floats || xa_bad(B, Lq, Lk, Hk, G, D, 0)) return L2I_ERR_ARG;
+extern "C" int l2i_cross_attention_scratch(int B, int Lq, int Lk, int Hk, int G, int D, int dtype, int bwd, long long* floats) {
+    if (!floats || xa_bad(B, Lq, Lk, Hk, G, D, dtype)) return L2I_ERR_ARG;
     const long long R = (long long)Lq * G;
-    const XaPlan q = xa_plan(B, R, Lk, Hk);
+    const XaPlan q = xa_plan(B, R, Lk, Hk, D, dtype);
     if (bwd) *floats = ((long long)B * Hk * R + 3) / 4 * 4 + (q.nsb > 1 ? 2LL * q.nsb * B * Hk * Lk * D : 0);
     else *floats = q.ns > 1 ? (long long)q.ns * B * Hk * R * (D + 2) : 0;
     return L2I_OK;
@@ -702,10 +992,19 @@ static int xa_fwd_launch(const XaArgs& a, const XaPlan& q, hipStream_t s) {
     hipLaunchKernelGGL((xa_fwd_kernel<T, DP, WQ>), dim3(xa_grid(total)), dim3(256), lds, s, a, q.nqt, total);
     return L2I_OK;
 }
+template <typename T, int DP>
+static int xa_short_fwd_launch(const XaArgs& a, const XaPlan& q, hipStream_t s) {
+    if constexpr (XaShort<T, DP>::OK) {
+        const int total = a.B * a.Hk * q.nwf;
+        hipLaunchKernelGGL((xa_short_fwd_kernel<T, DP>), dim3(xa_grid(total)), dim3(256), (size_t)2 * 32 * DP * sizeof(T), s, a, q.nwf, total);
+    }
+    return L2I_OK;
+}
 template <typename T>
 static int xa_fwd_type(const XaArgs& a, const XaPlan& q, hipStream_t s) {
     const int dp = xa_dp(a.D);
     int e;
+    if (q.nwf) return dp == 32 ? xa_short_fwd_launch<T, 32>(a, q, s) : dp == 64 ? xa_short_fwd_launch<T, 64>(a, q, s) : xa_short_fwd_launch<T, 128>(a, q, s);
     if (q.wq == 1) e = dp == 32 ? xa_fwd_launch<T, 32, 1>(a, q, s) : dp == 64 ? xa_fwd_launch<T, 64, 1>(a, q, s) : xa_fwd_launch<T, 128, 1>(a, q, s);
     else e = dp == 32 ? xa_fwd_launch<T, 32, 4>(a, q, s) : dp == 64 ? xa_fwd_launch<T, 64, 4>(a, q, s) : xa_fwd_launch<T, 128, 4>(a, q, s);
     if (e) return e;
@@ -715,8 +1014,24 @@ static int xa_fwd_type(const XaArgs& a, const XaPlan& q, hipStream_t s) {
     }
     return L2I_OK;
 }
+template <typename T>
+static void xa_fold_launch(const XaArgs& a, hipStream_t s) {
+    const long long n = (long long)a.B * a.Hk * a.Lk * a.D;
+    hipLaunchKernelGGL((xa_fold_kernel<T>), dim3((unsigned)((n / 4 + 255) / 256), 2), dim3(256), 0, s, a);
+}
 template <typename T, int DP>
 static int xa_bwd_launch(const XaArgs& a, const XaPlan& q, hipStream_t s) {
+    if (q.nwb) {
+        if constexpr (XaShort<T, DP>::OK) {
+            const int total = a.B * a.Hk * q.nwb;
+            // (the waves' shares of dk are joined over the whole of LDS: at least 512 DP bytes)
+            const size_t lds = XaShort<T, DP>::BWD > 512 * DP ? XaShort<T, DP>::BWD : 512 * DP;
+            if (int e = xa_lds(xa_short_bwd_kernel<T, DP>, lds)) return e;
+            hipLaunchKernelGGL((xa_short_bwd_kernel<T, DP>), dim3(xa_grid(total)), dim3(256), lds, s, a, q.nwb, total);
+            if (a.dk && a.Lk && a.ns > 1) xa_fold_launch<T>(a, s);
+        }
+        return L2I_OK;
+    }
     const int nqt = (a.R + 127) / 128, tq = a.B * a.Hk * nqt, tk = a.B * a.Hk * q.nkt * a.ns;
     const size_t lq = (size_t)4 * 64 * DP * sizeof(T), lk = lq + 6 * 64 * sizeof(float);
     if (int e = xa_lds(xa_dq_kernel<T, DP>, lq)) return e;
@@ -724,10 +1039,7 @@ static int xa_bwd_launch(const XaArgs& a, const XaPlan& q, hipStream_t s) {
     if (!a.dk || a.Lk == 0) return L2I_OK;
     if (int e = xa_lds(xa_dkv_kernel<T, DP>, lk)) return e;
     hipLaunchKernelGGL((xa_dkv_kernel<T, DP>), dim3(xa_grid(tk)), dim3(256), lk, s, a, q.nkt, tk);
-    if (a.ns > 1) {
-        const long long n = (long long)a.B * a.Hk * a.Lk * a.D;
-        hipLaunchKernelGGL((xa_fold_kernel<T>), dim3((unsigned)((n / 4 + 255) / 256), 2), dim3(256), 0, s, a);
-    }
+    if (a.ns > 1) xa_fold_launch<T>(a, s);
     return L2I_OK;
 }
 // strides: 16-byte steps between any two rows, so that every row starts on a 16-byte boundary; the rows of a tile (64 positions and the G heads
@@ -751,11 +1063,11 @@ extern "C" int l2i_cross_attention_fwd(const void* q, const void* k, const void*
     long long need = 0;
     if (xa_bad(B, Lq, Lk, Hk, G, D, dtype) || !q || !out || (Lk && (!k || !v)) || mb < 0 || mq < 0 || ((size_t)out & 15)) return L2I_ERR_ARG;
     if (!xa_rows_ok(q, qb, ql, qh, G, dtype) || !xa_rows_ok(k, kb, kl, kh, 0, dtype) || !xa_rows_ok(v, vb, vl, vh, 0, dtype)) return L2I_ERR_ARG;
-    if (l2i_cross_attention_scratch(B, Lq, Lk, Hk, G, D, 0, &need) != L2I_OK) return L2I_ERR_ARG;
+    if (l2i_cross_attention_scratch(B, Lq, Lk, Hk, G, D, dtype, 0, &need) != L2I_OK) return L2I_ERR_ARG;
     if (need && (!scratch || ((size_t)scratch & 15) || scratch_floats < need)) return L2I_ERR_ARG;
     XaArgs a = {};
     xa_setup(a, q, k, v, lengths, mask, B, Lq, Lk, Hk, G, D, qb, ql, qh, kb, kl, kh, vb, vl, vh, mb, mq, scale);
-    const XaPlan pl = xa_plan(B, a.R, Lk, Hk);
+    const XaPlan pl = xa_plan(B, a.R, Lk, Hk, D, dtype);
     a.o = out; a.lse = lse; a.ns = pl.ns;
     a.part = scratch; a.ml = scratch + (size_t)pl.ns * B * Hk * a.R * D;
     const int e = dtype ? xa_fwd_type<bf16_t>(a, pl, (hipStream_t)stream) : xa_fwd_type<float>(a, pl, (hipStream_t)stream);
@@ -769,10 +1081,10 @@ extern "C" int l2i_cross_attention_bwd(const void* q, const void* k, const void*
     if (xa_bad(B, Lq, Lk, Hk, G, D, dtype) || !q || !out || !lse || !dout || (Lk && (!k || !v)) || mb < 0 || mq < 0) return L2I_ERR_ARG;
     if ((dk == nullptr) != (dv == nullptr) || (((size_t)out | (size_t)dout | (size_t)dq | (size_t)dk | (size_t)dv) & 15)) return L2I_ERR_ARG;
     if (!xa_rows_ok(q, qb, ql, qh, G, dtype) || !xa_rows_ok(k, kb, kl, kh, 0, dtype) || !xa_rows_ok(v, vb, vl, vh, 0, dtype)) return L2I_ERR_ARG;
-    if (l2i_cross_attention_scratch(B, Lq, Lk, Hk, G, D, 1, &need) != L2I_OK || !scratch || ((size_t)scratch & 15) || scratch_floats < need) return L2I_ERR_ARG;
+    if (l2i_cross_attention_scratch(B, Lq, Lk, Hk, G, D, dtype, 1, &need) != L2I_OK || !scratch || ((size_t)scratch & 15) || scratch_floats < need) return L2I_ERR_ARG;
     XaArgs a = {};
     xa_setup(a, q, k, v, lengths, mask, B, Lq, Lk, Hk, G, D, qb, ql, qh, kb, kl, kh, vb, vl, vh, mb, mq, scale);
-    const XaPlan pl = xa_plan(B, a.R, Lk, Hk);
+    const XaPlan pl = xa_plan(B, a.R, Lk, Hk, D, dtype);
     a.o = const_cast<void*>(out); a.lse = const_cast<float*>(lse); a.g = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.ns = pl.nsb;
     a.delta = scratch; a.part = scratch + ((long long)B * Hk * a.R + 3) / 4 * 4;
     hipStream_t s = (hipStream_t)stream;

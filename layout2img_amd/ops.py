@@ -2155,7 +2155,7 @@ def _cross_attention_fwd(q, k, v, lengths, mask, scale, want_lse):
     sizes, strides = _xa_args(q, k, v, lengths, mask)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[0] * q.shape[1] * q.shape[2], dtype=torch.float32, device=q.device) if want_lse else None
-    ws, wp, wn = _scratch(q.device, "l2i_cross_attention_scratch", *sizes, 0)
+    ws, wp, wn = _scratch(q.device, "l2i_cross_attention_scratch", *sizes, _code(q.dtype), 0)
     _lib.call("l2i_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _code(q.dtype), _p(lengths), _p(mask), out.data_ptr(), _p(lse),
               *sizes, *strides, scale, wp, wn, _stream())
     return out, lse
@@ -2178,7 +2178,7 @@ class CrossAttentionFn(Function):
         nq, nk, nv = ctx.needs_input_grad[:3]
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if nq else None
         dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) if nk or nv else None for _ in range(2))
-        ws, wp, wn = _scratch(q.device, "l2i_cross_attention_scratch", *sizes, 1)
+        ws, wp, wn = _scratch(q.device, "l2i_cross_attention_scratch", *sizes, _code(q.dtype), 1)
         _lib.call("l2i_cross_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _code(q.dtype), _p(lengths), _p(mask), out.data_ptr(),
                   lse.data_ptr(), g.data_ptr(), _p(dq), _p(dk), _p(dv), *sizes, *strides, ctx.scale, wp, wn, _stream())
         return dq, dk if nk else None, dv if nv else None, None, None, None

@@ -152,14 +152,14 @@ def test_entry_points_refuse_before_a_launch():
 
 def test_scratch_sizes():
     assert _floats("l2i_group_norm_scratch", 2, 9, 8, 3, 0)[0] == -1
-    assert _floats("l2i_cross_attention_scratch", 1, 1, 1, 1, 1, 7, 0)[0] == -1
+    assert _floats("l2i_cross_attention_scratch", 1, 1, 1, 1, 1, 7, 1, 0)[0] == -1
     assert _floats("l2i_embedding_bwd_scratch", -1, 5, 8)[0] == -1
     for B, HW, C, G in ((1, 1, 1, 1), (32, 16384, 64, 32), (65535, 1, 4096, 1)):
         for bwd in (0, 1):
             rc, n = _floats("l2i_group_norm_scratch", B, HW, C, G, bwd)
             assert rc == 0 and 0 <= n < 1 << 31
-    assert _floats("l2i_cross_attention_scratch", 4, 4096, 2048, 4, 4, 128, 0) == (0, 0)   # rows enough: no splits
-    rc, n = _floats("l2i_cross_attention_scratch", 1, 1, 4096, 1, 1, 128, 0)
+    assert _floats("l2i_cross_attention_scratch", 4, 4096, 2048, 4, 4, 128, 1, 0) == (0, 0)   # rows enough: no splits
+    rc, n = _floats("l2i_cross_attention_scratch", 1, 1, 4096, 1, 1, 128, 1, 0)
     assert rc == 0 and n > 0
 
 
