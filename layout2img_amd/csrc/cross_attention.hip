@@ -55,23 +55,65 @@ __device__ __forceinline__ void xa_dot(f32x16_t& acc, const uint4& a, const uint
     acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), acc, 0, 0, 0);
     acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), acc, 0, 0, 0);
 }
-// acc[tile row row0 + ..][b's row] = sum over all dims
-template <typename T, int CH> __device__ __forceinline__ void xa_rows_dot(f32x16_t& acc, const char* tile, int row0, const uint4 (&b)[CH / 2]) {
-    const int lane = threadIdx.x & 63, h = lane >> 5;
+// The lane's places in a tile, as byte offsets: what differs by rows of 16 or 32, by tile or by buffer is a constant behind them, so that a read costs
+// no address arithmetic. row[s]: its chunk of step s of row lane % 32; tr[db][..]: see xa_tr; el: where a f32 value is counted from.
+template <typename T, int CH> struct XaAddr {
+    static constexpr int S = CH / 2, ND = CH * 16 / (int)sizeof(T) / 32;
+    int row[S], tr[sizeof(T) == 2 ? ND : 1][2], el = 0;
+    __device__ __forceinline__ XaAddr() {
+        const int lane = threadIdx.x & 63, h = lane >> 5, i = lane & 15, d16 = (lane >> 4) & 1;
+#pragma unroll
+        for (int s = 0; s < S; ++s) row[s] = xa_at<CH>(lane & 31, 2 * s + h);
+        if constexpr (sizeof(T) == 2) {
+            const int ra = 4 * h + (i >> 2);
+#pragma unroll
+            for (int db = 0; db < ND; ++db) {
+                const int chunk = db * 4 + d16 * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
+                tr[db][0] = xa_at<CH>(ra, chunk) + sub;
+                tr[db][1] = xa_at<CH>(ra + 8, chunk) + sub;
+            }
+        }
+    }
+    __device__ __forceinline__ void move(int bytes) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) row[s] += bytes;
+#pragma unroll
+        for (int db = 0; db < (sizeof(T) == 2 ? ND : 1); ++db) { tr[db][0] += bytes; tr[db][1] += bytes; }
+        el += bytes;
+    }
+};
+template <int NA> __device__ __forceinline__ void xa_zero(f32x16_t (&acc)[NA]) {
+#pragma unroll
+    for (int k = 0; k < NA; ++k)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[k][e] = 0.f;
+}
+__device__ __forceinline__ void xa_zero1(f32x16_t& acc) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+}
+// x = tile a . fa, y = tile b . fb (32 rows each): two chains of products, one behind the other in turn
+template <typename T, int CH>
+__device__ __forceinline__ void xa_rows_dot2(f32x16_t& x, f32x16_t& y, const char* a, const char* b, const XaAddr<T, CH>& ad, const uint4 (&fa)[CH / 2], const uint4 (&fb)[CH / 2]) {
+    xa_zero1(x); xa_zero1(y);
 #pragma unroll
-    for (int s = 0; s < CH / 2; ++s) xa_dot(acc, *reinterpret_cast<const uint4*>(tile + xa_at<CH>(row0 + (lane & 31), 2 * s + h)), b[s], T());
+    for (int s = 0; s < CH / 2; ++s) {
+        xa_dot(x, *reinterpret_cast<const uint4*>(a + ad.row[s]), fa[s], T());
+        xa_dot(y, *reinterpret_cast<const uint4*>(b + ad.row[s]), fb[s], T());
+    }
+}
+template <typename T, int CH> __device__ __forceinline__ void xa_rows_dot(f32x16_t& x, const char* a, const XaAddr<T, CH>& ad, const uint4 (&fa)[CH / 2]) {
+    xa_zero1(x);
+#pragma unroll
+    for (int s = 0; s < CH / 2; ++s) xa_dot(x, *reinterpret_cast<const uint4*>(a + ad.row[s]), fa[s], T());
 }
 
-// ---- bf16: the lane's column of 8 tile rows as a product operand: column 32 db + lane % 32, rows row0 + 16 t + 4 h + {0 .. 3} and 8 further on --
-// the order in which an accumulator's registers 8 t .. 8 t + 7 hold its rows
-template <int CH> __device__ __forceinline__ b16x8_t xa_tr(const char* tile, int row0, int t, int db) {
-    const int lane = threadIdx.x & 63, h = lane >> 5, i = lane & 15, d16 = (lane >> 4) & 1;
-    const int ra = row0 + 16 * t + 4 * h + (i >> 2), chunk = db * 4 + d16 * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
+// ---- bf16: the lane's column of 8 tile rows as a product operand: column 32 db + lane % 32, rows 4 h + {0 .. 3} and 8 further on (and 16 t behind
+// the tile pointer) -- the order in which an accumulator's registers 8 t .. 8 t + 7 hold its rows
+__device__ __forceinline__ b16x8_t xa_tr(const char* tile, const int (&at)[2]) {
     typedef __attribute__((address_space(3))) s16x4_t lds4_t;
-    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t*)(tile + xa_at<CH>(ra, chunk) + sub));
-    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t*)(tile + xa_at<CH>(ra + 8, chunk) + sub));
+    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t*)(tile + at[0]));
+    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t*)(tile + at[1]));
     bf16x8_t a;
 #pragma unroll
     for (int e = 0; e < 4; ++e) { a[e] = lo[e]; a[4 + e] = hi[e]; }
@@ -81,28 +123,26 @@ template <int CH> __device__ __forceinline__ float xa_el(const char* tile, int r
     return *reinterpret_cast<const float*>(tile + xa_at<CH>(row, col >> 2) + (col & 3) * 4);
 }
 
-// ---- acc[d][lane] += sum over 32 tile rows i of tile[row0 + i][d] p_i(lane); p: an accumulator (register r of a lane = row 8 (r / 4) + 4 (lane / 32) + r % 4)
+// ---- acc[d][lane] += sum over 32 tile rows i of tile[i][d] p_i(lane); p: an accumulator (register r of a lane = row 8 (r / 4) + 4 (lane / 32) + r % 4)
 template <int CH, int ND>
-__device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, int row0, const f32x16_t& p, bf16_t) {
+__device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, const XaAddr<bf16_t, CH>& ad, const f32x16_t& p) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         uint4 pb;
         pb.x = f2bf2(p[8 * t], p[8 * t + 1]); pb.y = f2bf2(p[8 * t + 2], p[8 * t + 3]);
         pb.z = f2bf2(p[8 * t + 4], p[8 * t + 5]); pb.w = f2bf2(p[8 * t + 6], p[8 * t + 7]);
 #pragma unroll
-        for (int db = 0; db < ND; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa_tr<CH>(tile, row0, t, db), __builtin_bit_cast(b16x8_t, pb), acc[db], 0, 0, 0);
+        for (int db = 0; db < ND; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa_tr(tile + 16 * t * CH * 16, ad.tr[db]), __builtin_bit_cast(b16x8_t, pb), acc[db], 0, 0, 0);
     }
 }
 template <int CH, int ND>
-__device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, int row0, const f32x16_t& p, float) {
+__device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, const XaAddr<float, CH>& ad, const f32x16_t& p) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const int row = row0 + 8 * (r >> 2) + 4 * h + (r & 3);
+        const int row = 8 * (r >> 2) + 4 * h + (r & 3);
 #pragma unroll
-        for (int db = 0; db < ND; ++db) {
-            acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(xa_el<CH>(tile, row, db * 32 + (lane & 31)), p[r], acc[db], 0, 0, 0);
-        }
+        for (int db = 0; db < ND; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(xa_el<CH>(tile + ad.el, row, db * 32 + (lane & 31)), p[r], acc[db], 0, 0, 0);
     }
 }
 // ---- the same with p from a second tile of 32 rows x 32 columns (row i, column = lane): what an accumulator's transpose is, through LDS
@@ -119,15 +159,17 @@ template <typename T> struct XaSquare {
         asm volatile("" ::: "memory");   // (the wave's own LDS accesses run in order; the compiler keeps them so)
     }
 };
-template <int CH, int ND> __device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, const char* sq, bf16_t) {
+template <int CH, int ND>
+__device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, const XaAddr<bf16_t, CH>& ad, const char* sq, const XaAddr<bf16_t, 4>& as) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        const b16x8_t pb = xa_tr<XaSquare<bf16_t>::CH>(sq, 0, t, 0);
+        const b16x8_t pb = xa_tr(sq + 16 * t * 4 * 16, as.tr[0]);
 #pragma unroll
-        for (int db = 0; db < ND; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa_tr<CH>(tile, 0, t, db), pb, acc[db], 0, 0, 0);
+        for (int db = 0; db < ND; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa_tr(tile + 16 * t * CH * 16, ad.tr[db]), pb, acc[db], 0, 0, 0);
     }
 }
-template <int CH, int ND> __device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, const char* sq, float) {
+template <int CH, int ND>
+__device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, const XaAddr<float, CH>&, const char* sq, const XaAddr<float, 8>&) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -283,8 +325,7 @@ __global__ __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : (sizeof
     const int nt = (st.len + KT - 1) / KT, per = (nt + p.ns - 1) / p.ns;
     const int t0 = split * per + (WQ == 4 ? 0 : wave), t1 = min(nt, split * per + per);
     const unsigned char* mrow = st.mb && !st.kmask ? st.mb + (long long)iq * p.mq : nullptr;   // (null or not: the same for the whole launch)
-    char* tiles = smem + (WQ == 4 ? 0 : wave * 2 * Tile::BYTES * NBUF);
-    const unsigned lds = lds_addr_of(tiles);
+    const unsigned lds = lds_addr_of(smem) + (WQ == 4 ? 0 : wave * 2 * Tile::BYTES * NBUF);
     XaDma<T, CH, KT, TH> dk, dv;
     dk.init(p.kl, p.D);
     dv.init(p.vl, p.D);
@@ -303,73 +344,87 @@ __global__ __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : (sizeof
     if (t0 < t1) issue(t0, 0);
     uint4 qf[S];
     xa_row_frag<T, CH>(qf, r < p.R ? reinterpret_cast<const T*>(p.q) + b * p.qb + (long long)iq * p.ql + head * p.qh : nullptr, p.D, p.scale < 0.f);
+    XaAddr<T, CH> ad;
+    if (WQ == 1) ad.move(wave * 2 * Tile::BYTES * NBUF);
     f32x16_t oacc[ND];
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) oacc[d][e] = 0.f;
+    xa_zero(oacc);
     float m = -INFINITY, l = 0.f;
-    int buf = 0;
-    for (int t = t0; t < t1; t += STEP) {
-        const int jl = t * KT + lane;
-        const unsigned long long kbits = __ballot(lane < KT && st.live(jl));
-        const bool all = !mrow && kbits == (KT == 64 ? ~0ull : 0xffffffffull);
-        unsigned live[KT / 32];
-        if (!all)
+    // one tile from the buffer at ks; live: its bits where `masked`
+    auto work = [&](auto masked, const char* ks, const unsigned (&live)[KT / 32]) {
+        constexpr bool M = decltype(masked)::value;
+        const char* vs = ks + Tile::BYTES;
+        f32x16_t sc[KT / 32];
+        if constexpr (KT == 64) xa_rows_dot2<T, CH>(sc[0], sc[1], ks, ks + 32 * CH * 16, ad, qf, qf);
+        else xa_rows_dot<T, CH>(sc[0], ks, ad, qf);
+        float tm = -INFINITY;
 #pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) live[kb] = xa_live((unsigned)(kbits >> (32 * kb)), mrow, t * KT + 32 * kb, p.Lk);
+        for (int kb = 0; kb < KT / 32; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                if constexpr (M) sc[kb][e] = xa_pick(live[kb], e, sc[kb][e], XA_NINF);
+                tm = fmaxf(tm, sc[kb][e]);
+            }
+        tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+        tm = M && tm == -INFINITY ? tm : tm * p.c;   // (c may be 0)
+        if (__any(tm > m + 8.f)) {   // the reference moves only when it has to: what is summed stays below 2^8
+            const float mn = fmaxf(m, tm), al = xa_exp2(m - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) oacc[d][e] *= al;
+        }
+        const float ref = M && m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int kb = 0; kb < KT / 32; ++kb) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float x = fmaf(sc[kb][e], p.c, -ref);
+                if constexpr (M) x = xa_pick(live[kb], e, x, XA_NINF);
+                sc[kb][e] = xa_exp2(x);
+                l += sc[kb][e];
+            }
+            xa_tdot<CH, ND>(oacc, vs + kb * 32 * CH * 16, ad, sc[kb]);
+        }
+    };
+    // the tile's data has come; the next one's is sent for
+    auto turn = [&](int t, int buf) {
         if (WQ == 4) {
             xa_wait_dma<0>();
             __syncthreads();
-            if (t + STEP < t1) issue(t + STEP, buf ^ 1);
+            if (NBUF == 2 && t + STEP < t1) issue(t + STEP, buf ^ 1);
         } else if (NBUF == 2 && t + STEP < t1) {
             issue(t + STEP, buf ^ 1);
             xa_wait_dma<2 * XaDma<T, CH, KT, TH>::N>();
         } else {
             xa_wait_dma<0>();
         }
-        const char *ks = tiles + buf * 2 * Tile::BYTES, *vs = ks + Tile::BYTES;
-        auto body = [&](auto masked) {
-            f32x16_t sc[KT / 32];
+    };
+    const unsigned none[KT / 32] = {};
+    const int tf = st.mb ? t0 : min(t1, st.len / KT);   // tiles below tf have no dead key
+    int t = t0;
+    if (NBUF == 2)
+        for (; t + STEP < tf; t += 2 * STEP) {   // two tiles a round: the buffers' addresses are constants
+            turn(t, 0);
+            work(std::false_type(), smem, none);
+            turn(t + STEP, 1);
+            work(std::false_type(), smem + 2 * Tile::BYTES, none);
+        }
+    int buf = 0;
+    for (; t < t1; t += STEP) {
+        const int jl = t * KT + lane;
+        const unsigned long long kbits = __ballot(lane < KT && st.live(jl));
+        unsigned live[KT / 32];
 #pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) xa_rows_dot<T, CH>(sc[kb], ks, kb * 32, qf);
-            float tm = -INFINITY;
-#pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    if constexpr (decltype(masked)::value) sc[kb][e] = xa_pick(live[kb], e, sc[kb][e], XA_NINF);
-                    tm = fmaxf(tm, sc[kb][e]);
-                }
-            tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
-            tm = tm == -INFINITY ? tm : tm * p.c;   // (c may be 0)
-            if (__ballot(tm > m + 8.f || (m == -INFINITY && tm > m))) {   // the reference moves only when it has to: scores stay below 2^8
-                const float mn = fmaxf(m, tm), al = xa_exp2(m - (mn == -INFINITY ? 0.f : mn));
-                m = mn;
-                l *= al;
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) oacc[d][e] *= al;
-            }
-            const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float x = fmaf(sc[kb][e], p.c, -ref);
-                    if constexpr (decltype(masked)::value) x = xa_pick(live[kb], e, x, XA_NINF);
-                    sc[kb][e] = xa_exp2(x);
-                    l += sc[kb][e];
-                }
-                xa_tdot<CH, ND>(oacc, vs, kb * 32, sc[kb], T());
-            }
-        };
-        if (all) body(std::false_type());
-        else body(std::true_type());
+        for (int kb = 0; kb < KT / 32; ++kb) live[kb] = xa_live((unsigned)(kbits >> (32 * kb)), mrow, t * KT + 32 * kb, p.Lk);
+        turn(t, buf);
+        work(std::true_type(), smem + buf * 2 * Tile::BYTES, live);
         if (NBUF == 2) buf ^= 1;
-        else if (WQ == 4) __syncthreads();
-        if (NBUF == 1 && WQ == 1 && t + STEP < t1) issue(t + STEP, 0);
+        else if (t + STEP < t1) {
+            if (WQ == 4) __syncthreads();
+            issue(t + STEP, 0);
+        }
     }
     xa_settle();
     l += __shfl_xor(l, 32, 64);
@@ -507,39 +562,45 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_d
     }
     const float ls = on ? p.lse[(size_t)bh * p.R + r] : INFINITY;
     if (on && h == 0) p.delta[(size_t)bh * p.R + r] = dl;
+    XaAddr<T, CH> ad;
     f32x16_t acc[ND];
+    xa_zero(acc);
+    auto work = [&](auto masked, const char* ks, const unsigned (&live)[2]) {
+        const char* vs = ks + BYTES;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+        for (int kb = 0; kb < 2; ++kb) {
+            f32x16_t sc, dp;
+            xa_rows_dot2<T, CH>(sc, dp, ks + kb * 32 * CH * 16, vs + kb * 32 * CH * 16, ad, qf, gf);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
-    for (int t = 0; t < nt; ++t) {
-        const int jl = t * KT + lane;
-        const unsigned long long kbits = __ballot(st.live(jl));
-        const bool all = !mrow && kbits == ~0ull;
-        unsigned live[2];
-        if (!all)
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) live[kb] = xa_live((unsigned)(kbits >> (32 * kb)), mrow, t * KT + 32 * kb, p.Lk);
+            for (int e = 0; e < 16; ++e) {
+                sc[e] = xa_exp2(fmaf(sc[e], p.c, -ls)) * (dp[e] - dl);
+                if constexpr (decltype(masked)::value) sc[e] = xa_pick(live[kb], e, sc[e], 0u);
+            }
+            xa_tdot<CH, ND>(acc, ks + kb * 32 * CH * 16, ad, sc);
+            __builtin_amdgcn_sched_barrier(0);   // (one block of 32 keys at a time: two would not fit the registers)
+        }
+    };
+    auto turn = [&](int t, int buf) {
         xa_wait_dma<0>();
         __syncthreads();
-        if (t + 1 < nt) issue(t + 1, (t + 1) & 1);
-        const char *ks = smem + (t & 1) * 2 * BYTES, *vs = ks + BYTES;
-        auto body = [&](auto masked) {
-#pragma unroll 1
-            for (int kb = 0; kb < 2; ++kb) {
-                f32x16_t sc, dp;
-                xa_rows_dot<T, CH>(sc, ks, kb * 32, qf);
-                xa_rows_dot<T, CH>(dp, vs, kb * 32, gf);
+        if (t + 1 < nt) issue(t + 1, buf ^ 1);
+    };
+    const unsigned none[2] = {};
+    const int tf = st.mb ? 0 : min(nt, st.len / KT);
+    int t = 0;
+    for (; t + 1 < tf; t += 2) {
+        turn(t, 0);
+        work(std::false_type(), smem, none);
+        turn(t + 1, 1);
+        work(std::false_type(), smem + 2 * BYTES, none);
+    }
+    for (int buf = 0; t < nt; ++t, buf ^= 1) {
+        const unsigned long long kbits = __ballot(st.live(t * KT + lane));
+        unsigned live[2];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    sc[e] = xa_exp2(fmaf(sc[e], p.c, -ls)) * (dp[e] - dl);
-                    if constexpr (decltype(masked)::value) sc[e] = xa_pick(kb ? live[1] : live[0], e, sc[e], 0u);
-                }
-                xa_tdot<CH, ND>(acc, ks, kb * 32, sc, T());
-            }
-        };
-        if (all) body(std::false_type());
-        else body(std::true_type());
+        for (int kb = 0; kb < 2; ++kb) live[kb] = xa_live((unsigned)(kbits >> (32 * kb)), mrow, t * KT + 32 * kb, p.Lk);
+        turn(t, buf);
+        work(std::true_type(), smem + buf * 2 * BYTES, live);
     }
     xa_settle();
     if (!on || !p.dq) return;
@@ -613,51 +674,59 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_d
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) { dk[d][e] = 0.f; dv[d][e] = 0.f; }
-    const bool all = !qmask && __ballot(klive) == ~0ull;
-    int buf = 0;
-    for (int t = t0; t < t1; ++t) {
+    XaAddr<T, CH> ad;
+    auto work = [&](auto masked, const char* qs, const float* rv) {
+        const char* gs = qs + BYTES;
+#pragma unroll
+        for (int row0 = 0; row0 < RT; row0 += 32) {
+            unsigned live = 0;
+            if constexpr (decltype(masked)::value) {
+                live = klive ? 0xffffu : 0u;
+                if (qmask && klive) {
+                    live = 0;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        live |= (st.mb[(long long)reinterpret_cast<const int*>(rv)[2 * RT + row0 + 8 * (e >> 2) + 4 * h + (e & 3)] * p.mq + key] != 0 ? 1u : 0u) << e;
+                }
+            }
+            f32x16_t pr, ds;
+            xa_rows_dot2<T, CH>(pr, ds, qs + row0 * CH * 16, gs + row0 * CH * 16, ad, kf, vf);
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const float4 ls = *reinterpret_cast<const float4*>(rv + row0 + 8 * a + 4 * h), dl = *reinterpret_cast<const float4*>(rv + RT + row0 + 8 * a + 4 * h);
+                const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dd[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 4 * a + i;
+                    pr[e] = xa_exp2(fmaf(pr[e], p.c, -lv[i]));
+                    if constexpr (decltype(masked)::value) pr[e] = xa_pick(live, e, pr[e], 0u);
+                    ds[e] = pr[e] * (ds[e] - dd[i]);
+                    if constexpr (decltype(masked)::value) ds[e] = xa_pick(live, e, ds[e], 0u);
+                }
+            }
+            xa_tdot<CH, ND>(dv, gs + row0 * CH * 16, ad, pr);
+            xa_tdot<CH, ND>(dk, qs + row0 * CH * 16, ad, ds);
+            __builtin_amdgcn_sched_barrier(0);   // (32 rows at a time: 64 would not fit the registers)
+        }
+    };
+    auto turn = [&](int t, int buf) {
         float* rv = rowv + buf * 3 * RT;
         if (threadIdx.x < RT) { rv[threadIdx.x] = nls; rv[RT + threadIdx.x] = ndl; reinterpret_cast<int*>(rv)[2 * RT + threadIdx.x] = niq; }
         xa_wait_dma<0>();
         __syncthreads();
         if (t + 1 < t1) issue(t + 1, buf ^ 1);
-        const char *qs = smem + buf * 2 * BYTES, *gs = qs + BYTES;
-        auto body = [&](auto masked) {
-#pragma unroll 1
-            for (int row0 = 0; row0 < RT; row0 += 32) {
-                unsigned live = 0;
-                if constexpr (decltype(masked)::value) {
-                    live = klive ? 0xffffu : 0u;
-                    if (qmask && klive) {
-                        live = 0;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            live |= (st.mb[(long long)reinterpret_cast<const int*>(rv)[2 * RT + row0 + 8 * (e >> 2) + 4 * h + (e & 3)] * p.mq + key] != 0 ? 1u : 0u) << e;
-                    }
-                }
-                f32x16_t pr, ds;
-                xa_rows_dot<T, CH>(pr, qs, row0, kf);
-                xa_rows_dot<T, CH>(ds, gs, row0, vf);
-#pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    const float4 ls = *reinterpret_cast<const float4*>(rv + row0 + 8 * a + 4 * h), dl = *reinterpret_cast<const float4*>(rv + RT + row0 + 8 * a + 4 * h);
-                    const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dd[4] = {dl.x, dl.y, dl.z, dl.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int e = 4 * a + i;
-                        pr[e] = xa_exp2(fmaf(pr[e], p.c, -lv[i]));
-                        if constexpr (decltype(masked)::value) pr[e] = xa_pick(live, e, pr[e], 0u);
-                        ds[e] = pr[e] * (ds[e] - dd[i]);
-                        if constexpr (decltype(masked)::value) ds[e] = xa_pick(live, e, ds[e], 0u);
-                    }
-                }
-                xa_tdot<CH, ND>(dv, gs, row0, pr, T());
-                xa_tdot<CH, ND>(dk, qs, row0, ds, T());
-            }
-        };
-        if (all) body(std::false_type());
-        else body(std::true_type());
-        buf ^= 1;
+    };
+    int t = t0;
+    if (!qmask && __ballot(klive) == ~0ull)
+        for (; t + 1 < t1; t += 2) {
+            turn(t, 0);
+            work(std::false_type(), smem, rowv);
+            turn(t + 1, 1);
+            work(std::false_type(), smem + 2 * BYTES, rowv + 3 * RT);
+        }
+    for (int buf = 0; t < t1; ++t, buf ^= 1) {
+        turn(t, buf);
+        work(std::true_type(), smem + buf * 2 * BYTES, rowv + buf * 3 * RT);
     }
     xa_settle();
     if (key >= p.Lk) return;
@@ -742,6 +811,7 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 2 : 4) void xa_s
     xa_stage32<T, CH>(ks, st.k, p.kl, p.D, st);
     xa_stage32<T, CH>(vs, st.v, p.vl, p.D, st);
     __syncthreads();
+    const XaAddr<T, CH> ad;
     for (; blk < nblk; blk += step) {
         uint4 qf[S];
 #pragma unroll
@@ -749,7 +819,7 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 2 : 4) void xa_s
         const unsigned live = nlive;
         if (blk + step < nblk) fetch(blk + step);
         f32x16_t sc, oacc[ND];
-        xa_rows_dot<T, CH>(sc, ks, 0, qf);
+        xa_rows_dot<T, CH>(sc, ks, ad, qf);
         float m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) { sc[e] = xa_pick(live, e, sc[e], XA_NINF); m = fmaxf(m, sc[e]); }
@@ -762,7 +832,7 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 2 : 4) void xa_s
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) oacc[d][e] = 0.f;
-        xa_tdot<CH, ND>(oacc, vs, 0, sc, T());
+        xa_tdot<CH, ND>(oacc, vs, ad, sc);
         const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -834,6 +904,8 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : DP == 64 ? 2
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) { dk[d][e] = 0.f; dv[d][e] = 0.f; }
+    const XaAddr<T, CH> ad;
+    const XaAddr<T, XaSquare<T>::CH> as;
     for (; blk < nblk; blk += step) {
         const int r = blk * 32 + (lane & 31);
         const bool on = r < p.R;
@@ -851,14 +923,12 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : DP == 64 ? 2
         const unsigned flip = p.scale < 0.f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const int at = xa_at<CH>(lane & 31, 2 * s + h);
-            qf[s] = *reinterpret_cast<const uint4*>(qs + at);
-            gf[s] = *reinterpret_cast<const uint4*>(gs + at);
+            qf[s] = *reinterpret_cast<const uint4*>(qs + ad.row[s]);
+            gf[s] = *reinterpret_cast<const uint4*>(gs + ad.row[s]);
             qf[s].x ^= flip; qf[s].y ^= flip; qf[s].z ^= flip; qf[s].w ^= flip;
         }
         f32x16_t sc, dp, dqa[ND];
-        xa_rows_dot<T, CH>(sc, ks, 0, qf);
-        xa_rows_dot<T, CH>(dp, vs, 0, gf);
+        xa_rows_dot2<T, CH>(sc, dp, ks, vs, ad, qf, gf);
         float dl = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -874,9 +944,9 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : DP == 64 ? 2
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) dqa[d][e] = 0.f;
-        xa_tdot<CH, ND>(dqa, ks, 0, sc, T());
-        xa_tdot<CH, ND>(dv, gs, sp, T());
-        xa_tdot<CH, ND>(dk, qs, sd, T());
+        xa_tdot<CH, ND>(dqa, ks, ad, sc);
+        xa_tdot<CH, ND>(dv, gs, ad, sp, as);
+        xa_tdot<CH, ND>(dk, qs, ad, sd, as);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
