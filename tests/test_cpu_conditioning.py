@@ -141,7 +141,7 @@ def test_entry_points_refuse_before_a_launch():
     for bad in (dict(w=None), dict(t=None), dict(o=None), dict(wd=3), dict(od=2), dict(n=-1), dict(n=1 << 31), dict(V=0), dict(V=0x7fffffff), dict(D=0), dict(D=65537)):
         assert ef(**bad) == -1, bad
     assert ef(n=0) == 0
-    eb = lambda t=P, dy=P, dw=P, n=3, V=5, D=8, s=P, sn=big: lib.l2i_embedding_bwd(t, dy, 0, dw, 0, n, V, D, 1.0, -1, s, sn, None)
+    eb = lambda t=P, dy=P, dw=P, n=3000, V=5, D=8, s=P, sn=big: lib.l2i_embedding_bwd(t, dy, 0, dw, 0, n, V, D, 1.0, -1, s, sn, None)
     for bad in (dict(t=None), dict(dy=None), dict(dw=None), dict(n=-1), dict(n=0x7fffffff), dict(V=0), dict(D=0), dict(s=None), dict(s=P + 4), dict(sn=3)):
         assert eb(**bad) == -1, bad
     dr = lambda x=P, xd=0, o=P, od=0, r=P, n=5, t=7, layer=0: lib.l2i_dropout(x, xd, None, o, od, r, None, n, t, 1.0, layer, None)
