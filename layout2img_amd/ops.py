@@ -2042,10 +2042,11 @@ def _op(t, what, *dtypes):
 
 def _same_device(t, *others):
     """Every tensor of a call lives on the current device (behind the checks of shapes and types, which need none)."""
-    dev = _lib.current_device() if t.is_cuda else None
-    for o in (t,) + others:
-        if o is not None and (not o.is_cuda or o.device.index != dev):
-            _chk(o)   # (its message)
+    dev = t.get_device()
+    if dev < 0 or dev != _lib.current_device():
+        _chk(t.new_empty(0))   # (its message)
+    for o in others:
+        if o is not None and o.get_device() != dev:
             raise RuntimeError(f"tensors of one call on {t.device} and {o.device}")
 
 
@@ -2073,43 +2074,49 @@ def _scratch(device, name, *sizes):
 
 
 def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
-def _group_norm_fwd(x, groups, weight, bias, eps, act, op_dtype):
-    B, C = x.shape[0], x.shape[-1]
-    HW = x.numel() // (B * C)
-    y = torch.empty(x.shape, dtype=op_dtype, device=x.device)
-    st = torch.empty((2, B, groups), dtype=torch.float32, device=x.device)
-    ws, wp, wn = _scratch(x.device, "l2i_group_norm_scratch", B, HW, C, groups, 0)
-    _lib.call("l2i_group_norm_fwd", x.data_ptr(), _code(x.dtype), _p(weight), _p(bias), y.data_ptr(), _code(op_dtype), st[0].data_ptr(),
-              st[1].data_ptr(), B, HW, C, groups, float(eps), act, wp, wn, _stream())
+def _group_norm_fwd(x, sizes, weight, bias, eps, act, op_dtype):
+    """sizes: (B, HW, C, G). -> y, (2, B, G) mean and rstd"""
+    B, HW, C, G = sizes
+    dev = x.device
+    y = torch.empty(x.shape, dtype=op_dtype, device=dev)
+    st = torch.empty((2, B, G), dtype=torch.float32, device=dev)
+    mean = st.data_ptr()
+    ws, wp, wn = _scratch(dev, "l2i_group_norm_scratch", B, HW, C, G, 0)
+    _lib.call("l2i_group_norm_fwd", x.data_ptr(), _code(x.dtype), _p(weight), _p(bias), y.data_ptr(), _code(op_dtype), mean, mean + 4 * B * G,
+              B, HW, C, G, eps, act, wp, wn, _stream())
     return y, st
 
 
 class GroupNormActFn(Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act, op_dtype):
-        y, st = _group_norm_fwd(x, groups, weight, bias, eps, act, op_dtype)
+    def forward(ctx, x, weight, bias, sizes, eps, act, op_dtype):
+        y, st = _group_norm_fwd(x, sizes, weight, bias, eps, act, op_dtype)
         ctx.save_for_backward(x, weight, bias, st)
-        ctx.cfg = (groups, act, op_dtype)
+        ctx.cfg = (sizes, act, _code(op_dtype))
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, st = ctx.saved_tensors
-        groups, act, op_dtype = ctx.cfg
+        sizes, act, y_code = ctx.cfg
+        B, HW, C, G = sizes
         dy = dy.contiguous()
-        B, C = x.shape[0], x.shape[-1]
-        HW = x.numel() // (B * C)
         nx, nw, nb = ctx.needs_input_grad[:3]
         dx = torch.empty_like(x) if nx else None
         dw = torch.empty_like(weight) if nw else None
         db = torch.empty_like(bias) if nb else None
-        ws, wp, wn = _scratch(x.device, "l2i_group_norm_scratch", B, HW, C, groups, 1)
-        _lib.call("l2i_group_norm_bwd", x.data_ptr(), _code(x.dtype), _p(weight), _p(bias), st[0].data_ptr(), st[1].data_ptr(), dy.data_ptr(),
-                  _code(op_dtype), _p(dx), _p(dw), _p(db), B, HW, C, groups, act, wp, wn, _stream())
+        ws, wp, wn = _scratch(x.device, "l2i_group_norm_scratch", B, HW, C, G, 1)
+        mean = st.data_ptr()
+        _lib.call("l2i_group_norm_bwd", x.data_ptr(), _code(x.dtype), _p(weight), _p(bias), mean, mean + 4 * B * G, dy.data_ptr(), y_code, _p(dx),
+                  _p(dw), _p(db), B, HW, C, G, act, wp, wn, _stream())
         return dx, dw, db, None, None, None, None
 
 
@@ -2121,67 +2128,70 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act=None, op_dty
     op_dtype = _op_dtype(op_dtype, x.dtype, "group_norm_act")
     if x.dim() < 2 or x.numel() == 0 or not x.is_contiguous():
         raise RuntimeError(f"group_norm_act: a contiguous (B, ..., C) map with values expected, got {tuple(x.shape)}, strides {x.stride()}")
-    C = x.shape[-1]
+    B, C = x.shape[0], x.shape[-1]
     if not isinstance(groups, int) or groups < 1 or C % groups:
         raise RuntimeError(f"group_norm_act: {C} channels do not divide into {groups} groups")
-    if C > 4096 or x.shape[0] > 65535:
-        raise RuntimeError(f"group_norm_act: at most 4096 channels and 65535 images, got {C} and {x.shape[0]}")
+    if C > 4096 or B > 65535:
+        raise RuntimeError(f"group_norm_act: at most 4096 channels and 65535 images, got {C} and {B}")
     if act not in _ACTS:
         raise RuntimeError(f"group_norm_act: act is None, 'relu' or 'silu', got {act!r}")
-    for t, what in ((weight, "weight"), (bias, "bias")):
-        if t is not None and (_op(t, "group_norm_act: " + what, torch.float32).shape != (C,) or not t.is_contiguous()):
-            raise RuntimeError(f"group_norm_act: {what} is a contiguous ({C},) tensor, got {tuple(t.shape)}, strides {t.stride()}")
+    for t, what in ((weight, "group_norm_act: weight"), (bias, "group_norm_act: bias")):
+        if t is not None and (_op(t, what, torch.float32).shape != (C,) or not t.is_contiguous()):
+            raise RuntimeError(f"{what} is a contiguous ({C},) tensor, got {tuple(t.shape)}, strides {t.stride()}")
     _same_device(x, weight, bias)
+    sizes, eps = (B, x.numel() // (B * C), C, groups), float(eps)
     if _wants_grad(x, weight, bias):
-        return GroupNormActFn.apply(x, weight, bias, groups, eps, _ACTS[act], op_dtype)
-    return _group_norm_fwd(x, groups, weight, bias, eps, _ACTS[act], op_dtype)[0]
+        return GroupNormActFn.apply(x, weight, bias, sizes, eps, _ACTS[act], op_dtype)
+    return _group_norm_fwd(x, sizes, weight, bias, eps, _ACTS[act], op_dtype)[0]
 
 
-def _strides3(t):
-    """Element strides of (batch, position, head); a dimension of one has none."""
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3]))
+def _strides3(t, what):
+    """Element strides of (batch, position, head), 0 for a dimension of one; refuses what the kernels do not read."""
+    s, n = t.stride(), t.shape
+    r = (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+    if s[3] != 1 or (r[0] | r[1] | r[2]) & (7 if t.dtype is torch.bfloat16 else 3) or t.data_ptr() & 15:
+        raise RuntimeError(f"cross_attention: {what} needs consecutive head values and rows on 16-byte boundaries, got strides {s} "
+                           f"at address {t.data_ptr() % 16} modulo 16 (.contiguous() first)")
+    if r[1] >= 1 << 22 or r[2] >= 1 << 28:
+        raise RuntimeError(f"cross_attention: {what} steps by less than 2^22 values from position to position and 2^28 from head to head, got {s}")
+    return r
 
 
-def _xa_args(q, k, v, lengths, mask):
-    B, Lq, H, D = q.shape
-    Lk, Hk = k.shape[1], k.shape[2]
-    mb = mq = 0
-    if mask is not None:
-        mb, mq = (s if n > 1 else 0 for s, n in zip(mask.stride()[:2], mask.shape[:2]))
-    return (B, Lq, Lk, Hk, H // Hk, D), _strides3(q) + _strides3(k) + _strides3(v) + (mb, mq)
-
-
-def _cross_attention_fwd(q, k, v, lengths, mask, scale, want_lse):
-    sizes, strides = _xa_args(q, k, v, lengths, mask)
+def _cross_attention_fwd(q, k, v, lengths, mask, scale, args, want_lse):
+    """args: (B, Lq, Lk, Hk, G, D) and the strides, as the library takes them."""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[0] * q.shape[1] * q.shape[2], dtype=torch.float32, device=q.device) if want_lse else None
-    ws, wp, wn = _scratch(q.device, "l2i_cross_attention_scratch", *sizes, _code(q.dtype), 0)
-    _lib.call("l2i_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _code(q.dtype), _p(lengths), _p(mask), out.data_ptr(), _p(lse),
-              *sizes, *strides, scale, wp, wn, _stream())
+    lse = torch.empty(args[0] * args[1] * args[3] * args[4], dtype=torch.float32, device=q.device) if want_lse else None
+    code = _code(q.dtype)
+    ws, wp, wn = _scratch(q.device, "l2i_cross_attention_scratch", *args[:6], code, 0)
+    _lib.call("l2i_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, _p(lengths), _p(mask), out.data_ptr(), _p(lse),
+              *args, scale, wp, wn, _stream())
     return out, lse
 
 
 class CrossAttentionFn(Function):
     @staticmethod
-    def forward(ctx, q, k, v, lengths, mask, scale):
-        out, lse = _cross_attention_fwd(q, k, v, lengths, mask, scale, True)
+    def forward(ctx, q, k, v, lengths, mask, scale, args):
+        out, lse = _cross_attention_fwd(q, k, v, lengths, mask, scale, args, True)
         ctx.save_for_backward(q, k, v, lengths, mask, out, lse)
-        ctx.scale = scale
+        ctx.cfg = (scale, args)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         q, k, v, lengths, mask, out, lse = ctx.saved_tensors
-        sizes, strides = _xa_args(q, k, v, lengths, mask)
+        scale, args = ctx.cfg
         g = _aligned(g.contiguous())
         nq, nk, nv = ctx.needs_input_grad[:3]
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if nq else None
-        dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) if nk or nv else None for _ in range(2))
-        ws, wp, wn = _scratch(q.device, "l2i_cross_attention_scratch", *sizes, _code(q.dtype), 1)
-        _lib.call("l2i_cross_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _code(q.dtype), _p(lengths), _p(mask), out.data_ptr(),
-                  lse.data_ptr(), g.data_ptr(), _p(dq), _p(dk), _p(dv), *sizes, *strides, ctx.scale, wp, wn, _stream())
-        return dq, dk if nk else None, dv if nv else None, None, None, None
+        dev, dtype, code = q.device, q.dtype, _code(q.dtype)
+        dq = torch.empty(q.shape, dtype=dtype, device=dev) if nq else None
+        dk = dv = None
+        if nk or nv:
+            dk, dv = torch.empty(k.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev)
+        ws, wp, wn = _scratch(dev, "l2i_cross_attention_scratch", *args[:6], code, 1)
+        _lib.call("l2i_cross_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, _p(lengths), _p(mask), out.data_ptr(),
+                  lse.data_ptr(), g.data_ptr(), _p(dq), _p(dk), _p(dv), *args, scale, wp, wn, _stream())
+        return dq, dk if nk else None, dv if nv else None, None, None, None, None
 
 
 def _aligned(t):
@@ -2195,11 +2205,10 @@ def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
     lengths: (B,) int32, states at and behind a sequence's length do not exist. mask: (B | 1, Lq | 1, Lk) bool, False = query i does not see state j.
     A query that sees no state gives zeros. What `lengths` or a mask row shared by all queries takes out is not read, whatever it holds; a state
     that only some queries see has to be finite. The D values of a head are consecutive; the other strides may be any of whole 16 bytes (slices of
-    a grouped projection, transposed heads, expanded batches)."""
-    for t, what in ((q, "q"), (k, "k"), (v, "v")):
-        _op(t, "cross_attention: " + what)
-        if t.dim() != 4:
-            raise RuntimeError(f"cross_attention: {what} is (B, L, heads, D), got {tuple(t.shape)}")
+    a grouped projection, transposed heads, expanded batches), less than 2^22 values from position to position."""
+    for t, what in ((q, "cross_attention: q"), (k, "cross_attention: k"), (v, "cross_attention: v")):
+        if _op(t, what).dim() != 4:
+            raise RuntimeError(f"{what} is (B, L, heads, D), got {tuple(t.shape)}")
         if t.dtype != q.dtype:
             raise RuntimeError(f"cross_attention: q, k, v have one type, got {q.dtype} and {t.dtype}")
     B, Lq, H, D = q.shape
@@ -2212,11 +2221,7 @@ def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
         raise RuntimeError(f"cross_attention: {H} query heads do not divide over {Hk} state heads")
     if B < 1 or Lq < 1:
         raise RuntimeError(f"cross_attention: at least one query, got {tuple(q.shape)}")
-    for t, what in ((q, "q"), (k, "k"), (v, "v")):
-        step = 16 // t.element_size()
-        if t.stride(3) != 1 or any(s % step for s in _strides3(t)) or t.data_ptr() % 16:
-            raise RuntimeError(f"cross_attention: {what} needs consecutive head values and rows on 16-byte boundaries, got strides {t.stride()} "
-                               f"at address {t.data_ptr() % 16} modulo 16 (.contiguous() first)")
+    args = (B, Lq, Lk, Hk, H // Hk, D) + _strides3(q, "q") + _strides3(k, "k") + _strides3(v, "v")
     if lengths is not None and (_op(lengths, "cross_attention: lengths", torch.int32).shape != (B,) or not lengths.is_contiguous()):
         raise RuntimeError(f"cross_attention: lengths is a contiguous ({B},) tensor, got {tuple(lengths.shape)}, strides {lengths.stride()}")
     if mask is not None:
@@ -2224,11 +2229,15 @@ def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
             raise RuntimeError(f"cross_attention: mask is ({B} or 1, {Lq} or 1, {Lk}) bool, got {tuple(mask.shape)}")
         if Lk > 1 and mask.stride(2) != 1:
             raise RuntimeError("cross_attention: the mask's last dimension has to be consecutive (.contiguous() first)")
+        ms = mask.stride()
+        args += (ms[0] if mask.shape[0] > 1 else 0, ms[1] if mask.shape[1] > 1 else 0)
+    else:
+        args += (0, 0)
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     _same_device(q, k, v, lengths, mask)
     if _wants_grad(q, k, v):
-        return CrossAttentionFn.apply(q, k, v, lengths, mask, scale)
-    return _cross_attention_fwd(q, k, v, lengths, mask, scale, False)[0]
+        return CrossAttentionFn.apply(q, k, v, lengths, mask, scale, args)
+    return _cross_attention_fwd(q, k, v, lengths, mask, scale, args, False)[0]
 
 
 def _embedding_fwd(weight, tokens, scale, padding_idx, op_dtype):
