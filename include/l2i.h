@@ -495,15 +495,17 @@ int l2i_group_norm_bwd(const void* x, int x_dtype, const float* gamma, const flo
  * lengths [B] int32 or NULL: keys at and behind it are not read. mask: bytes, address b mb + i mq + j, 0 = key j is masked for query i, or NULL;
  * mq = 0: one row for all queries, whose masked keys are not read either. A pair that is masked for some queries only weighs zero: its values
  * have to be finite. A query without a live key gives zeros (and no gradient).
- * out [B][Lq][Hk G][D] contiguous; lse [B][Hk][Lq G] (optional in fwd) is kept for bwd.
+ * out [B][Lq][Hk G][D] contiguous; lse [B][Hk][Lq G] (optional in fwd) is kept for bwd, as is out_lo (bf16 only, optional, out's layout: what the
+ * rounding of out left; worth its bytes where l2i_cross_attention_wants_lo says 1).
  * bwd: out, dout, dq [B][Lq][Hk G][D] and dk, dv [B][Lk][Hk][D] contiguous and 16-byte aligned; dq, and dk with dv, optional. */
 int l2i_cross_attention_scratch(int B, int Lq, int Lk, int Hk, int G, int D, int dtype, int bwd, long long* floats);
+int l2i_cross_attention_wants_lo(int B, int Lq, int Lk, int Hk, int G, int D, int dtype);   /* 1 or 0 */
 int l2i_cross_attention_fwd(const void* q, const void* k, const void* v, int dtype, const int* lengths, const unsigned char* mask, void* out,
-                            float* lse, int B, int Lq, int Lk, int Hk, int G, int D, long long qb, long long ql, long long qh, long long kb,
+                            void* out_lo, float* lse, int B, int Lq, int Lk, int Hk, int G, int D, long long qb, long long ql, long long qh, long long kb,
                             long long kl, long long kh, long long vb, long long vl, long long vh, long long mb, long long mq, float scale,
                             float* scratch, long long scratch_floats, void* stream);
 int l2i_cross_attention_bwd(const void* q, const void* k, const void* v, int dtype, const int* lengths, const unsigned char* mask,
-                            const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, int B, int Lq, int Lk, int Hk,
+                            const void* out, const void* out_lo, const float* lse, const void* dout, void* dq, void* dk, void* dv, int B, int Lq, int Lk, int Hk,
                             int G, int D, long long qb, long long ql, long long qh, long long kb, long long kl, long long kh, long long vb,
                             long long vl, long long vh, long long mb, long long mq, float scale, float* scratch, long long scratch_floats,
                             void* stream);

@@ -87,9 +87,10 @@ SIGNATURES = {
     "l2i_group_norm_fwd": [_p, _i, _p, _p, _p, _i, _p, _p, _i, _ll, _i, _i, _f, _i, _p, _ll, _p],
     "l2i_group_norm_bwd": [_p, _i, _p, _p, _p, _p, _p, _i, _p, _p, _p, _i, _ll, _i, _i, _i, _p, _ll, _p],
     "l2i_cross_attention_scratch": [_i, _i, _i, _i, _i, _i, _i, _i, _p],
-    "l2i_cross_attention_fwd": [_p, _p, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _f,
+    "l2i_cross_attention_wants_lo": [_i, _i, _i, _i, _i, _i, _i],
+    "l2i_cross_attention_fwd": [_p, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _f,
                                 _p, _ll, _p],
-    "l2i_cross_attention_bwd": [_p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll,
+    "l2i_cross_attention_bwd": [_p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll,
                                 _ll, _ll, _f, _p, _ll, _p],
     "l2i_embedding_fwd": [_p, _i, _p, _p, _i, _ll, _i, _i, _f, _i, _p],
     "l2i_embedding_bwd_scratch": [_ll, _i, _i, _p],

@@ -26,6 +26,8 @@ typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 
 struct XaArgs {
     const void *q, *k, *v; void* o;          // o, g, dq: [B][Lq][H][D]; dk, dv: [B][Lk][Hk][D]
+    bf16_t* lo;                               // what rounding o to bf16 left, or null: D = g . (o + lo) is exact to f32 then (o alone: relative 2^-9 of |g| |o|,
+                                              // which where few keys share the weight is more than the rounding of dS itself)
     const void* g; void *dq, *dk, *dv;
     float* lse;                               // [B Hk][R] log2 of the softmax's denominator; +inf for a row without a live key
     float* delta;                             // [B Hk][R] D
@@ -261,6 +263,37 @@ __device__ __forceinline__ float xa_pick(unsigned live, int e, float x, unsigned
     const unsigned m = (unsigned)((int)(live << (31 - e)) >> 31);
     return __uint_as_float((__float_as_uint(x) & m) | (other & ~m));
 }
+// One 32-row block of an accumulator (times f) to the D values of the lane's row from `row` on; lo: what rounding left, if wanted. bf16: the wave's halves
+// trade registers (their rows are the same) so that each lane stores eight consecutive values at once.
+template <typename T> __device__ __forceinline__ void xa_put(T* row, const f32x16_t& acc, float f, int d0, int D, bf16_t* lo = nullptr) {
+    const int h = (threadIdx.x & 63) >> 5;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const int dd = d0 + 8 * a + 4 * h;
+            const float v[4] = {acc[4 * a] * f, acc[4 * a + 1] * f, acc[4 * a + 2] * f, acc[4 * a + 3] * f};
+            if (dd < D) Op4<float>::store(row + dd, v);
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            unsigned u[4], w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = acc[8 * q + 2 * i] * f, y = acc[8 * q + 2 * i + 1] * f;
+                u[i] = f2bf2(x, y);
+                w[i] = f2bf2(x - __uint_as_float(u[i] << 16), y - __uint_as_float(u[i] & 0xffff0000u));
+            }
+            const int dd = d0 + 16 * q + 8 * h;
+            auto trade = [&](unsigned (&z)[4], bf16_t* to) {   // halves hold 4 h + 0 .. 3 and 8 + 4 h + 0 .. 3: -> 8 h + 0 .. 7
+                const auto a = __builtin_amdgcn_permlane32_swap(z[0], z[2], false, false), b = __builtin_amdgcn_permlane32_swap(z[1], z[3], false, false);
+                if (dd < D) *reinterpret_cast<uint4*>(to + dd) = make_uint4(a[0], b[0], a[1], b[1]);
+            };
+            trade(u, row);
+            if (lo) trade(w, lo);
+        }
+    }
+}
 #define XA_NINF 0xff800000u
 // Between a matrix instruction and the first read of its result no branch may join: the compiler's wait count there follows one of the joining
 // paths only. Live bits are therefore made in front of the products, masked and unmasked tiles are separate straight bodies, and behind a
@@ -469,15 +502,9 @@ __global__ __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : (sizeof
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;
     if (p.lse && h == 0 && (WQ == 4 || wave == 0)) p.lse[row] = l > 0.f ? m + log2f(l) : INFINITY;
-    T* o = reinterpret_cast<T*>(p.o) + (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D;
+    const size_t o = (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D;
 #pragma unroll
-    for (int d = 0; d < (WQ == 1 ? 1 : ND); ++d)
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const int dd = (WQ == 1 ? wave : d) * 32 + 8 * a + 4 * h;
-            const float v[4] = {oacc[d][4 * a] * inv, oacc[d][4 * a + 1] * inv, oacc[d][4 * a + 2] * inv, oacc[d][4 * a + 3] * inv};
-            if (dd < p.D) Op4<T>::store(o + dd, v);
-        }
+    for (int d = 0; d < (WQ == 1 ? 1 : ND); ++d) xa_put<T>(reinterpret_cast<T*>(p.o) + o, oacc[d], inv, (WQ == 1 ? wave : d) * 32, p.D, p.lo ? p.lo + o : nullptr);
 }
 
 // the ns ranges of a row, in range order: 32 lanes a row, four dims a lane
@@ -506,7 +533,13 @@ __global__ __launch_bounds__(256) void xa_join_kernel(XaArgs p) {
     for (int e = 0; e < 4; ++e) o[e] *= inv;
     const int bh = (int)(row / p.R), r = (int)(row - (long long)bh * p.R), b = bh / p.Hk, hk = bh - b * p.Hk;
     const int iq = xa_row_query(p, r), head = hk * p.G + r - iq * p.G;
-    Op4<T>::store(reinterpret_cast<T*>(p.o) + (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D + d, o);
+    const size_t at = (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D + d;
+    Op4<T>::store(reinterpret_cast<T*>(p.o) + at, o);
+    if (sizeof(T) == 2 && p.lo) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] -= bf2f(f2bf(o[e]));
+        Op4<bf16_t>::store(p.lo + at, o);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq (and D)
@@ -558,6 +591,18 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_d
 #pragma unroll
             for (int e = 0; e < E; ++e) dl += OpT<T>::to(ga[e]) * OpT<T>::to(oa[e]);
         }
+        if constexpr (sizeof(T) == 2) {
+            if (p.lo) {
+                xa_row_frag<T, CH>(of, on ? p.lo + orow : nullptr, p.D);
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    const T* ga = reinterpret_cast<const T*>(&gf[s]);
+                    const T* oa = reinterpret_cast<const T*>(&of[s]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dl += bf2f(ga[e]) * bf2f(oa[e]);
+                }
+            }
+        }
         dl += __shfl_xor(dl, 32, 64);
     }
     const float ls = on ? p.lse[(size_t)bh * p.R + r] : INFINITY;
@@ -604,15 +649,8 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_d
     }
     xa_settle();
     if (!on || !p.dq) return;
-    T* o = reinterpret_cast<T*>(p.dq) + orow;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const int dd = d * 32 + 8 * a + 4 * h;
-            const float v[4] = {acc[d][4 * a] * p.scale, acc[d][4 * a + 1] * p.scale, acc[d][4 * a + 2] * p.scale, acc[d][4 * a + 3] * p.scale};
-            if (dd < p.D) Op4<T>::store(o + dd, v);
-        }
+    for (int d = 0; d < ND; ++d) xa_put<T>(reinterpret_cast<T*>(p.dq) + orow, acc[d], p.scale, d * 32, p.D);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
@@ -730,24 +768,21 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_d
     }
     xa_settle();
     if (key >= p.Lk) return;
+    if (p.ns > 1) {
+        const size_t n = (size_t)p.B * p.Hk * p.Lk * p.D, at = ((size_t)bh * p.Lk + key) * p.D;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const int dd = d * 32 + 8 * a + 4 * h;
-            if (dd >= p.D) continue;
-            const float vk[4] = {dk[d][4 * a] * p.scale, dk[d][4 * a + 1] * p.scale, dk[d][4 * a + 2] * p.scale, dk[d][4 * a + 3] * p.scale};
-            const float vv[4] = {dv[d][4 * a], dv[d][4 * a + 1], dv[d][4 * a + 2], dv[d][4 * a + 3]};
-            if (p.ns > 1) {
-                const size_t n = (size_t)p.B * p.Hk * p.Lk * p.D, at = ((size_t)bh * p.Lk + key) * p.D + dd;
-                Op4<float>::store(p.part + (size_t)split * n + at, vk);
-                Op4<float>::store(p.part + (size_t)(p.ns + split) * n + at, vv);
-            } else {
-                const size_t at = (((size_t)b * p.Lk + key) * p.Hk + hk) * p.D + dd;
-                Op4<T>::store(reinterpret_cast<T*>(p.dk) + at, vk);
-                Op4<T>::store(reinterpret_cast<T*>(p.dv) + at, vv);
-            }
+        for (int d = 0; d < ND; ++d) {
+            xa_put<float>(p.part + (size_t)split * n + at, dk[d], p.scale, d * 32, p.D);
+            xa_put<float>(p.part + (size_t)(p.ns + split) * n + at, dv[d], 1.f, d * 32, p.D);
         }
+    } else {
+        const size_t at = (((size_t)b * p.Lk + key) * p.Hk + hk) * p.D;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            xa_put<T>(reinterpret_cast<T*>(p.dk) + at, dk[d], p.scale, d * 32, p.D);
+            xa_put<T>(reinterpret_cast<T*>(p.dv) + at, dv[d], 1.f, d * 32, p.D);
+        }
+    }
 }
 template <typename T>
 __global__ __launch_bounds__(256) void xa_fold_kernel(XaArgs p) {
@@ -844,13 +879,7 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 2 : 4) void xa_s
             if (p.lse && h == 0) p.lse[(size_t)bh * p.R + r] = l > 0.f ? ref + log2f(l) : INFINITY;
             T* o = reinterpret_cast<T*>(p.o) + (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D;
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    const int dd = d * 32 + 8 * a + 4 * h;
-                    const float v[4] = {oacc[d][4 * a], oacc[d][4 * a + 1], oacc[d][4 * a + 2], oacc[d][4 * a + 3]};
-                    if (dd < p.D) Op4<T>::store(o + dd, v);
-                }
+            for (int d = 0; d < ND; ++d) xa_put<T>(o, oacc[d], 1.f, d * 32, p.D);
         }
     }
 }
@@ -954,13 +983,7 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : DP == 64 ? 2
         if (on && p.dq) {
             T* o = reinterpret_cast<T*>(p.dq) + (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + hk * p.G + r - iq * p.G) * p.D;
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    const int dd = d * 32 + 8 * a + 4 * h;
-                    const float v[4] = {dqa[d][4 * a], dqa[d][4 * a + 1], dqa[d][4 * a + 2], dqa[d][4 * a + 3]};
-                    if (dd < p.D) Op4<T>::store(o + dd, v);
-                }
+            for (int d = 0; d < ND; ++d) xa_put<T>(o, dqa[d], 1.f, d * 32, p.D);
         }
         if (NBUF == 2) buf ^= 1;
         else if (blk + step < nblk) issue(blk + step, 0);
@@ -1126,36 +1149,40 @@ static void xa_setup(XaArgs& a, const void* q, const void* k, const void* v, con
     a.qb = qb; a.ql = ql; a.qh = qh; a.kb = kb; a.kl = kl; a.kh = kh; a.vb = vb; a.vl = vl; a.vh = vh; a.mb = mb; a.mq = mq;
     a.scale = scale; a.c = fabsf(scale) * 1.44269504088896340736f;
 }
+// whether out_lo is of use to the backward pass of these sizes: not in f32, nor where D does not come from out
+extern "C" int l2i_cross_attention_wants_lo(int B, int Lq, int Lk, int Hk, int G, int D, int dtype) {
+    return !xa_bad(B, Lq, Lk, Hk, G, D, dtype) && dtype && !xa_plan(B, (long long)Lq * G, Lk, Hk, D, dtype).nwb;
+}
 extern "C" int l2i_cross_attention_fwd(const void* q, const void* k, const void* v, int dtype, const int* lengths, const unsigned char* mask, void* out,
-                                       float* lse, int B, int Lq, int Lk, int Hk, int G, int D, long long qb, long long ql, long long qh, long long kb,
+                                       void* out_lo, float* lse, int B, int Lq, int Lk, int Hk, int G, int D, long long qb, long long ql, long long qh, long long kb,
                                        long long kl, long long kh, long long vb, long long vl, long long vh, long long mb, long long mq, float scale,
                                        float* scratch, long long scratch_floats, void* stream) {
     long long need = 0;
-    if (xa_bad(B, Lq, Lk, Hk, G, D, dtype) || !q || !out || (Lk && (!k || !v)) || mb < 0 || mq < 0 || ((size_t)out & 15)) return L2I_ERR_ARG;
+    if (xa_bad(B, Lq, Lk, Hk, G, D, dtype) || !q || !out || (Lk && (!k || !v)) || mb < 0 || mq < 0 || (((size_t)out | (size_t)out_lo) & 15) || (out_lo && !dtype)) return L2I_ERR_ARG;
     if (!xa_rows_ok(q, qb, ql, qh, G, dtype) || !xa_rows_ok(k, kb, kl, kh, 0, dtype) || !xa_rows_ok(v, vb, vl, vh, 0, dtype)) return L2I_ERR_ARG;
     if (l2i_cross_attention_scratch(B, Lq, Lk, Hk, G, D, dtype, 0, &need) != L2I_OK) return L2I_ERR_ARG;
     if (need && (!scratch || ((size_t)scratch & 15) || scratch_floats < need)) return L2I_ERR_ARG;
     XaArgs a = {};
     xa_setup(a, q, k, v, lengths, mask, B, Lq, Lk, Hk, G, D, qb, ql, qh, kb, kl, kh, vb, vl, vh, mb, mq, scale);
     const XaPlan pl = xa_plan(B, a.R, Lk, Hk, D, dtype);
-    a.o = out; a.lse = lse; a.ns = pl.ns;
+    a.o = out; a.lo = (bf16_t*)out_lo; a.lse = lse; a.ns = pl.ns;
     a.part = scratch; a.ml = scratch + (size_t)pl.ns * B * Hk * a.R * D;
     const int e = dtype ? xa_fwd_type<bf16_t>(a, pl, (hipStream_t)stream) : xa_fwd_type<float>(a, pl, (hipStream_t)stream);
     return e ? e : l2i_check_launch();
 }
 extern "C" int l2i_cross_attention_bwd(const void* q, const void* k, const void* v, int dtype, const int* lengths, const unsigned char* mask, const void* out,
-                                       const float* lse, const void* dout, void* dq, void* dk, void* dv, int B, int Lq, int Lk, int Hk, int G, int D,
+                                       const void* out_lo, const float* lse, const void* dout, void* dq, void* dk, void* dv, int B, int Lq, int Lk, int Hk, int G, int D,
                                        long long qb, long long ql, long long qh, long long kb, long long kl, long long kh, long long vb, long long vl,
                                        long long vh, long long mb, long long mq, float scale, float* scratch, long long scratch_floats, void* stream) {
     long long need = 0;
     if (xa_bad(B, Lq, Lk, Hk, G, D, dtype) || !q || !out || !lse || !dout || (Lk && (!k || !v)) || mb < 0 || mq < 0) return L2I_ERR_ARG;
-    if ((dk == nullptr) != (dv == nullptr) || (((size_t)out | (size_t)dout | (size_t)dq | (size_t)dk | (size_t)dv) & 15)) return L2I_ERR_ARG;
+    if ((dk == nullptr) != (dv == nullptr) || (out_lo && !dtype) || (((size_t)out | (size_t)out_lo | (size_t)dout | (size_t)dq | (size_t)dk | (size_t)dv) & 15)) return L2I_ERR_ARG;
     if (!xa_rows_ok(q, qb, ql, qh, G, dtype) || !xa_rows_ok(k, kb, kl, kh, 0, dtype) || !xa_rows_ok(v, vb, vl, vh, 0, dtype)) return L2I_ERR_ARG;
     if (l2i_cross_attention_scratch(B, Lq, Lk, Hk, G, D, dtype, 1, &need) != L2I_OK || !scratch || ((size_t)scratch & 15) || scratch_floats < need) return L2I_ERR_ARG;
     XaArgs a = {};
     xa_setup(a, q, k, v, lengths, mask, B, Lq, Lk, Hk, G, D, qb, ql, qh, kb, kl, kh, vb, vl, vh, mb, mq, scale);
     const XaPlan pl = xa_plan(B, a.R, Lk, Hk, D, dtype);
-    a.o = const_cast<void*>(out); a.lse = const_cast<float*>(lse); a.g = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.ns = pl.nsb;
+    a.o = const_cast<void*>(out); a.lo = (bf16_t*)const_cast<void*>(out_lo); a.lse = const_cast<float*>(lse); a.g = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.ns = pl.nsb;
     a.delta = scratch; a.part = scratch + ((long long)B * Hk * a.R + 3) / 4 * 4;
     hipStream_t s = (hipStream_t)stream;
     const int dp = xa_dp(D);

@@ -2157,29 +2157,39 @@ def _strides3(t, what):
     return r
 
 
+@functools.lru_cache(maxsize=4096)
+def _wants_lo(*sizes):
+    _lib.load()
+    return bool(_lib._FN["l2i_cross_attention_wants_lo"](*sizes, _lib.BF16))   # (an answer, not a status)
+
+
 def _cross_attention_fwd(q, k, v, lengths, mask, scale, args, want_lse):
     """args: (B, Lq, Lk, Hk, G, D) and the strides, as the library takes them."""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(args[0] * args[1] * args[3] * args[4], dtype=torch.float32, device=q.device) if want_lse else None
     code = _code(q.dtype)
+    lse = lo = None
+    if want_lse:
+        lse = torch.empty(args[0] * args[1] * args[3] * args[4], dtype=torch.float32, device=q.device)
+        if code and _wants_lo(*args[:6]):
+            lo = torch.empty(q.shape, dtype=q.dtype, device=q.device)   # (what rounding out leaves: for D in the backward pass)
     ws, wp, wn = _scratch(q.device, "l2i_cross_attention_scratch", *args[:6], code, 0)
-    _lib.call("l2i_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, _p(lengths), _p(mask), out.data_ptr(), _p(lse),
-              *args, scale, wp, wn, _stream())
-    return out, lse
+    _lib.call("l2i_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, _p(lengths), _p(mask), out.data_ptr(), _p(lo),
+              _p(lse), *args, scale, wp, wn, _stream())
+    return out, lo, lse
 
 
 class CrossAttentionFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, mask, scale, args):
-        out, lse = _cross_attention_fwd(q, k, v, lengths, mask, scale, args, True)
-        ctx.save_for_backward(q, k, v, lengths, mask, out, lse)
+        out, lo, lse = _cross_attention_fwd(q, k, v, lengths, mask, scale, args, True)
+        ctx.save_for_backward(q, k, v, lengths, mask, out, lo, lse)
         ctx.cfg = (scale, args)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        q, k, v, lengths, mask, out, lse = ctx.saved_tensors
+        q, k, v, lengths, mask, out, lo, lse = ctx.saved_tensors
         scale, args = ctx.cfg
         g = _aligned(g.contiguous())
         nq, nk, nv = ctx.needs_input_grad[:3]
@@ -2190,7 +2200,7 @@ class CrossAttentionFn(Function):
             dk, dv = torch.empty(k.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev)
         ws, wp, wn = _scratch(dev, "l2i_cross_attention_scratch", *args[:6], code, 1)
         _lib.call("l2i_cross_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, _p(lengths), _p(mask), out.data_ptr(),
-                  lse.data_ptr(), g.data_ptr(), _p(dq), _p(dk), _p(dv), *args, scale, wp, wn, _stream())
+                  _p(lo), lse.data_ptr(), g.data_ptr(), _p(dq), _p(dk), _p(dv), *args, scale, wp, wn, _stream())
         return dq, dk if nk else None, dv if nv else None, None, None, None, None
 
 

@@ -127,14 +127,14 @@ def test_entry_points_refuse_before_a_launch():
         assert gn(**bad) == -1, bad
     for bad in (dict(x=None), dict(dy=None), dict(m=None), dict(G=5), dict(C=0), dict(s=None), dict(n=1)):
         assert gb(**bad) == -1, bad
-    xa = lambda q=P, k=P, v=P, dt=1, o=P, B=2, Lq=3, Lk=5, Hk=2, G=2, D=16, st=(0,) * 9, mb=0, mq=0, s=None, n=0: lib.l2i_cross_attention_fwd(
-        q, k, v, dt, None, None, o, None, B, Lq, Lk, Hk, G, D, *st, mb, mq, 1.0, s, n, None)
+    xa = lambda q=P, k=P, v=P, dt=1, o=P, B=2, Lq=3, Lk=5, Hk=2, G=2, D=16, st=(0,) * 9, mb=0, mq=0, s=None, n=0, lo=None: lib.l2i_cross_attention_fwd(
+        q, k, v, dt, None, None, o, lo, None, B, Lq, Lk, Hk, G, D, *st, mb, mq, 1.0, s, n, None)
     for bad in (dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(dt=2), dict(B=0), dict(Lq=0), dict(Lk=-1), dict(Hk=0), dict(G=0), dict(D=0), dict(D=12),
                 dict(D=136), dict(q=P + 8), dict(o=P + 2), dict(st=(4,) + (0,) * 8), dict(st=(0,) * 8 + (-8,)), dict(mb=-1), dict(mq=-1), dict(Lq=1 << 30, G=2),
-                dict(Lk=100000)):   # (the last one needs scratch)
+                dict(lo=P, dt=0), dict(lo=P + 8), dict(Lk=100000)):   # (the last one needs scratch)
         assert xa(**bad) == -1, bad
     xb = lambda lse=P, g=P, dq=P, dk=P, dv=P, s=P, n=big: lib.l2i_cross_attention_bwd(
-        P, P, P, 1, None, None, P, lse, g, dq, dk, dv, 2, 3, 5, 2, 2, 16, *(0,) * 11, 1.0, s, n, None)
+        P, P, P, 1, None, None, P, None, lse, g, dq, dk, dv, 2, 3, 5, 2, 2, 16, *(0,) * 11, 1.0, s, n, None)
     for bad in (dict(lse=None), dict(g=None), dict(dk=None), dict(dv=None), dict(dq=P + 8), dict(s=None), dict(s=P + 4), dict(n=1)):
         assert xb(**bad) == -1, bad
     ef = lambda w=P, wd=0, t=P, o=P, od=0, n=3, V=5, D=8: lib.l2i_embedding_fwd(w, wd, t, o, od, n, V, D, 1.0, -1, None)
@@ -159,6 +159,8 @@ def test_scratch_sizes():
             rc, n = _floats("l2i_group_norm_scratch", B, HW, C, G, bwd)
             assert rc == 0 and 0 <= n < 1 << 31
     assert _floats("l2i_cross_attention_scratch", 4, 4096, 2048, 4, 4, 128, 1, 0) == (0, 0)   # rows enough: no splits
+    lib = _lib()
+    assert [lib.l2i_cross_attention_wants_lo(1, 64, lk, 1, 1, 64, dt) for lk, dt in ((31, 1), (33, 1), (33, 0), (-1, 1))] == [0, 1, 0, 0]
     rc, n = _floats("l2i_cross_attention_scratch", 1, 1, 4096, 1, 1, 128, 1, 0)
     assert rc == 0 and n > 0
 
