@@ -545,7 +545,7 @@ __global__ __launch_bounds__(256) void xa_join_kernel(XaArgs p) {
 // ------------------------------------------------------------------------------------------------ backward: dq (and D)
 // Four waves x 32 rows, tiles of 64 keys, as the forward; also leaves D for the kernel behind it.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_dq_kernel(XaArgs p, int nqt, int total) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void xa_dq_kernel(XaArgs p, int nqt, int total) {
     constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, KT = 64, BYTES = KT * CH * 16;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int id = xa_tile_id(total);
@@ -654,11 +654,11 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_d
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
-// A lane owns one key: four waves x 32 keys, every wave reads all 64 rows of a tile of queries and their gradients. ns > 1: the rows are cut in ns
-// ranges, added in range order by xa_fold_kernel.
-template <typename T, int DP>
+// A lane owns one key. WK = 4: four waves x 32 keys, every wave reads all 64 rows of a tile of queries and their gradients. WK = 2: two x 32 keys, a
+// pair of waves each take half of the rows of a tile and are joined at the end. ns > 1: the rows are cut in ns ranges, added in range order by xa_fold_kernel.
+template <typename T, int DP, int WK>
 __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_dkv_kernel(XaArgs p, int nkt, int total) {
-    constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, RT = 64, BYTES = RT * CH * 16;
+    constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, RT = 64, BYTES = RT * CH * 16, KEYS = 32 * WK, ROWS = RT * WK / 4;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* rowv = reinterpret_cast<float*>(smem + 4 * BYTES);   // two of: [RT] lse, [RT] D, [RT] query of the row
     const int id = xa_tile_id(total);
@@ -666,10 +666,10 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_d
     const int bh = id / (nkt * p.ns), rest = id - bh * nkt * p.ns, kt = rest / p.ns, split = rest - kt * p.ns;
     const int b = bh / p.Hk, hk = bh - b * p.Hk;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int key = kt * 128 + wave * 32 + (lane & 31);
+    const int key = kt * KEYS + (wave % WK) * 32 + (lane & 31), first = wave / WK * ROWS;   // first: of the wave's rows in a tile
     const XaStates<T> st(p, b, hk);
     const bool klive = st.live(key), qmask = st.mb && !st.kmask;
-    const int nt = kt * 128 < st.len ? (p.R + RT - 1) / RT : 0, per = (nt + p.ns - 1) / p.ns;
+    const int nt = kt * KEYS < st.len ? (p.R + RT - 1) / RT : 0, per = (nt + p.ns - 1) / p.ns;
     const int t0 = split * per, t1 = min(nt, t0 + per);
     const unsigned lds = lds_addr_of(smem);
     const T* qp = reinterpret_cast<const T*>(p.q) + b * p.qb + hk * p.G * p.qh;
@@ -713,10 +713,12 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_d
 #pragma unroll
         for (int e = 0; e < 16; ++e) { dk[d][e] = 0.f; dv[d][e] = 0.f; }
     XaAddr<T, CH> ad;
+    if (WK == 2) ad.move(first * CH * 16);
+    const float* const mine = rowv + first;
     auto work = [&](auto masked, const char* qs, const float* rv) {
         const char* gs = qs + BYTES;
 #pragma unroll
-        for (int row0 = 0; row0 < RT; row0 += 32) {
+        for (int row0 = 0; row0 < ROWS; row0 += 32) {
             unsigned live = 0;
             if constexpr (decltype(masked)::value) {
                 live = klive ? 0xffffu : 0u;
@@ -758,15 +760,39 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_d
     if (!qmask && __ballot(klive) == ~0ull)
         for (; t + 1 < t1; t += 2) {
             turn(t, 0);
-            work(std::false_type(), smem, rowv);
+            work(std::false_type(), smem, mine);
             turn(t + 1, 1);
-            work(std::false_type(), smem + 2 * BYTES, rowv + 3 * RT);
+            work(std::false_type(), smem + 2 * BYTES, mine + 3 * RT);
         }
     for (int buf = 0; t < t1; ++t, buf ^= 1) {
         turn(t, buf);
-        work(std::true_type(), smem + buf * 2 * BYTES, rowv + buf * 3 * RT);
+        work(std::true_type(), smem + buf * 2 * BYTES, mine + buf * 3 * RT);
     }
     xa_settle();
+    if constexpr (WK == 2) {   // the second half's sums through LDS to the first
+        float* ob = reinterpret_cast<float*>(smem) + (wave & 1) * DP * 64 + (lane & 31);   // [2 DP][32]
+        __syncthreads();
+        if (wave >= 2) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int dd = d * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+                    ob[dd * 32] = dk[d][e];
+                    ob[(DP + dd) * 32] = dv[d][e];
+                }
+        }
+        __syncthreads();
+        if (wave >= 2) return;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int dd = d * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+                dk[d][e] += ob[dd * 32];
+                dv[d][e] += ob[(DP + dd) * 32];
+            }
+    }
     if (key >= p.Lk) return;
     if (p.ns > 1) {
         const size_t n = (size_t)p.B * p.Hk * p.Lk * p.D, at = ((size_t)bh * p.Lk + key) * p.D;
@@ -1035,7 +1061,7 @@ static int xa_splits(long long tiles, long long nt) {
     if (ns > 64) ns = 64;
     return ns < 1 ? 1 : (int)ns;
 }
-struct XaPlan { int wq, nqt, ns, nkt, nsb, nwf, nwb; };   // nwf, nwb: workgroups an (image, state head) of the one-tile form has, 0: not that form
+struct XaPlan { int wq, nqt, ns, wk, nkt, nsb, nwf, nwb; };   // nwf, nwb: workgroups an (image, state head) of the one-tile form has, 0: not that form
 static bool xa_short_fits(int dp, int dtype) {
     return dtype ? (dp == 32 ? XaShort<bf16_t, 32>::OK : dp == 64 ? XaShort<bf16_t, 64>::OK : XaShort<bf16_t, 128>::OK)
                  : (dp == 32 ? XaShort<float, 32>::OK : dp == 64 ? XaShort<float, 64>::OK : XaShort<float, 128>::OK);
@@ -1052,7 +1078,10 @@ static XaPlan xa_plan(int B, long long R, int Lk, int Hk, int D, int dtype) {
     q.nqt = (int)((R + 32 * q.wq - 1) / (32 * q.wq));
     const int kt = q.wq == 4 ? 64 : 128;   // keys a workgroup takes at a time
     q.ns = xa_splits((long long)B * Hk * q.nqt, (Lk + kt - 1) / kt);
-    q.nkt = (Lk + 127) / 128;
+    // 64 keys a workgroup where 128 would leave waves or CUs without any (f32, 64 states of 64 x 4 heads x 16 images: 278 -> 218 us for dq, dk, dv;
+    // 77 states of 40 x 2 x 8, f32: 22 -> 16 us for dk, dv), else 128, which stage the rows half as often (2048 states, bf16: 510 us, not 560)
+    q.wk = Lk <= 64 || (Lk <= 128 && bh * ((Lk + 127) / 128) < 256) ? 2 : 4;
+    q.nkt = (Lk + 32 * q.wk - 1) / (32 * q.wk);
     q.nsb = q.nwb ? q.nwb : xa_splits((long long)B * Hk * q.nkt, (R + 63) / 64);
     if (q.nwf) q.ns = 1;
     return q;
@@ -1130,8 +1159,13 @@ static int xa_bwd_launch(const XaArgs& a, const XaPlan& q, hipStream_t s) {
     if (int e = xa_lds(xa_dq_kernel<T, DP>, lq)) return e;
     hipLaunchKernelGGL((xa_dq_kernel<T, DP>), dim3(xa_grid(tq)), dim3(256), lq, s, a, nqt, tq);
     if (!a.dk || a.Lk == 0) return L2I_OK;
-    if (int e = xa_lds(xa_dkv_kernel<T, DP>, lk)) return e;
-    hipLaunchKernelGGL((xa_dkv_kernel<T, DP>), dim3(xa_grid(tk)), dim3(256), lk, s, a, q.nkt, tk);
+    if (q.wk == 4) {
+        if (int e = xa_lds(xa_dkv_kernel<T, DP, 4>, lk)) return e;
+        hipLaunchKernelGGL((xa_dkv_kernel<T, DP, 4>), dim3(xa_grid(tk)), dim3(256), lk, s, a, q.nkt, tk);
+    } else {
+        if (int e = xa_lds(xa_dkv_kernel<T, DP, 2>, lk)) return e;
+        hipLaunchKernelGGL((xa_dkv_kernel<T, DP, 2>), dim3(xa_grid(tk)), dim3(256), lk, s, a, q.nkt, tk);
+    }
     if (a.ns > 1) xa_fold_launch<T>(a, s);
     return L2I_OK;
 }
