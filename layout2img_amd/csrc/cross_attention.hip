@@ -507,23 +507,54 @@ __global__ __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : (sizeof
     for (int d = 0; d < (WQ == 1 ? 1 : ND); ++d) xa_put<T>(reinterpret_cast<T*>(p.o) + o, oacc[d], inv, (WQ == 1 ? wave : d) * 32, p.D, p.lo ? p.lo + o : nullptr);
 }
 
-// the ns ranges of a row, in range order: 32 lanes a row, four dims a lane
-template <typename T>
+// The ns ranges of a row: 32 lanes a row, four dims a lane. The lanes take the ranges' maxima and sums side by side (at most XA_MAX_SPLITS), then walk the
+// ranges' partial rows in range order, eight in flight. WIDE: a row's ranges are many, and all eight groups of 32 lanes walk every eighth of them.
+#define XA_MAX_SPLITS 256
+template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void xa_join_kernel(XaArgs p) {
-    const long long rows = (long long)p.B * p.Hk * p.R, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    __shared__ float ws[8][XA_MAX_SPLITS];
+    const int grp = threadIdx.x >> 5, n = threadIdx.x & 31, d = n * 4;
+    const long long rows = (long long)p.B * p.Hk * p.R, row = WIDE ? (long long)blockIdx.x : (long long)blockIdx.x * 8 + grp;
     if (row >= rows) return;
-    const int d = (threadIdx.x & 31) * 4;
-    float mn = -INFINITY;
-    for (int s = 0; s < p.ns; ++s) mn = fmaxf(mn, p.ml[((size_t)s * rows + row) * 2]);
+    float* w = ws[grp];
+    float mm[XA_MAX_SPLITS / 32], ll[XA_MAX_SPLITS / 32], mn = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < XA_MAX_SPLITS / 32; ++k) {
+        const int s = n + 32 * k;
+        const float2 q = s < p.ns ? *reinterpret_cast<const float2*>(p.ml + ((size_t)s * rows + row) * 2) : make_float2(-INFINITY, 0.f);
+        mm[k] = q.x; ll[k] = q.y;
+        mn = fmaxf(mn, q.x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor(mn, o, 64));
     const float ref = mn == -INFINITY ? 0.f : mn;
-    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.ns; ++s) {
-        const float* q = p.ml + ((size_t)s * rows + row) * 2;
-        const float w = xa_exp2(q[0] - ref);
-        l += q[1] * w;
-        if (d < p.D) {
-            const float4 a = *reinterpret_cast<const float4*>(p.part + ((size_t)s * rows + row) * p.D + d);
-            o[0] += a.x * w; o[1] += a.y * w; o[2] += a.z * w; o[3] += a.w * w;
+#pragma unroll
+    for (int k = 0; k < XA_MAX_SPLITS / 32; ++k) {
+        const float f = xa_exp2(mm[k] - ref);
+        l += ll[k] * f;
+        w[n + 32 * k] = f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+    asm volatile("" ::: "memory");   // (a row's lanes lie in one wave, whose LDS accesses run in order)
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    if (d < p.D) {
+        const float* src = p.part + row * p.D + d;
+#pragma unroll 8
+        for (int s = WIDE ? grp : 0; s < p.ns; s += WIDE ? 8 : 1) {
+            const float4 a = *reinterpret_cast<const float4*>(src + (size_t)s * rows * p.D);
+            o[0] = fmaf(a.x, w[s], o[0]); o[1] = fmaf(a.y, w[s], o[1]); o[2] = fmaf(a.z, w[s], o[2]); o[3] = fmaf(a.w, w[s], o[3]);
+        }
+    }
+    if (WIDE) {
+        __shared__ __attribute__((aligned(16))) float4 os[8][32];
+        os[grp][n] = make_float4(o[0], o[1], o[2], o[3]);
+        __syncthreads();
+        if (grp) return;
+#pragma unroll
+        for (int g = 1; g < 8; ++g) {
+            const float4 a = os[g][n];
+            o[0] += a.x; o[1] += a.y; o[2] += a.z; o[3] += a.w;
         }
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -1051,14 +1082,15 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : DP == 64 ? 2
 }
 
 // ------------------------------------------------------------------------------------------------ entry points
-#define XA_WGS 512   // workgroups that fill the chip: 256 CUs, two each
+#define XA_WGS 512   // workgroups that fill the chip: 256 CUs, two each. Kernels of one workgroup a CU (the forward's few rows) take half of it: 32768
+                     // states of 128 x 8 heads, one query: 33 us at 512, 31 at 256; 32 images of 4096 x 8 x 64: 50 and 46
 static int xa_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
-// ranges of the states (forward) for `tiles` workgroups over `nt` tiles of states: enough workgroups, at least two tiles each
-static int xa_splits(long long tiles, long long nt) {
-    if (tiles >= XA_WGS || nt < 2) return 1;
-    long long ns = (XA_WGS + tiles - 1) / tiles;
+// ranges of the states (forward) or rows (backward) for `tiles` workgroups over `nt` tiles of them: `wgs` workgroups, at least two tiles each
+static int xa_splits(long long tiles, long long nt, int wgs) {
+    if (tiles >= wgs || nt < 2) return 1;
+    long long ns = (wgs + tiles - 1) / tiles;
     if (ns > nt / 2) ns = nt / 2;
-    if (ns > 64) ns = 64;
+    if (ns > XA_MAX_SPLITS) ns = XA_MAX_SPLITS;
     return ns < 1 ? 1 : (int)ns;
 }
 struct XaPlan { int wq, nqt, ns, wk, nkt, nsb, nwf, nwb; };   // nwf, nwb: workgroups an (image, state head) of the one-tile form has, 0: not that form
@@ -1077,12 +1109,12 @@ static XaPlan xa_plan(int B, long long R, int Lk, int Hk, int D, int dtype) {
     q.wq = R <= 32 ? 1 : 4;
     q.nqt = (int)((R + 32 * q.wq - 1) / (32 * q.wq));
     const int kt = q.wq == 4 ? 64 : 128;   // keys a workgroup takes at a time
-    q.ns = xa_splits((long long)B * Hk * q.nqt, (Lk + kt - 1) / kt);
+    q.ns = xa_splits((long long)B * Hk * q.nqt, (Lk + kt - 1) / kt, q.wq == 4 ? XA_WGS : XA_WGS / 2);
     // 64 keys a workgroup where 128 would leave waves or CUs without any (f32, 64 states of 64 x 4 heads x 16 images: 278 -> 218 us for dq, dk, dv;
     // 77 states of 40 x 2 x 8, f32: 22 -> 16 us for dk, dv), else 128, which stage the rows half as often (2048 states, bf16: 510 us, not 560)
     q.wk = Lk <= 64 || (Lk <= 128 && bh * ((Lk + 127) / 128) < 256) ? 2 : 4;
     q.nkt = (Lk + 32 * q.wk - 1) / (32 * q.wk);
-    q.nsb = q.nwb ? q.nwb : xa_splits((long long)B * Hk * q.nkt, (R + 63) / 64);
+    q.nsb = q.nwb ? q.nwb : xa_splits((long long)B * Hk * q.nkt, (R + 63) / 64, XA_WGS);
     if (q.nwf) q.ns = 1;
     return q;
 }
@@ -1132,7 +1164,9 @@ static int xa_fwd_type(const XaArgs& a, const XaPlan& q, hipStream_t s) {
     if (e) return e;
     if (a.ns > 1) {
         const long long rows = (long long)a.B * a.Hk * a.R;
-        hipLaunchKernelGGL((xa_join_kernel<T>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a);
+        // (one query over 262144 states of 128, 128 ranges: 59 us for both kernels with 32 lanes a row, 31 with 256)
+        if (a.ns > 16) hipLaunchKernelGGL((xa_join_kernel<T, true>), dim3((unsigned)rows), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((xa_join_kernel<T, false>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a);
     }
     return L2I_OK;
 }

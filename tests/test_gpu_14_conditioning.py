@@ -137,6 +137,22 @@ def test_cross_attention_masks_and_rows_without_a_state(Lq, Lk, G, dtype):
     _check_xa(q, k, v, g, mask=wide[:, :, 3:3 + Lk])         # rows that start anywhere
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,Lq,Hk,G,D", [(1, 1, 1, 1, 40), (2, 1, 2, 4, 128), (1, 2, 1, 9, 64), (1, 60, 1, 1, 64)])
+def test_cross_attention_of_few_queries_over_many_ranges(B, Lq, Hk, G, D, dtype):
+    """Enough states that they are cut in dozens of ranges, of which a length or a mask leaves many without a state."""
+    Lk = 9001
+    q, k, v, g = _xa(B, Lq, Lk, Hk, G, D, dtype, 11)
+    _check_xa(q, k, v, g)
+    n = torch.tensor([700, 0][:B], dtype=torch.int32, device=DEV)
+    bad = torch.arange(Lk, device=DEV)[None, :, None, None] >= n[:, None, None, None]
+    _check_xa(q, k.masked_fill(bad, math.nan), v.masked_fill(bad, math.inf), g, lengths=n)
+    mask = torch.zeros(B, Lq, Lk, dtype=torch.bool, device=DEV)
+    mask[:, :, 5000:5003] = True
+    mask[:, :, 8999] = True
+    _check_xa(q, k, v, g, mask=mask)
+
+
 def test_cross_attention_with_scores_of_any_size():
     q, k, v, g = _xa(1, 50, 90, 1, 1, 64, F32, 6)
     _check_xa(q * 30, k, v, g, scale=0.5)                    # probabilities of one and zero
@@ -426,3 +442,93 @@ def test_no_second_derivative():
     (g,) = torch.autograd.grad(ops.group_norm_act(x, 2, act="silu").sum(), (x,), create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_wide_heads_captured_and_replayed():
+    """Kernels that ask for more than 64 KiB of LDS, split ranges and joins, inside a graph; the scratch of a replay is the graph's own."""
+    from layout2img_amd import ops
+    gen = _gen(31)
+    sets = []
+    for Lq, Lk in ((1, 3000), (70, 600), (300, 40)):
+        q, k, v = (_rnd(gen, 2, n, 2, 128, dtype=BF16).requires_grad_() for n in (Lq, Lk, Lk))
+        sets.append((q, k, v, _rnd(gen, 2, Lq, 2, 128, dtype=BF16), torch.tensor([Lk, Lk // 3], dtype=torch.int32, device=DEV)))
+
+    def run():
+        out = []
+        for q, k, v, g, n in sets:
+            y = ops.cross_attention(q, k, v, lengths=n)
+            out += [y.detach(), *torch.autograd.grad(y, (q, k, v), g)]
+        return out
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = run()
+    for step in range(3):
+        with torch.no_grad():
+            for q, k, v, g, n in sets:
+                q.mul_(0.9), g.neg_()
+                n[0] -= 7
+        want = run()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), step
+
+
+def test_gradients_of_some_inputs_only_and_of_an_expanded_gradient():
+    from layout2img_amd import ops
+    q, k, v, g = _xa(2, 40, 70, 2, 1, 32, F32, 32)
+    want, tol = R.cross_attention(q, k, v, g=torch.ones_like(g))
+    for i in range(3):
+        leaves = [t.detach().requires_grad_(j == i) for j, t in enumerate((q, k, v))]
+        y = ops.cross_attention(*leaves)
+        first = torch.autograd.grad(y.sum(), (leaves[i],), retain_graph=True)[0]      # (the gradient of a sum is an expanded one)
+        R.close(first, want[1 + i], tol[1 + i], f"input {i}")
+        assert torch.equal(torch.autograd.grad(y.sum(), (leaves[i],))[0], first)     # a graph that is used twice
+    x, w, b = _rnd(_gen(33), 2, 20, 20, 16), 1 + 0.1 * _rnd(_gen(34), 16), _rnd(_gen(35), 16)
+    want, tol = R.group_norm_act(x, 4, w, b, 1e-5, "silu", F32, torch.ones_like(x))
+    for i in range(3):
+        leaves = [t.detach().requires_grad_(j == i) for j, t in enumerate((x, w, b))]
+        R.close(torch.autograd.grad(ops.group_norm_act(leaves[0], 4, leaves[1], leaves[2], act="silu").sum(), (leaves[i],))[0], want[1 + i], tol[1 + i], f"gn {i}")
+
+
+def test_two_streams_at_once():
+    """The same operators on two streams at the same time: no workspace is shared."""
+    from layout2img_amd import ops
+    gen = _gen(36)
+    q, k, v = _rnd(gen, 1, 4, 2, 64, dtype=BF16), _rnd(gen, 1, 5000, 2, 64, dtype=BF16), _rnd(gen, 1, 5000, 2, 64, dtype=BF16)
+    x = _rnd(gen, 4, 64, 64, 32)
+    w = _rnd(gen, 300, 16).requires_grad_()
+    tok = torch.randint(0, 300, (30000,), generator=gen, device=DEV)
+    dy = _rnd(gen, 30000, 16)
+    run = lambda: [ops.cross_attention(q, k, v), ops.group_norm_act(x, 8, act="silu"), torch.autograd.grad(ops.embedding(w, tok), (w,), dy)[0]]
+    want = run()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    for outs in got:
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+
+
+def test_a_tensor_of_the_cpu_is_refused():
+    from layout2img_amd import ops
+    q = torch.zeros(1, 2, 2, 16, device=DEV)
+    for bad in (dict(lengths=torch.zeros(1, dtype=torch.int32)), dict(mask=torch.zeros(1, 1, 2, dtype=torch.bool))):
+        with pytest.raises(RuntimeError):
+            ops.cross_attention(q, q, q, **bad)
+    with pytest.raises(RuntimeError):
+        ops.embedding(torch.zeros(3, 4, device=DEV), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(RuntimeError):
+        ops.dropout(torch.zeros(4, device=DEV), 0.5, torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(RuntimeError):
+        ops.group_norm_act(torch.zeros(1, 2, 2, 8, device=DEV), 2, torch.ones(8))
