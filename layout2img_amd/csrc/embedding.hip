@@ -108,8 +108,9 @@ __global__ __launch_bounds__(256) void embedding_direct_kernel(EmbDirectArgs p) 
 
 // ------------------------------------------------------------------------------------------------ sort
 // The rank of pair i is the number of pairs in front of it: those with a smaller key, and those with the same key at a smaller position.
-// Counting it directly is n^2 comparisons and one launch (29 us at 16384 pairs, where the radix sort's six launches take 35). A workgroup ranks 64 pairs: each of its NW waves counts over its share of every
-// tile of 256 NW keys that the workgroup stages in LDS (four waves up to 2048 pairs, sixteen above: four a SIMD hide the LDS reads).
+// Counting it directly is n^2 comparisons and one launch: what up to EMB_RANK_MAX pairs take (lookup and gradient of 4096 rows of 512 in a table of
+// 32000: 43 us, with the radix sort 46; even at 6000 pairs; 49 and 45 at 8192). A workgroup ranks 64 pairs: each of its NW waves counts over its share of
+// every tile of 256 NW keys that the workgroup stages in LDS (four waves up to 2048 pairs, sixteen above: four a SIMD hide the LDS reads).
 // The sort's first launch also marks every row of dW as absent (range[v] = (-1, 0)); the next kernel fills in the tokens that occur.
 __device__ __forceinline__ int emb_key(long long t, int V, int pad) { return (t >= 0 && t < V && t != pad) ? (int)t : V; }
 __device__ __forceinline__ void emb_clear(int2* range, int V) {
@@ -160,23 +161,28 @@ __global__ __launch_bounds__(NW * 64) void embedding_rank_kernel(const long long
     }
 }
 
-// Above EMB_RANK_MAX pairs: a stable radix sort, eight bits a pass from the lowest, three launches a pass. A workgroup owns 2048
-// consecutive pairs, a wave 512 of them; hist[digit][workgroup] counts, its exclusive scan is where each workgroup's pairs of a digit go.
-#define EMB_RANK_MAX 16384
-#define EMB_TILE 2048
+// Above EMB_RANK_MAX pairs: a stable radix sort, eight bits a pass from the lowest. A workgroup owns 256 R consecutive pairs (R: 2, or 8 above
+// EMB_FEW pairs), a wave a quarter of them; hist[digit][workgroup] counts, its exclusive scan is where each workgroup's pairs of a digit go. Up to
+// EMB_SCAN workgroups each of them scans the counts by itself, above that a launch of its own does (262144 rows of 512, lookup and gradient: 291 us with
+// that launch, 237 without). Sizes: 16384 pairs are sorted by the four launches of two passes in 16 us (a rank by n^2 comparisons: 29), 8192 the same.
+#define EMB_RANK_MAX 6144
+#define EMB_FEW 32768
+#define EMB_SCAN 256
 struct EmbSortArgs {
     const long long* tok; const int* kin; const int* pin; int* kout; int* pout; int* hist; int2* range;   // range: first pass only
-    int n, V, pad, shift, nblk;
+    int n, V, pad, shift, nblk, scanned;
 };
 __device__ __forceinline__ int emb_sort_key(const EmbSortArgs& p, int i) { return p.tok ? emb_key(p.tok[i], p.V, p.pad) : p.kin[i]; }
 
+template <int R>
 __global__ __launch_bounds__(256) void embedding_hist_kernel(EmbSortArgs p) {
     __shared__ int h[256];
     if (p.range) emb_clear(p.range, p.V);
     h[threadIdx.x] = 0;
     __syncthreads();
-    for (int k = threadIdx.x; k < EMB_TILE; k += 256) {
-        const int i = blockIdx.x * EMB_TILE + k;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int i = (blockIdx.x * R + k) * 256 + threadIdx.x;
         if (i < p.n) atomicAdd(&h[(emb_sort_key(p, i) >> p.shift) & 255], 1);   // (integers: the order does not matter)
     }
     __syncthreads();
@@ -202,27 +208,45 @@ __global__ __launch_bounds__(1024) void embedding_scan_kernel(int* __restrict__ 
         __syncthreads();
     }
 }
+template <int R>
 __global__ __launch_bounds__(256) void embedding_scatter_kernel(EmbSortArgs p) {
     __shared__ int at[4][256];   // where the wave's next pair of a digit goes
+    __shared__ int wtot[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int k = threadIdx.x; k < 1024; k += 256) (&at[0][0])[k] = 0;
-    __syncthreads();
-    const int base = blockIdx.x * EMB_TILE + wave * 512;
-    int key[8];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int w = 0; w < 4; ++w) at[w][threadIdx.x] = 0;
+    __syncthreads();
+    const int base = blockIdx.x * 256 * R + wave * 64 * R;
+    int key[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
         const int i = base + r * 64 + lane;
         key[r] = i < p.n ? emb_sort_key(p, i) : -1;
         if (i < p.n) atomicAdd(&at[wave][(key[r] >> p.shift) & 255], 1);
     }
-    __syncthreads();
-    {
-        int s = p.hist[(size_t)threadIdx.x * p.nblk + blockIdx.x];
-        for (int w = 0; w < 4; ++w) { const int t = at[w][threadIdx.x]; at[w][threadIdx.x] = s; s += t; }
+    int s;
+    if (p.scanned) {
+        s = p.hist[(size_t)threadIdx.x * p.nblk + blockIdx.x];
+        __syncthreads();
+    } else {   // thread d: this digit's pairs in the workgroups in front of this one, and the pairs of all smaller digits
+        const int* row = p.hist + (size_t)threadIdx.x * p.nblk;
+        int tot = 0;
+        s = 0;
+#pragma unroll 16
+        for (int k = 0; k < p.nblk; ++k) { const int t = row[k]; tot += t; s += k < (int)blockIdx.x ? t : 0; }
+        int run = tot;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int t = __shfl_up(run, o, 64); if (lane >= o) run += t; }
+        if (lane == 63) wtot[wave] = run;
+        __syncthreads();
+        s += run - tot;
+        for (int w = 0; w < wave; ++w) s += wtot[w];
     }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) { const int t = at[w][threadIdx.x]; at[w][threadIdx.x] = s; s += t; }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int r = 0; r < R; ++r) {
         const int i = base + r * 64 + lane;
         const bool on = i < p.n;
         const int d = on ? (key[r] >> p.shift) & 255 : 0;
@@ -402,11 +426,13 @@ extern "C" int l2i_embedding_fwd(const void* weight, int w_dtype, const long lon
 }
 
 // scratch, in ints: sorted keys and positions [n] each, the tokens' ranges [V][2], a second pair of them and the histogram when the radix sort runs, then the partial rows
-static int emb_chunk(long long n) { return n <= 2048 ? 8 : n <= 65536 ? 32 : 128; }   // few pairs: more workgroups; many: fewer partial rows
+static int emb_chunk(long long n) { return n <= 2048 ? 8 : n <= 8192 ? 16 : n <= 65536 ? 32 : 128; }   // few pairs: more workgroups; many: fewer partial rows
 // every row of dW looks through all pairs: few pairs, and not millions of rows
 static bool emb_direct(long long n, int V) { return n <= EMB_DIRECT && n * V <= (1 << 24); }
 static long long emb_al(long long ints) { return (ints + 3) & ~3LL; }
-static long long emb_hist_ints(long long n) { return 256 * ((n + EMB_TILE - 1) / EMB_TILE); }
+static int emb_rounds(long long n) { return n <= EMB_FEW ? 2 : 8; }
+static long long emb_blocks(long long n) { return (n + 256 * emb_rounds(n) - 1) / (256 * emb_rounds(n)); }
+static long long emb_hist_ints(long long n) { return 256 * emb_blocks(n); }
 extern "C" int l2i_embedding_bwd_scratch(long long n, int V, int D, long long* floats) {
     if (!floats || n < 0 || n > 0x7fffffffLL || V < 1 || V > 0x7fffff00 || D < 1 || D > 65536) return L2I_ERR_ARG;
     if (emb_direct(n, V)) { *floats = 0; return L2I_OK; }
@@ -437,7 +463,7 @@ static void emb_bwd_launch(const EmbBwdArgs& a, hipStream_t s) {
 }
 extern "C" int l2i_embedding_bwd(const long long* tokens, const void* dy, int dy_dtype, void* dw, int dw_dtype, long long n, int V, int D, float scale,
                                  int padding_idx, float* scratch, long long scratch_floats, void* stream) {
-    if (n < 0 || n > 0x7fffffffLL - EMB_TILE || V < 1 || V > 0x7fffff00 || D < 1 || D > 65536 || (dy_dtype | dw_dtype) & ~1) return L2I_ERR_ARG;
+    if (n < 0 || n > 0x7fffffffLL - 2048 || V < 1 || V > 0x7fffff00 || D < 1 || D > 65536 || (dy_dtype | dw_dtype) & ~1) return L2I_ERR_ARG;
     if (!dw || (n && (!tokens || !dy))) return L2I_ERR_ARG;
     long long need = 0;
     if (l2i_embedding_bwd_scratch(n, V, D, &need) != L2I_OK) return L2I_ERR_ARG;
@@ -461,16 +487,21 @@ extern "C" int l2i_embedding_bwd(const long long* tokens, const void* dy, int dy
         while (bits < 31 && (V >> bits)) ++bits;   // keys 0 .. V
         const int passes = (bits + 7) / 8;
         EmbSortArgs a;
-        a.n = (int)n; a.V = V; a.pad = padding_idx; a.hist = hist; a.nblk = (int)((n + EMB_TILE - 1) / EMB_TILE);
+        a.n = (int)n; a.V = V; a.pad = padding_idx; a.hist = hist; a.nblk = (int)emb_blocks(n); a.scanned = a.nblk > EMB_SCAN;
         for (int q = 0; q < passes; ++q) {   // the last pass writes skey / spos
             const bool to_first = (passes - 1 - q) % 2 == 0;
             a.tok = q == 0 ? tokens : nullptr;
             a.kin = to_first ? k2 : skey; a.pin = q == 0 ? nullptr : (to_first ? p2 : spos);
             a.kout = to_first ? skey : k2; a.pout = to_first ? spos : p2;
             a.shift = 8 * q; a.range = q == 0 ? range : nullptr;
-            hipLaunchKernelGGL(embedding_hist_kernel, dim3(a.nblk), dim3(256), 0, s, a);
-            hipLaunchKernelGGL(embedding_scan_kernel, dim3(1), dim3(1024), 0, s, hist, 256 * a.nblk);
-            hipLaunchKernelGGL(embedding_scatter_kernel, dim3(a.nblk), dim3(256), 0, s, a);
+            if (emb_rounds(n) == 2) {
+                hipLaunchKernelGGL((embedding_hist_kernel<2>), dim3(a.nblk), dim3(256), 0, s, a);
+                hipLaunchKernelGGL((embedding_scatter_kernel<2>), dim3(a.nblk), dim3(256), 0, s, a);
+            } else {
+                hipLaunchKernelGGL((embedding_hist_kernel<8>), dim3(a.nblk), dim3(256), 0, s, a);
+                if (a.scanned) hipLaunchKernelGGL(embedding_scan_kernel, dim3(1), dim3(1024), 0, s, hist, 256 * a.nblk);
+                hipLaunchKernelGGL((embedding_scatter_kernel<8>), dim3(a.nblk), dim3(256), 0, s, a);
+            }
         }
     } else if (n) {
         int grid = (int)((n + 63) / 64);

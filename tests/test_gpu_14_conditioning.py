@@ -220,6 +220,7 @@ EMB = [  # tokens' shape, V, D, W, y
     ((5, 3), 7, 180, F32, F32), ((1,), 1, 1, F32, F32), ((256,), 184, 180, F32, BF16), ((33, 31), 500, 64, BF16, BF16), ((5000,), 3, 7, F32, F32),
     ((9000,), 300, 20, BF16, F32), ((20000,), 70000, 8, F32, F32), ((100,), 100000, 1, BF16, F32), ((8192,), 256, 4, F32, F32), ((8193,), 255, 4, F32, F32),
     ((12345,), 1, 100, F32, F32), ((64,), 40, 1026, F32, F32), ((1024,), 9, 520, BF16, BF16), ((1025,), 9, 520, BF16, BF16), ((1000,), 17000, 12, F32, F32),
+    ((32768,), 300, 6, F32, F32), ((32769,), 66000, 6, BF16, BF16), ((131072,), 1000, 3, F32, F32), ((131073,), 40, 3, F32, F32), ((524289,), 70000, 1, F32, F32), ((300, 1001), 70000, 2, F32, F32),
 ]
 
 
