@@ -94,10 +94,11 @@ __device__ __forceinline__ void xa_zero1(f32x16_t& acc) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
 }
-// x = tile a . fa, y = tile b . fb (32 rows each): two chains of products, one behind the other in turn
+// x = tile a . fa, y = tile b . fb (32 rows each; y on top of what it holds if not from0): two chains of products, one behind the other in turn
 template <typename T, int CH>
-__device__ __forceinline__ void xa_rows_dot2(f32x16_t& x, f32x16_t& y, const char* a, const char* b, const XaAddr<T, CH>& ad, const uint4 (&fa)[CH / 2], const uint4 (&fb)[CH / 2]) {
-    xa_zero1(x); xa_zero1(y);
+__device__ __forceinline__ void xa_rows_dot2(f32x16_t& x, f32x16_t& y, const char* a, const char* b, const XaAddr<T, CH>& ad, const uint4 (&fa)[CH / 2], const uint4 (&fb)[CH / 2], bool from0 = true) {
+    xa_zero1(x);
+    if (from0) xa_zero1(y);
 #pragma unroll
     for (int s = 0; s < CH / 2; ++s) {
         xa_dot(x, *reinterpret_cast<const uint4*>(a + ad.row[s]), fa[s], T());
@@ -182,7 +183,9 @@ __device__ __forceinline__ void xa_tdot(f32x16_t (&acc)[ND], const char* tile, c
     }
 }
 
-// workgroups go to the eight XCDs in turn: give each XCD a contiguous range of tiles, so that the tiles which read the same states share its L2
+// workgroups go to the eight XCDs in turn: give each XCD a contiguous range of tiles, so that the tiles which read the same states share its L2.
+// Pair j of an image and a state head is head j / B of image j % B: an XCD has many images' states, not a few images' heads, and no XCD is left
+// with the long ones where lengths differ.
 __device__ __forceinline__ int xa_tile_id(int n) {
     const int per = (n + 7) >> 3;
     return (blockIdx.x & 7) * per + (blockIdx.x >> 3);
@@ -257,11 +260,22 @@ __device__ __forceinline__ unsigned xa_live(unsigned kbits, const unsigned char*
     }
     return m;
 }
+typedef __bf16 xa_bf2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float xa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }   // (below 2^-126: 0)
 // x where bit e of live is set, else `other` (both by bits: two instructions)
 __device__ __forceinline__ float xa_pick(unsigned live, int e, float x, unsigned other) {
-    const unsigned m = (unsigned)((int)(live << (31 - e)) >> 31);
+    const unsigned m = (unsigned)__builtin_amdgcn_sbfe((int)live, e, 1);
     return __uint_as_float((__float_as_uint(x) & m) | (other & ~m));
+}
+// d + the dot product of two chunks, summed in 32 bits
+template <typename T> __device__ __forceinline__ float xa_chunk_dot(const uint4& a, const uint4& b, float d) {
+    const unsigned x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) d = fmaf(__uint_as_float(x[i]), __uint_as_float(y[i]), d);
+        else d = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(xa_bf2_t, x[i]), __builtin_bit_cast(xa_bf2_t, y[i]), d, false);
+    }
+    return d;
 }
 // One 32-row block of an accumulator (times f) to the D values of the lane's row from `row` on; lo: what rounding left, if wanted. bf16: the wave's halves
 // trade registers (their rows are the same) so that each lane stores eight consecutive values at once.
@@ -349,8 +363,8 @@ __global__ __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : (sizeof
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int id = xa_tile_id(total);
     if (id >= total) return;
-    const int bh = id / (nqt * p.ns), rest = id - bh * nqt * p.ns, split = rest / nqt, qt = rest - split * nqt;
-    const int b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int j = id / (nqt * p.ns), rest = id - j * nqt * p.ns, split = rest / nqt, qt = rest - split * nqt;
+    const int hk = j / p.B, b = j - hk * p.B, bh = b * p.Hk + hk;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int r = qt * QT + (WQ == 4 ? wave * 32 : 0) + (lane & 31);
     const int iq = r < p.R ? xa_row_query(p, r) : 0, head = hk * p.G + (r < p.R ? r - iq * p.G : 0);
@@ -398,7 +412,7 @@ __global__ __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : (sizeof
                 tm = fmaxf(tm, sc[kb][e]);
             }
         tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
-        tm = M && tm == -INFINITY ? tm : tm * p.c;   // (c may be 0)
+        tm *= p.c;   // (c > 0: -inf stays)
         if (__any(tm > m + 8.f)) {   // the reference moves only when it has to: what is summed stays below 2^8
             const float mn = fmaxf(m, tm), al = xa_exp2(m - (mn == -INFINITY ? 0.f : mn));
             m = mn;
@@ -413,9 +427,7 @@ __global__ __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : (sizeof
         for (int kb = 0; kb < KT / 32; ++kb) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                float x = fmaf(sc[kb][e], p.c, -ref);
-                if constexpr (M) x = xa_pick(live[kb], e, x, XA_NINF);
-                sc[kb][e] = xa_exp2(x);
+                sc[kb][e] = xa_exp2(fmaf(sc[kb][e], p.c, -ref));
                 l += sc[kb][e];
             }
             xa_tdot<CH, ND>(oacc, vs + kb * 32 * CH * 16, ad, sc[kb]);
@@ -581,7 +593,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void xa_dq_kernel(XaAr
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int id = xa_tile_id(total);
     if (id >= total) return;
-    const int bh = id / nqt, qt = id - bh * nqt, b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int j = id / nqt, qt = id - j * nqt, hk = j / p.B, b = j - hk * p.B, bh = b * p.Hk + hk;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     const int r = qt * 128 + wave * 32 + (lane & 31);
     const bool on = r < p.R;
@@ -612,36 +624,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void xa_dq_kernel(XaAr
     xa_row_frag<T, CH>(gf, on ? reinterpret_cast<const T*>(p.g) + orow : nullptr, p.D);
     float dl = 0.f;
     {
-        uint4 of[S];
+        const bool two = sizeof(T) == 2 && p.lo;   // (what rounding the result left; both parts' loads are in flight together)
+        uint4 of[S], lf[sizeof(T) == 2 ? S : 1];
         xa_row_frag<T, CH>(of, on ? reinterpret_cast<const T*>(p.o) + orow : nullptr, p.D);
+        if constexpr (sizeof(T) == 2) xa_row_frag<T, CH>(lf, on && two ? p.lo + orow : nullptr, p.D);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            constexpr int E = 16 / (int)sizeof(T);
-            const T* ga = reinterpret_cast<const T*>(&gf[s]);
-            const T* oa = reinterpret_cast<const T*>(&of[s]);
-#pragma unroll
-            for (int e = 0; e < E; ++e) dl += OpT<T>::to(ga[e]) * OpT<T>::to(oa[e]);
-        }
-        if constexpr (sizeof(T) == 2) {
-            if (p.lo) {
-                xa_row_frag<T, CH>(of, on ? p.lo + orow : nullptr, p.D);
-#pragma unroll
-                for (int s = 0; s < S; ++s) {
-                    const T* ga = reinterpret_cast<const T*>(&gf[s]);
-                    const T* oa = reinterpret_cast<const T*>(&of[s]);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) dl += bf2f(ga[e]) * bf2f(oa[e]);
-                }
-            }
+            dl = xa_chunk_dot<T>(gf[s], of[s], dl);
+            if constexpr (sizeof(T) == 2) dl = xa_chunk_dot<T>(gf[s], lf[s], dl);
         }
         dl += __shfl_xor(dl, 32, 64);
     }
     const float ls = on ? p.lse[(size_t)bh * p.R + r] : INFINITY;
+    if (ls == INFINITY) dl = 0.f;   // (a row that sees nothing)
     if (on && h == 0) p.delta[(size_t)bh * p.R + r] = dl;
     XaAddr<T, CH> ad;
     f32x16_t acc[ND];
     xa_zero(acc);
+    // masked: 0: every key is live. 1: some are dead for all queries: their rows are zeros in LDS, so that whatever finite number stands in their places
+    // adds nothing (a score of 0 lies far above a row of very low ones: 2^8 at most). 2: by the query's own mask.
     auto work = [&](auto masked, const char* ks, const unsigned (&live)[2]) {
+        constexpr int M = decltype(masked)::value;
         const char* vs = ks + BYTES;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -649,8 +652,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void xa_dq_kernel(XaAr
             xa_rows_dot2<T, CH>(sc, dp, ks + kb * 32 * CH * 16, vs + kb * 32 * CH * 16, ad, qf, gf);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                sc[e] = xa_exp2(fmaf(sc[e], p.c, -ls)) * (dp[e] - dl);
-                if constexpr (decltype(masked)::value) sc[e] = xa_pick(live[kb], e, sc[e], 0u);
+                float x = fmaf(sc[e], p.c, -ls);
+                if constexpr (M == 1) x = fminf(x, 8.f);
+                sc[e] = xa_exp2(x) * (dp[e] - dl);
+                if constexpr (M == 2) sc[e] = xa_pick(live[kb], e, sc[e], 0u);
             }
             xa_tdot<CH, ND>(acc, ks + kb * 32 * CH * 16, ad, sc);
             __builtin_amdgcn_sched_barrier(0);   // (one block of 32 keys at a time: two would not fit the registers)
@@ -666,17 +671,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void xa_dq_kernel(XaAr
     int t = 0;
     for (; t + 1 < tf; t += 2) {
         turn(t, 0);
-        work(std::false_type(), smem, none);
+        work(std::integral_constant<int, 0>(), smem, none);
         turn(t + 1, 1);
-        work(std::false_type(), smem + 2 * BYTES, none);
+        work(std::integral_constant<int, 0>(), smem + 2 * BYTES, none);
     }
-    for (int buf = 0; t < nt; ++t, buf ^= 1) {
+    int buf = 0;
+    if (!st.mb || st.kmask)
+        for (; t < nt; ++t, buf ^= 1) {
+            turn(t, buf);
+            work(std::integral_constant<int, 1>(), smem + buf * 2 * BYTES, none);
+        }
+    for (; t < nt; ++t, buf ^= 1) {
         const unsigned long long kbits = __ballot(st.live(t * KT + lane));
         unsigned live[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) live[kb] = xa_live((unsigned)(kbits >> (32 * kb)), mrow, t * KT + 32 * kb, p.Lk);
         turn(t, buf);
-        work(std::true_type(), smem + buf * 2 * BYTES, live);
+        work(std::integral_constant<int, 2>(), smem + buf * 2 * BYTES, live);
     }
     xa_settle();
     if (!on || !p.dq) return;
@@ -691,11 +702,11 @@ template <typename T, int DP, int WK>
 __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_dkv_kernel(XaArgs p, int nkt, int total) {
     constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, RT = 64, BYTES = RT * CH * 16, KEYS = 32 * WK, ROWS = RT * WK / 4;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float* rowv = reinterpret_cast<float*>(smem + 4 * BYTES);   // two of: [RT] lse, [RT] D, [RT] query of the row
+    float* rowv = reinterpret_cast<float*>(smem + 4 * BYTES);   // two of: [RT] lse, [RT] -D, [RT] query of the row
     const int id = xa_tile_id(total);
     if (id >= total) return;
-    const int bh = id / (nkt * p.ns), rest = id - bh * nkt * p.ns, kt = rest / p.ns, split = rest - kt * p.ns;
-    const int b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int j = id / (nkt * p.ns), rest = id - j * nkt * p.ns, kt = rest / p.ns, split = rest - kt * p.ns;
+    const int hk = j / p.B, b = j - hk * p.B, bh = b * p.Hk + hk;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     const int key = kt * KEYS + (wave % WK) * 32 + (lane & 31), first = wave / WK * ROWS;   // first: of the wave's rows in a tile
     const XaStates<T> st(p, b, hk);
@@ -752,26 +763,29 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_d
         for (int row0 = 0; row0 < ROWS; row0 += 32) {
             unsigned live = 0;
             if constexpr (decltype(masked)::value) {
-                live = klive ? 0xffffu : 0u;
-                if (qmask && klive) {
-                    live = 0;
+                if (klive) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         live |= (st.mb[(long long)reinterpret_cast<const int*>(rv)[2 * RT + row0 + 8 * (e >> 2) + 4 * h + (e & 3)] * p.mq + key] != 0 ? 1u : 0u) << e;
                 }
             }
             f32x16_t pr, ds;
-            xa_rows_dot2<T, CH>(pr, ds, qs + row0 * CH * 16, gs + row0 * CH * 16, ad, kf, vf);
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {   // (dP - D: the products are added to -D)
+                const float4 dl = *reinterpret_cast<const float4*>(rv + RT + row0 + 8 * a + 4 * h);
+                ds[4 * a] = dl.x; ds[4 * a + 1] = dl.y; ds[4 * a + 2] = dl.z; ds[4 * a + 3] = dl.w;
+            }
+            xa_rows_dot2<T, CH>(pr, ds, qs + row0 * CH * 16, gs + row0 * CH * 16, ad, kf, vf, false);
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
-                const float4 ls = *reinterpret_cast<const float4*>(rv + row0 + 8 * a + 4 * h), dl = *reinterpret_cast<const float4*>(rv + RT + row0 + 8 * a + 4 * h);
-                const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dd[4] = {dl.x, dl.y, dl.z, dl.w};
+                const float4 ls = *reinterpret_cast<const float4*>(rv + row0 + 8 * a + 4 * h);
+                const float lv[4] = {ls.x, ls.y, ls.z, ls.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int e = 4 * a + i;
                     pr[e] = xa_exp2(fmaf(pr[e], p.c, -lv[i]));
                     if constexpr (decltype(masked)::value) pr[e] = xa_pick(live, e, pr[e], 0u);
-                    ds[e] = pr[e] * (ds[e] - dd[i]);
+                    ds[e] = pr[e] * ds[e];
                     if constexpr (decltype(masked)::value) ds[e] = xa_pick(live, e, ds[e], 0u);
                 }
             }
@@ -782,24 +796,36 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_d
     };
     auto turn = [&](int t, int buf) {
         float* rv = rowv + buf * 3 * RT;
-        if (threadIdx.x < RT) { rv[threadIdx.x] = nls; rv[RT + threadIdx.x] = ndl; reinterpret_cast<int*>(rv)[2 * RT + threadIdx.x] = niq; }
+        if (threadIdx.x < RT) { rv[threadIdx.x] = nls; rv[RT + threadIdx.x] = -ndl; reinterpret_cast<int*>(rv)[2 * RT + threadIdx.x] = niq; }
         xa_wait_dma<0>();
         __syncthreads();
         if (t + 1 < t1) issue(t + 1, buf ^ 1);
     };
     int t = t0;
-    if (!qmask && __ballot(klive) == ~0ull)
+    if (qmask) {
+        for (int buf = 0; t < t1; ++t, buf ^= 1) {
+            turn(t, buf);
+            work(std::true_type(), smem + buf * 2 * BYTES, mine + buf * 3 * RT);
+        }
+    } else {   // (a dead key's lane works on zeros; what it sums is dropped below)
         for (; t + 1 < t1; t += 2) {
             turn(t, 0);
             work(std::false_type(), smem, mine);
             turn(t + 1, 1);
             work(std::false_type(), smem + 2 * BYTES, mine + 3 * RT);
         }
-    for (int buf = 0; t < t1; ++t, buf ^= 1) {
-        turn(t, buf);
-        work(std::true_type(), smem + buf * 2 * BYTES, mine + buf * 3 * RT);
+        if (t < t1) {
+            turn(t, 0);
+            work(std::false_type(), smem, mine);
+        }
     }
     xa_settle();
+    if (!klive) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) { dk[d][e] = 0.f; dv[d][e] = 0.f; }
+    }
     if constexpr (WK == 2) {   // the second half's sums through LDS to the first
         float* ob = reinterpret_cast<float*>(smem) + (wave & 1) * DP * 64 + (lane & 31);   // [2 DP][32]
         __syncthreads();
@@ -918,7 +944,7 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 2 : 4) void xa_s
         m = fmaxf(m, __shfl_xor(m, 32, 64));
         const float ref = m == -INFINITY ? 0.f : m * p.c;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) { sc[e] = xa_exp2(xa_pick(live, e, fmaf(sc[e], p.c, -ref), XA_NINF)); l += sc[e]; }
+        for (int e = 0; e < 16; ++e) { sc[e] = xa_exp2(fmaf(sc[e], p.c, -ref)); l += sc[e]; }
         l += __shfl_xor(l, 32, 64);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -1216,6 +1242,7 @@ static void xa_setup(XaArgs& a, const void* q, const void* k, const void* v, con
     a.q = q; a.k = k; a.v = v; a.len = lengths; a.mask = mask; a.B = B; a.Lq = Lq; a.Lk = Lk; a.Hk = Hk; a.G = G; a.D = D; a.R = Lq * G;
     a.qb = qb; a.ql = ql; a.qh = qh; a.kb = kb; a.kl = kl; a.kh = kh; a.vb = vb; a.vl = vl; a.vh = vh; a.mb = mb; a.mq = mq;
     a.scale = scale; a.c = fabsf(scale) * 1.44269504088896340736f;
+    if (a.c < 1.17549435e-38f) a.c = 1.17549435e-38f;   // (a scale of 0: scores of 0 all the same, and a dead key's -inf stays)
 }
 // whether out_lo is of use to the backward pass of these sizes: not in f32, nor where D does not come from out
 extern "C" int l2i_cross_attention_wants_lo(int B, int Lq, int Lk, int Hk, int G, int D, int dtype) {

@@ -164,6 +164,19 @@ def test_cross_attention_with_scores_of_any_size():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Lq,Lk", [(1, 200), (50, 150), (50, 20)])
+def test_cross_attention_of_far_low_scores_beside_dead_states(Lq, Lk, dtype):
+    """Every live score lies hundreds below 0, where a state that is not there would score 0 and take the row over (or overflow) if it counted."""
+    q, k, v, g = _xa(2, Lq, Lk, 2, 1, 64, dtype, 17)
+    q, k = q * 0.1 + 6, k * 0.1 - 6                          # scores about -288 with a scale of 1 / 8
+    n = torch.tensor([Lk - 7, Lk // 2], dtype=torch.int32, device=DEV)
+    _check_xa(q, k, v, g, lengths=n)
+    mask = (torch.arange(Lk, device=DEV) % 3 > 0)[None, None]
+    _check_xa(q, k, v, g, mask=mask, lengths=n)
+    _check_xa(q, k, v, g, mask=mask.expand(2, Lq, Lk).contiguous())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_cross_attention_strides(dtype):
     """Slices of a grouped projection, heads in front of positions, states expanded over the batch; gradients come in the leaves' own form."""
     from layout2img_amd import ops
