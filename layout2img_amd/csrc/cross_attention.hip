@@ -16,7 +16,9 @@
 //
 // What bounds it: with 64 values a head, a wave's 32 x 64 scores cost 16 MFMAs (512 cycles) and 32 exponentials a lane with what surrounds
 // them (about 900 cycles), so the vector unit; tiles therefore come to LDS by LDS-DMA (no registers, no instructions of the waves), two
-// buffers deep, and the rescaling of the accumulators waits until the maximum has grown by 2^8.
+// buffers deep, and the rescaling of the accumulators waits until the maximum has grown by 2^8. Measured in bf16: 4096 queries of 16 x 128 over 2048 states
+// of 4 x 128, four images, 277 us (990 TFLOP/s); 4096 queries over up to 512 states of 8 x 64, 16 images, 97 us (530 TFLOP/s; 42 of them for q, out and
+// what rounding left of it). One query of 16 x 128 over up to 4096 states of 4 x 128, 32 images: 35 us (5.8 TB/s) and 4 for the join.
 #include "igemm.h"
 #include <algorithm>
 #include <type_traits>
@@ -586,7 +588,8 @@ __global__ __launch_bounds__(256) void xa_join_kernel(XaArgs p) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq (and D)
-// Four waves x 32 rows, tiles of 64 keys, as the forward; also leaves D for the kernel behind it.
+// Four waves x 32 rows, tiles of 64 keys, as the forward; also leaves D for the kernel behind it. 4096 queries over up to 512 states of 8 x 64, 16 images, bf16:
+// 135 us (570 TFLOP/s), of which reading q, g, out and what rounding left of it and writing dq (335 MB) takes 94 by itself.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void xa_dq_kernel(XaArgs p, int nqt, int total) {
     constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, KT = 64, BYTES = KT * CH * 16;
@@ -698,6 +701,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void xa_dq_kernel(XaAr
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
 // A lane owns one key. WK = 4: four waves x 32 keys, every wave reads all 64 rows of a tile of queries and their gradients. WK = 2: two x 32 keys, a
 // pair of waves each take half of the rows of a tile and are joined at the end. ns > 1: the rows are cut in ns ranges, added in range order by xa_fold_kernel.
+// 16 images of 4096 queries, up to 512 states of 8 x 64, bf16: 155 us (660 TFLOP/s); a workgroup's chain of products and exponentials takes 1.9 us a tile where
+// it is alone on its CU, two share 2.5. Three waves a SIMD do not fit the registers, and 64-row blocks side by side came out the same.
 template <typename T, int DP, int WK>
 __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_dkv_kernel(XaArgs p, int nkt, int total) {
     constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, RT = 64, BYTES = RT * CH * 16, KEYS = 32 * WK, ROWS = RT * WK / 4;
@@ -883,6 +888,7 @@ __global__ __launch_bounds__(256) void xa_fold_kernel(XaArgs p) {
 }
 
 // ------------------------------------------------------------------------------------------------ states that fit one tile
+// 32 images of 4096 queries over 31 states of 4 x 32 with a mask, bf16: forward 24 us (71 MB), backward 34 (105 MB) and 4 for the fold.
 // At most 32 states (a layout's objects): K and V stand in LDS for a whole workgroup, whose waves each walk row blocks of 32 on their own, with no
 // barrier. Bound by bytes: q and out forward; q, g and dq backward -- S, P and D = sum_j P_ij (g_i . v_j) are made from them in registers, so
 // that one launch gives dq and (through a transpose of P and dS in LDS) its rows' share of dk and dv.
@@ -1128,10 +1134,15 @@ static XaPlan xa_plan(int B, long long R, int Lk, int Hk, int D, int dtype) {
     XaPlan q;
     const long long bh = (long long)B * Hk, groups = (R + 127) / 128;   // a workgroup's four waves take at least a block of 32 rows each
     q.nwf = q.nwb = 0;
+    // the one-tile form, forward and forward with backward, against the general one: 32 images of 4096 queries over 31 states of 4 x 32 bf16 17 and 47 us, not 25
+    // and 104; of 4 x 64 f32 75 and 242, not 109 and 548; one query of 8 x 64 bf16 5 and 12, not 7 and 17. Workgroups: 1024 and 512 in all (2048 and 1024: 18 and 51,
+    // 4096 each: 23 and 73): staging the states and joining the shares of dk and dv are paid less often
     if (Lk <= 32 && xa_short_fits(xa_dp(D), dtype)) {
-        q.nwf = (int)std::min(groups, std::max(1LL, (2048 + bh - 1) / bh));
-        q.nwb = (int)std::min(groups, std::max(1LL, (1024 + bh - 1) / bh));
+        q.nwf = (int)std::min(groups, std::max(1LL, (1024 + bh - 1) / bh));
+        q.nwb = (int)std::min(groups, std::max(1LL, (512 + bh - 1) / bh));
     }
+    // up to 32 rows a wave a tile of its own, four tiles at once: 16 rows over 4096 states of 8 x 64 x 8 images 20 us, not 21; 64 images of 256 states 8.7, not 10.1. From
+    // 33 rows on it would read the states twice: 64 images of 64 rows over 100 states 12.5 us, not 8.6 (though over 4096 states 20, not 23)
     q.wq = R <= 32 ? 1 : 4;
     q.nqt = (int)((R + 32 * q.wq - 1) / (32 * q.wq));
     const int kt = q.wq == 4 ? 64 : 128;   // keys a workgroup takes at a time

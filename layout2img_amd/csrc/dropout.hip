@@ -3,6 +3,8 @@
 //   out[i] = keep_i ? in[i] * scale : 0   (+ res[i]),     keep_i = word_i >= threshold
 //   word_{4 j + e} = word e of Philox4x32 (ten rounds) with key = seed and counter = (j, layer, offset)
 // (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011: the rounds and their four constants are the paper's).
+// Bound by bytes: ten rounds are some 70 integer instructions for four elements, hidden under the loads. 33.5 M elements, bf16 in, f32 residual and
+// out: 56 us (6.0 TB/s); their gradient, f32 to bf16: 38 us (5.2 TB/s). 79 k elements: 2.5 us, a launch.
 // The words depend on (seed, offset, layer, i) alone: the backward pass calls the same entry point with in = dy and the (seed, offset)
 // the forward read, and a mask is the same for every launch shape, type and GPU.
 #include "common.h"

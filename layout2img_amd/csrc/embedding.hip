@@ -6,6 +6,8 @@
 // Lookup: bound by bytes (a row read, a row written). Gradient: V rows of D values are written, most of them zeros for a large
 // vocabulary, and n rows of dy are read once in the order of their tokens: (token, position) pairs are sorted stably, so that the rows
 // of a token are added in the order of their positions, by ONE writer -- no float atomics, the same bits on every run.
+// Measured, 16384 skewed tokens of a 32000 x 1024 table in bf16: lookup 11 us (6.0 TB/s), sort 16, rows in the order of their tokens 15, the rest of
+// dW 19 (65 MB written).
 #include "vec.h"
 
 // ------------------------------------------------------------------------------------------------ lookup

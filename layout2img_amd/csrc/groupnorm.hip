@@ -7,11 +7,13 @@
 //
 // Bound by bytes. Two forms:
 //   resident: a workgroup holds all pixels of a slab of whole groups (at least 64 contiguous bytes a pixel) in registers: one launch, every
-//     value read once; used where a slab is at most 32768 values (maps up to 32 x 32 of the wide layers).
+//     value read once; used where a slab is at most 4096 values (8192 in bf16: maps up to 16 x 16 of the wide layers).
 //   split: the map is cut in NCH chunks of rows (pixels) per image. The first launch leaves every chunk's moments (mean and sum of squared
 //     deviations per group: sums around a value of the chunk itself, so that a mean far from zero costs no digits), the second joins
 //     them in a fixed order and writes the result, reading the map a second time -- from the chunk that was read last backwards, on the
 //     XCD that read it, so that L2 and the Infinity Cache still hold what is read first.
+// Measured, B = 32 with silu: 64 x 64 x 128 in bf16 (33.5 MB a map): moments 8.6 us, result 17 (4.0 TB/s), backward sums 19, dx 21 (4.8 TB/s);
+// 128 x 128 x 64 in f32 (134 MB): 25, 43 (6.3 TB/s), 51 (5.2), 66 (6.1) -- what a copy of that size reaches. One 4 x 4 x 1024 image, resident: 6 us.
 // In the backward pass the sums are S1, S2 per group and rows of (sum dz xh | sum dz) per channel, which the ordered fold adds into dgamma / dbeta (in
 // workgroups of their own at the end of the second launch). Statistics are f32; nothing is accumulated by atomics.
 #include "vec.h"
@@ -280,9 +282,8 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(GnArgs p, RowsFoldArg
 #undef GN_L2
 
 // ------------------------------------------------------------------------------------------------ resident form
-// Thread (ty, tx) holds rows ty, ty + nr, ... (at most GN_R) of V channels of the slab. Sums over the slab's groups: row lanes meet in a tree in
+// Thread (ty, tx) holds rows ty, ty + nr, ... (at most R: 4, for maps of two bytes a value up to 8) of V channels of the slab. Sums over the slab's groups: row lanes meet in a tree in
 // LDS (fixed order), a wave adds a group's channels.
-#define GN_R 4
 template <int V>
 __device__ __forceinline__ void gn_channel_sums(const GnArgs& p, int cs, int tx, int ty, bool on, const float (&s)[V], float* red /* [nr][cs] */, float* out /* [cs] */) {
     __syncthreads();
@@ -309,20 +310,20 @@ __device__ __forceinline__ void gn_channel_sums(const GnArgs& p, int cs, int tx,
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;                                \
     const size_t base = ((size_t)b * p.HW + ty) * p.C + c, step = (size_t)p.nr * p.C;
 
-template <typename TI, typename TO, int V, int ACT, int THR>
-__global__ __launch_bounds__(THR) void gn_res_kernel(GnArgs p) {
+template <typename TI, typename TO, int V, int ACT, int R>
+__global__ __launch_bounds__(256) void gn_res_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) float sm[];   // [nr][Cs], [Cs] channel sums, [2][Cs] per-group results
     float *red = sm, *chan = sm + p.nr * p.Cs, *gres = chan + p.Cs;
     GN_RES(V)
     const TI* x = reinterpret_cast<const TI*>(p.x) + base;
-    Vec<TI, V> a[GN_R];
+    Vec<TI, V> a[R];
     float s[V], v[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) s[e] = 0.f;
 #pragma unroll
-    for (int k = 0; k < GN_R; ++k) if (on && ty + k * p.nr < p.HW) a[k].load(x + k * step);
+    for (int k = 0; k < R; ++k) if (on && ty + k * p.nr < p.HW) a[k].load(x + k * step);
 #pragma unroll
-    for (int k = 0; k < GN_R; ++k)
+    for (int k = 0; k < R; ++k)
         if (on && ty + k * p.nr < p.HW) {
             a[k].get(v);
 #pragma unroll
@@ -340,7 +341,7 @@ __global__ __launch_bounds__(THR) void gn_res_kernel(GnArgs p) {
     float m[V], r[V];
     gn_each<V>(on ? c : c0, p.cg, [&](int e, int, int g) { m[e] = gres[g - g0]; s[e] = 0.f; });
 #pragma unroll
-    for (int k = 0; k < GN_R; ++k)
+    for (int k = 0; k < R; ++k)
         if (on && ty + k * p.nr < p.HW) {
             a[k].get(v);
 #pragma unroll
@@ -362,7 +363,7 @@ __global__ __launch_bounds__(THR) void gn_res_kernel(GnArgs p) {
     TO* y = reinterpret_cast<TO*>(p.y) + base;
     gn_each<V>(c, p.cg, [&](int e, int ce, int g) { r[e] = gres[p.Cs + g - g0] * (p.gamma ? p.gamma[ce] : 1.f); s[e] = p.beta ? p.beta[ce] : 0.f; });
 #pragma unroll
-    for (int k = 0; k < GN_R; ++k)
+    for (int k = 0; k < R; ++k)
         if (ty + k * p.nr < p.HW) {
             a[k].get(v);
 #pragma unroll
@@ -371,17 +372,17 @@ __global__ __launch_bounds__(THR) void gn_res_kernel(GnArgs p) {
         }
 }
 
-template <typename TI, typename TO, int V, int ACT, int THR>
-__global__ __launch_bounds__(THR) void gn_res_bwd_kernel(GnArgs p) {
+template <typename TI, typename TO, int V, int ACT, int R>
+__global__ __launch_bounds__(256) void gn_res_bwd_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) float sm[];   // [nr][Cs], [2][Cs] channel sums, [2][Cs] per-group results
     float *red = sm, *ra = sm + p.nr * p.Cs, *rb = ra + p.Cs, *gres = rb + p.Cs;
     GN_RES(V)
     const TI* x = reinterpret_cast<const TI*>(p.x) + base;
     const TO* dy = reinterpret_cast<const TO*>(p.dy) + base;
-    Vec<TI, V> a[GN_R];
-    Vec<TO, V> d[GN_R];
+    Vec<TI, V> a[R];
+    Vec<TO, V> d[R];
 #pragma unroll
-    for (int k = 0; k < GN_R; ++k) if (on && ty + k * p.nr < p.HW) { a[k].load(x + k * step); d[k].load(dy + k * step); }
+    for (int k = 0; k < R; ++k) if (on && ty + k * p.nr < p.HW) { a[k].load(x + k * step); d[k].load(dy + k * step); }
     float m[V], rs[V], A[V], be[V], sa[V], sb[V], v[V], w[V];
     gn_each<V>(on ? c : c0, p.cg, [&](int e, int ce, int g) {
         m[e] = p.mean[(size_t)b * p.G + g]; rs[e] = p.rstd[(size_t)b * p.G + g];
@@ -389,7 +390,7 @@ __global__ __launch_bounds__(THR) void gn_res_bwd_kernel(GnArgs p) {
         sa[e] = 0.f; sb[e] = 0.f;
     });
 #pragma unroll
-    for (int k = 0; k < GN_R; ++k)
+    for (int k = 0; k < R; ++k)
         if (on && ty + k * p.nr < p.HW) {
             a[k].get(v); d[k].get(w);
 #pragma unroll
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(THR) void gn_res_bwd_kernel(GnArgs p) {
     TI* dx = reinterpret_cast<TI*>(p.dx) + base;
     gn_each<V>(c, p.cg, [&](int e, int, int g) { sa[e] = rs[e] * gres[g - g0]; sb[e] = rs[e] * rs[e] * gres[p.Cs + g - g0]; });
 #pragma unroll
-    for (int k = 0; k < GN_R; ++k)
+    for (int k = 0; k < R; ++k)
         if (ty + k * p.nr < p.HW) {
             a[k].get(v); d[k].get(w);
 #pragma unroll
@@ -454,23 +455,20 @@ extern "C" int l2i_group_norm_scratch(int B, long long HW, int C, int G, int bwd
     *floats = ((rows * G * 2 + 3) & ~3LL) + (bwd ? rows * 2 * Cp + (rows > L2I_FOLD_DIRECT ? rows_fold_tmp_floats((int)rows, (int)Cp, 1) : 0) : 0);
     return L2I_OK;
 }
-// resident form: the threads of a workgroup, 0 where a slab does not fit (or nothing is gained: V = 1)
-static int gn_resident(GnArgs& a, int v, int in, int out) {
-    if (v == 1) return 0;
+// resident form: where a slab of whole groups and vectors of four fits a workgroup's registers, 64 bytes of x a thread. Both forms, forward and
+// forward with backward, silu: one bf16 image of 4 x 4 x 1024 7 and 16 us, split 14 and 29; 32 of 16 x 16 x 512 bf16 11 and 28, split 16 and 40; 32 of 12 x 12 x
+// 512 f32 11 and 28, split 13 and 30; at 32 of 16 x 16 x 512 f32 they meet (15 and 38, split 14 and 35). Workgroups of 1024 threads for
+// 32 x 32 x 256 lose (bf16 26 and 60, split 18 and 45), vectors of eight too (32 of 8 x 8 x 1024: 16 and 35, of four 10 and 22).
+static bool gn_resident(GnArgs& a, int v, int in, int out) {
+    if (v == 1) return false;
     const int es = in && out ? 2 : 4;
     int cs = a.cg;
-    while (cs < a.C && (cs % v || cs * es < 64)) cs += a.cg;   // whole groups, whole vectors, 64 bytes of a pixel
+    while (cs < a.C && (cs % 4 || cs * es < 64)) cs += a.cg;   // 64 bytes of a pixel
     if (cs > a.C) cs = a.C;
-    a.Cs = cs; a.slabs = (a.C + cs - 1) / cs; a.tw = cs / v;
-    if (cs % v || a.tw > 256) return 0;
-    for (int thr = 256; thr <= 1024; thr <<= 1) {
-        const int nr = thr / a.tw;
-        if ((long long)nr * GN_R >= a.HW) {
-            a.nr = nr < a.HW ? nr : (int)a.HW;
-            return ((long long)a.nr * cs + 4 * cs) * 4 <= 64 * 1024 ? thr : 0;
-        }
-    }
-    return 0;
+    a.Cs = cs; a.slabs = (a.C + cs - 1) / cs; a.tw = cs / 4;
+    if (cs % 4 || a.tw > 256 || (long long)(256 / a.tw) * (in && out ? 8 : 4) < a.HW) return false;
+    a.nr = 256 / a.tw < a.HW ? 256 / a.tw : (int)a.HW;
+    return true;
 }
 static void gn_setup(GnArgs& a, int B, long long HW, int C, int G, int act, float eps, float* scratch) {
     a.B = B; a.HW = HW; a.C = C; a.Cp = (C + 3) & ~3; a.G = G; a.cg = C / G; a.act = act; a.eps = eps;
@@ -481,14 +479,12 @@ static void gn_setup(GnArgs& a, int B, long long HW, int C, int G, int act, floa
     a.cpart = scratch + ((((long long)B * a.nch * G * 2) + 3) & ~3LL);
 }
 template <typename TI, typename TO, int V, int ACT>
-static void gn_fwd_launch(GnArgs& a, int thr, hipStream_t s) {
-    if constexpr (V > 1) {
-        if (thr) {
+static void gn_fwd_launch(GnArgs& a, bool res, hipStream_t s) {
+    if constexpr (V == 4) {
+        if (res) {
             const size_t lds = sizeof(float) * ((size_t)a.nr * a.Cs + 3 * a.Cs);
-            const dim3 grid(a.B * a.slabs);
-            if (thr == 256) hipLaunchKernelGGL((gn_res_kernel<TI, TO, V, ACT, 256>), grid, dim3(256), lds, s, a);
-            else if (thr == 512) hipLaunchKernelGGL((gn_res_kernel<TI, TO, V, ACT, 512>), grid, dim3(512), lds, s, a);
-            else hipLaunchKernelGGL((gn_res_kernel<TI, TO, V, ACT, 1024>), grid, dim3(1024), lds, s, a);
+            if (a.HW <= 4 * a.nr) hipLaunchKernelGGL((gn_res_kernel<TI, TO, V, ACT, 4>), dim3(a.B * a.slabs), dim3(256), lds, s, a);
+            else if constexpr (sizeof(TI) == 2 && sizeof(TO) == 2) hipLaunchKernelGGL((gn_res_kernel<TI, TO, V, ACT, 8>), dim3(a.B * a.slabs), dim3(256), lds, s, a);
             return;
         }
     }
@@ -497,22 +493,20 @@ static void gn_fwd_launch(GnArgs& a, int thr, hipStream_t s) {
     hipLaunchKernelGGL((gn_apply_kernel<TI, TO, V, ACT>), grid, dim3(256), sizeof(float) * 2 * a.G, s, a);
 }
 template <typename TI, typename TO, int V, int ACT>
-static void gn_bwd_launch(GnArgs& a, int thr, hipStream_t s, float* dgamma, float* dbeta) {
+static void gn_bwd_launch(GnArgs& a, bool res, hipStream_t s, float* dgamma, float* dbeta) {
     int rows = a.B * a.nch;
     bool folded = !dgamma && !dbeta;
-    if constexpr (V > 1) {
-        if (thr) {
+    if constexpr (V == 4) {
+        if (res) {
             const size_t lds = sizeof(float) * ((size_t)a.nr * a.Cs + 4 * a.Cs);
-            const dim3 grid(a.B * a.slabs);
-            if (thr == 256) hipLaunchKernelGGL((gn_res_bwd_kernel<TI, TO, V, ACT, 256>), grid, dim3(256), lds, s, a);
-            else if (thr == 512) hipLaunchKernelGGL((gn_res_bwd_kernel<TI, TO, V, ACT, 512>), grid, dim3(512), lds, s, a);
-            else hipLaunchKernelGGL((gn_res_bwd_kernel<TI, TO, V, ACT, 1024>), grid, dim3(1024), lds, s, a);
+            if (a.HW <= 4 * a.nr) hipLaunchKernelGGL((gn_res_bwd_kernel<TI, TO, V, ACT, 4>), dim3(a.B * a.slabs), dim3(256), lds, s, a);
+            else if constexpr (sizeof(TI) == 2 && sizeof(TO) == 2) hipLaunchKernelGGL((gn_res_bwd_kernel<TI, TO, V, ACT, 8>), dim3(a.B * a.slabs), dim3(256), lds, s, a);
             rows = a.B;
         }
     }
     RowsFoldArgs f = {};
     if (!folded && rows <= L2I_FOLD_DIRECT) f = rows_fold_args4(a.cpart, rows, 2 * a.Cp, 1, dgamma, dbeta, nullptr, nullptr, a.Cp, a.C, 0, 0, nullptr, 2 * a.Cp);
-    if (!thr) {
+    if (!res) {
         hipLaunchKernelGGL((gn_bwd_sums_kernel<TI, TO, V, ACT>), dim3(rows), dim3(256), sizeof(float) * (2 * a.Cp + 512 * V), s, a);
         if (a.dx) {
             const size_t lds = sizeof(float) * 2 * a.G;
@@ -539,11 +533,13 @@ static void gn_bwd_launch(GnArgs& a, int thr, hipStream_t s, float* dgamma, floa
     } while (0)
 #define GN_DISPATCH(FN, ...)                                                                                         \
     do {                                                                                                             \
-        const int vec = vec_width(a.C, (const void*)((size_t)a.x | (size_t)a.dx), x_dtype, (const void*)((size_t)a.y | (size_t)a.dy), y_dtype), thr = gn_resident(a, vec, x_dtype, y_dtype);                    \
-        if (x_dtype == 0 && y_dtype == 0) GN_VECS(FN, float, float, a, thr, __VA_ARGS__);                            \
-        else if (x_dtype == 0) GN_VECS(FN, float, bf16_t, a, thr, __VA_ARGS__);                                      \
-        else if (y_dtype == 0) GN_VECS(FN, bf16_t, float, a, thr, __VA_ARGS__);                                      \
-        else GN_VECS(FN, bf16_t, bf16_t, a, thr, __VA_ARGS__);                                                       \
+        int vec = vec_width(a.C, (const void*)((size_t)a.x | (size_t)a.dx), x_dtype, (const void*)((size_t)a.y | (size_t)a.dy), y_dtype); \
+        const bool res = gn_resident(a, vec, x_dtype, y_dtype);                                                      \
+        if (res) vec = 4;                                                                                            \
+        if (x_dtype == 0 && y_dtype == 0) GN_VECS(FN, float, float, a, res, __VA_ARGS__);                            \
+        else if (x_dtype == 0) GN_VECS(FN, float, bf16_t, a, res, __VA_ARGS__);                                      \
+        else if (y_dtype == 0) GN_VECS(FN, bf16_t, float, a, res, __VA_ARGS__);                                      \
+        else GN_VECS(FN, bf16_t, bf16_t, a, res, __VA_ARGS__);                                                       \
     } while (0)
 
 extern "C" int l2i_group_norm_fwd(const void* x, int x_dtype, const float* gamma, const float* beta, void* y, int y_dtype, float* mean, float* rstd,

@@ -26,6 +26,7 @@ GN = [  # B, spatial, C, G, act, x, y
     (2, (16, 16), 100, 4, "silu", BF16, BF16), (1, (33, 31), 64, 32, "silu", BF16, F32), (2, (64, 64), 32, 1, None, BF16, BF16),
     (4, (8, 8), 96, 96, "silu", F32, F32), (1, (5,), 4096, 1, "relu", BF16, F32), (1, (2, 3), 1023, 33, "silu", F32, F32), (2, (128, 96), 8, 8, "silu", F32, F32),
     (1, (1, 1), 1, 1, None, F32, F32), (70, (2, 2), 16, 4, "silu", F32, F32),
+    (2, (15, 15), 512, 32, "silu", BF16, BF16), (2, (16, 16), 96, 3, "relu", BF16, BF16), (1, (257,), 64, 2, "silu", BF16, BF16), (2, (11, 12), 64, 2, None, BF16, BF16),
 ]
 
 
