@@ -492,6 +492,7 @@ int l2i_group_norm_bwd(const void* x, int x_dtype, const float* gamma, const flo
 /* Attention of queries [B][Lq][Hk G][D] to states [B][Lk][Hk][D] of another length (what l2i_box_attention_* is for a layout's objects among
  * themselves, model/resnet_generator_app_v2.py:79-120): query head h reads state head h / G; D a multiple of 8 up to 128; one type for all.
  * q, k, v: element strides of batch, position and head (any, 0 among them, in whole 16 bytes; the D values are consecutive; 16-byte aligned).
+ * G <= 65536; B Hk times ceil(Lq G / 128), or ceil(Lk / 64), at most 2^24 - 8.
  * lengths [B] int32 or NULL: keys at and behind it are not read. mask: bytes, address b mb + i mq + j, 0 = key j is masked for query i, or NULL;
  * mq = 0: one row for all queries, whose masked keys are not read either. A pair that is masked for some queries only weighs zero: its values
  * have to be finite. A query without a live key gives zeros (and no gradient).

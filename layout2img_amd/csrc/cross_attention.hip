@@ -1157,9 +1157,9 @@ static XaPlan xa_plan(int B, long long R, int Lk, int Hk, int D, int dtype) {
 }
 static bool xa_bad(int B, int Lq, int Lk, int Hk, int G, int D, int dtype) {
     if (B < 1 || Lq < 1 || Lk < 0 || Hk < 1 || G < 1 || D < 8 || D > 128 || D % 8 || (dtype & ~1)) return true;
-    const long long R = (long long)Lq * G;
-    // (rows, tiles and workgroups are counted in 32 bits; the offsets of rows in 64)
-    return R > (1LL << 30) || Lk > (1 << 30) || (long long)B * Hk * ((R + 31) / 32) > (1LL << 28) || (long long)B * Hk * ((Lk + 31) / 32) > (1LL << 28);
+    const long long R = (long long)Lq * G, bh = (long long)B * Hk, most = (1LL << 24) - 8;
+    // (rows are counted in 32 bits, their offsets in 64; a launch has less than 2^32 threads: 2^24 workgroups; a group's head is found by a f32 product)
+    return G > 65536 || R > (1LL << 30) || Lk > (1 << 30) || bh > most || bh * ((R + 127) / 128) > most || bh * (((long long)Lk + 63) / 64) > most;
 }
 extern "C" int l2i_cross_attention_scratch(int B, int Lq, int Lk, int Hk, int G, int D, int dtype, int bwd, long long* floats) {
     if (!floats || xa_bad(B, Lq, Lk, Hk, G, D, dtype)) return L2I_ERR_ARG;

@@ -13,7 +13,7 @@ struct DropArgs {
     const void* in; const void* res; void* out;
     const long long* rng;   // device: seed, offset
     long long* used;        // device, optional: the pair this launch read
-    long long n;
+    long long n, j0;        // j0: first block of four of the launch
     unsigned threshold; int all, layer; float scale;   // all: threshold 2^32, nothing is kept
 };
 
@@ -31,8 +31,8 @@ __device__ __forceinline__ uint4 philox4x32(unsigned k0, unsigned k1, uint4 c) {
 template <typename TI, typename TO, bool VEC>
 __global__ __launch_bounds__(256) void dropout_kernel(DropArgs p) {
     const unsigned long long seed = (unsigned long long)p.rng[0], off = (unsigned long long)p.rng[1];
-    if (p.used && blockIdx.x == 0 && threadIdx.x == 0) { p.used[0] = (long long)seed; p.used[1] = (long long)off; }
-    const long long j = (long long)blockIdx.x * 256 + threadIdx.x, i = 4 * j;
+    if (p.used && p.j0 == 0 && blockIdx.x == 0 && threadIdx.x == 0) { p.used[0] = (long long)seed; p.used[1] = (long long)off; }
+    const long long j = p.j0 + (long long)blockIdx.x * 256 + threadIdx.x, i = 4 * j;
     if (i >= p.n) return;
     const TI* in = reinterpret_cast<const TI*>(p.in) + i;
     const TO* res = p.res ? reinterpret_cast<const TO*>(p.res) + i : nullptr;
@@ -55,11 +55,15 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropArgs p) {
 }
 
 template <typename TI, typename TO>
-static void dropout_launch(const DropArgs& a, hipStream_t s) {
-    const unsigned grid = (unsigned)(((a.n + 3) / 4 + 255) / 256);
+static void dropout_launch(DropArgs a, hipStream_t s) {
     const bool vec = !((size_t)a.in & (4 * sizeof(TI) - 1)) && !(((size_t)a.out | (size_t)a.res) & (4 * sizeof(TO) - 1));
-    if (vec) hipLaunchKernelGGL((dropout_kernel<TI, TO, true>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((dropout_kernel<TI, TO, false>), dim3(grid), dim3(256), 0, s, a);
+    const long long blocks = ((a.n + 3) / 4 + 255) / 256, most = 1LL << 23;   // (a launch has less than 2^32 threads)
+    for (long long i = 0; i < blocks; i += most) {
+        a.j0 = i * 256;
+        const dim3 grid((unsigned)(blocks - i < most ? blocks - i : most));
+        if (vec) hipLaunchKernelGGL((dropout_kernel<TI, TO, true>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((dropout_kernel<TI, TO, false>), grid, dim3(256), 0, s, a);
+    }
 }
 
 extern "C" int l2i_dropout(const void* in, int in_dtype, const void* res, void* out, int out_dtype, const long long* rng, long long* used,

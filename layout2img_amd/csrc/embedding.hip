@@ -280,6 +280,7 @@ struct EmbBwdArgs {
     float* part /* [chunks][2][D]: come in, go on */; void* dw;
     int n, V, D, chunk, nch; float scale;
     int tx;   // lanes along a row: a power of two
+    int v0;   // first row of the launch (embedding_rows_kernel)
 };
 
 template <typename TO, typename TW, int V>
@@ -342,7 +343,7 @@ template <typename TW, int V>
 __global__ __launch_bounds__(256) void embedding_rows_kernel(EmbBwdArgs p) {
     __shared__ int ra[EMB_VROWS], rk[EMB_VROWS];   // first chunk of a row and chunks it runs through; 0: absent, 1: finished
     __shared__ float red[256 * V];
-    const int v0 = blockIdx.x * EMB_VROWS, nv = min(EMB_VROWS, p.V - v0);
+    const int v0 = p.v0 + blockIdx.x * EMB_VROWS, nv = min(EMB_VROWS, p.V - v0);
     if ((int)threadIdx.x < nv) {
         const int2 a = p.n ? p.range[v0 + threadIdx.x] : make_int2(-1, 0);
         ra[threadIdx.x] = a.x / p.chunk;
@@ -400,6 +401,7 @@ __global__ __launch_bounds__(256) void embedding_rows_kernel(EmbBwdArgs p) {
 }
 
 // ------------------------------------------------------------------------------------------------ entry points
+#define EMB_GRID (1LL << 23)   // workgroups of a launch, which has less than 2^32 threads: what takes more is cut
 static int emb_lanes(int D, int E) {
     int tx = 1;
     while (tx < 256 && tx * E < D) tx <<= 1;
@@ -409,10 +411,16 @@ template <typename TI, typename TO>
 static void emb_fwd_launch(EmbArgs a, hipStream_t s) {
     const int v = vec_width(a.D, a.w, sizeof(TI) == 2, a.out, sizeof(TO) == 2);
     a.tx = emb_lanes(a.D, v);
-    const dim3 grid((unsigned)((a.n + 256 / a.tx - 1) / (256 / a.tx)));
-    if (v == 8) hipLaunchKernelGGL((embedding_fwd_kernel<TI, TO, 8>), grid, dim3(256), 0, s, a);
-    else if (v == 4) hipLaunchKernelGGL((embedding_fwd_kernel<TI, TO, 4>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((embedding_fwd_kernel<TI, TO, 1>), grid, dim3(256), 0, s, a);
+    const long long n = a.n, per = 256 / a.tx;
+    for (long long i = 0; i < n; i += per * EMB_GRID) {
+        a.n = n - i < per * EMB_GRID ? n - i : per * EMB_GRID;
+        const dim3 grid((unsigned)((a.n + per - 1) / per));
+        if (v == 8) hipLaunchKernelGGL((embedding_fwd_kernel<TI, TO, 8>), grid, dim3(256), 0, s, a);
+        else if (v == 4) hipLaunchKernelGGL((embedding_fwd_kernel<TI, TO, 4>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((embedding_fwd_kernel<TI, TO, 1>), grid, dim3(256), 0, s, a);
+        a.tok += per * EMB_GRID;
+        a.out = reinterpret_cast<TO*>(a.out) + (size_t)per * EMB_GRID * a.D;
+    }
 }
 extern "C" int l2i_embedding_fwd(const void* weight, int w_dtype, const long long* tokens, void* out, int out_dtype, long long n, int V, int D,
                                  float scale, int padding_idx, void* stream) {
@@ -430,7 +438,7 @@ extern "C" int l2i_embedding_fwd(const void* weight, int w_dtype, const long lon
 // scratch, in ints: sorted keys and positions [n] each, the tokens' ranges [V][2], a second pair of them and the histogram when the radix sort runs, then the partial rows
 static int emb_chunk(long long n) { return n <= 2048 ? 8 : n <= 8192 ? 16 : n <= 65536 ? 32 : 128; }   // few pairs: more workgroups; many: fewer partial rows
 // every row of dW looks through all pairs: few pairs, and not millions of rows
-static bool emb_direct(long long n, int V) { return n <= EMB_DIRECT && n * V <= (1 << 24); }
+static bool emb_direct(long long n, int V) { return n <= EMB_DIRECT && n * V <= (1 << 24) && V <= EMB_GRID; }
 static long long emb_al(long long ints) { return (ints + 3) & ~3LL; }
 static int emb_rounds(long long n) { return n <= EMB_FEW ? 2 : 8; }
 static long long emb_blocks(long long n) { return (n + 256 * emb_rounds(n) - 1) / (256 * emb_rounds(n)); }
@@ -452,9 +460,13 @@ static void emb_direct_launch(const EmbDirectArgs& a, hipStream_t s) {
 template <typename TO, typename TW, int V>
 static void emb_bwd_kernels(EmbBwdArgs a, hipStream_t s) {
     a.tx = emb_lanes(a.D, V);
-    const unsigned grid = (unsigned)((a.V + EMB_VROWS - 1) / EMB_VROWS), per = 256 / a.tx;
+    const long long groups = ((long long)a.V + EMB_VROWS - 1) / EMB_VROWS;
+    const unsigned per = 256 / a.tx;
     if (a.n) hipLaunchKernelGGL((embedding_part_kernel<TO, TW, V>), dim3((a.nch + per - 1) / per), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((embedding_rows_kernel<TW, V>), dim3(grid), dim3(256), 0, s, a);
+    for (long long i = 0; i < groups; i += EMB_GRID) {
+        a.v0 = (int)(i * EMB_VROWS);
+        hipLaunchKernelGGL((embedding_rows_kernel<TW, V>), dim3((unsigned)(groups - i < EMB_GRID ? groups - i : EMB_GRID)), dim3(256), 0, s, a);
+    }
 }
 template <typename TO, typename TW>
 static void emb_bwd_launch(const EmbBwdArgs& a, hipStream_t s) {
@@ -513,7 +525,7 @@ extern "C" int l2i_embedding_bwd(const long long* tokens, const void* dy, int dy
         else hipLaunchKernelGGL((embedding_rank_kernel<16>), dim3(grid), dim3(1024), 0, s, tokens, (int)n, V, padding_idx, skey, spos, range);
     }
     EmbBwdArgs b;
-    b.skey = skey; b.spos = spos; b.range = range; b.dy = dy; b.part = reinterpret_cast<float*>(end); b.dw = dw; b.n = (int)n; b.V = V; b.D = D; b.scale = scale; b.tx = 0;
+    b.skey = skey; b.spos = spos; b.range = range; b.dy = dy; b.part = reinterpret_cast<float*>(end); b.dw = dw; b.n = (int)n; b.V = V; b.D = D; b.scale = scale; b.tx = 0; b.v0 = 0;
     b.chunk = emb_chunk(n); b.nch = (int)((n + b.chunk - 1) / b.chunk);
     if (dy_dtype == 0) { if (dw_dtype == 0) emb_bwd_launch<float, float>(b, s); else emb_bwd_launch<float, bf16_t>(b, s); }
     else { if (dw_dtype == 0) emb_bwd_launch<bf16_t, float>(b, s); else emb_bwd_launch<bf16_t, bf16_t>(b, s); }

@@ -2211,7 +2211,8 @@ def _aligned(t):
 
 def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
     """softmax(scale q k^T) v of queries q (B, Lq, H, D) over the states k, v (B, Lk, Hk, D) of another sequence -> (B, Lq, H, D), all f32 or all bf16.
-    H is a multiple of Hk: query head h reads state head h // (H // Hk). D: a multiple of 8, at most 128. scale: default 1 / sqrt(D).
+    H is a multiple of Hk: query head h reads state head h // (H // Hk). D: a multiple of 8, at most 128. scale: default 1 / sqrt(D). B * Hk times the
+    rows of a head group over 128 (or the states over 64) stays below 2^24.
     lengths: (B,) int32, states at and behind a sequence's length do not exist. mask: (B | 1, Lq | 1, Lk) bool, False = query i does not see state j.
     A query that sees no state gives zeros. What `lengths` or a mask row shared by all queries takes out is not read, whatever it holds; a state
     that only some queries see has to be finite. The D values of a head are consecutive; the other strides may be any of whole 16 bytes (slices of
@@ -2231,7 +2232,10 @@ def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
         raise RuntimeError(f"cross_attention: {H} query heads do not divide over {Hk} state heads")
     if B < 1 or Lq < 1:
         raise RuntimeError(f"cross_attention: at least one query, got {tuple(q.shape)}")
-    args = (B, Lq, Lk, Hk, H // Hk, D) + _strides3(q, "q") + _strides3(k, "k") + _strides3(v, "v")
+    G = H // Hk
+    if G > 65536 or max(Lq * G, Lk) > 1 << 30 or B * Hk * max((Lq * G + 127) // 128, (Lk + 63) // 64, 1) > (1 << 24) - 8:
+        raise RuntimeError(f"cross_attention: less than 2^24 tiles of 128 rows or 64 states and groups of at most 65536 heads, got {tuple(q.shape)} and {tuple(k.shape)}")
+    args = (B, Lq, Lk, Hk, G, D) + _strides3(q, "q") + _strides3(k, "k") + _strides3(v, "v")
     if lengths is not None and (_op(lengths, "cross_attention: lengths", torch.int32).shape != (B,) or not lengths.is_contiguous()):
         raise RuntimeError(f"cross_attention: lengths is a contiguous ({B},) tensor, got {tuple(lengths.shape)}, strides {lengths.stride()}")
     if mask is not None:

@@ -52,6 +52,10 @@ def test_cross_attention_refusals():
     for d in (4, 12, 136, 0):
         _refused("multiple of 8", f, Z(1, 1, 1, d), Z(1, 1, 1, d), Z(1, 1, 1, d))
     _refused("divide", f, q, Z(2, 5, 3, 16), Z(2, 5, 3, 16))
+    one = Z(1, 1, 1, 8)
+    for shapes in (((1 << 24, 1, 1, 8), (1 << 24, 1, 1, 8)), ((1, 1, 65537, 8), (1, 1, 1, 8)), ((1 << 14, 1 << 17, 1, 8), (1 << 14, 1, 1, 8)),
+                   ((1 << 14, 1, 1, 8), (1 << 14, 1 << 16, 1, 8)), ((1, (1 << 30) + 1, 1, 8), (1, 1, 1, 8))):
+        _refused("tiles", f, one.expand(shapes[0]), one.expand(shapes[1]), one.expand(shapes[1]))
     _refused("at least one", f, Z(2, 0, 4, 16), k, k)
     _refused("consecutive", f, Z(2, 3, 16, 4).transpose(2, 3), k, k)
     _refused("16-byte", f, Z(2, 3, 4, 18)[..., :16], k, k)
@@ -131,7 +135,7 @@ def test_entry_points_refuse_before_a_launch():
         q, k, v, dt, None, None, o, lo, None, B, Lq, Lk, Hk, G, D, *st, mb, mq, 1.0, s, n, None)
     for bad in (dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(dt=2), dict(B=0), dict(Lq=0), dict(Lk=-1), dict(Hk=0), dict(G=0), dict(D=0), dict(D=12),
                 dict(D=136), dict(q=P + 8), dict(o=P + 2), dict(st=(4,) + (0,) * 8), dict(st=(0,) * 8 + (-8,)), dict(mb=-1), dict(mq=-1), dict(Lq=1 << 30, G=2),
-                dict(lo=P, dt=0), dict(lo=P + 8), dict(Lk=100000)):   # (the last one needs scratch)
+                dict(lo=P, dt=0), dict(lo=P + 8), dict(B=1 << 24), dict(G=65537), dict(B=1 << 14, Lq=1 << 17, G=1), dict(B=1 << 14, Lk=1 << 16), dict(Lk=100000)):   # (the last one needs scratch)
         assert xa(**bad) == -1, bad
     xb = lambda lse=P, g=P, dq=P, dk=P, dv=P, s=P, n=big: lib.l2i_cross_attention_bwd(
         P, P, P, 1, None, None, P, None, lse, g, dq, dk, dv, 2, 3, 5, 2, 2, 16, *(0,) * 11, 1.0, s, n, None)

@@ -266,6 +266,25 @@ def test_embedding_of_nothing_and_of_a_transposed_batch():
     assert torch.equal(ops.embedding(w, tok.t()), w[tok.t()])
 
 
+def test_embedding_of_more_rows_than_a_launch_has_workgroups():
+    from layout2img_amd import ops
+    w = torch.arange(1.0, 3 * 255 + 1, device=DEV).view(3, 255).to(BF16)      # a workgroup a row
+    n = (1 << 24) + 5
+    tok = torch.arange(n, device=DEV) % 3
+    y = ops.embedding(w, tok)
+    for at in (0, (1 << 23) - 1, 1 << 23, (1 << 23) + 1, (1 << 24) - 1, 1 << 24, n - 1):
+        assert torch.equal(y[at], w[at % 3]), at
+    assert int((y[:, 254] == w[tok, 254]).sum()) == n
+    del y
+    for V, toks in (((1 << 23) + 5, [(1 << 23) + 4]), ((1 << 27) + 9, [0, 1 << 26, (1 << 26) - 1, (1 << 27) + 8, 1 << 26]), ((1 << 23) + 5, [])):
+        w = torch.zeros(V, 1, device=DEV, requires_grad=True)
+        t = torch.tensor(toks, dtype=torch.int64, device=DEV)
+        dy = torch.arange(1.0, len(toks) + 1, device=DEV)[:, None]
+        (dw,) = torch.autograd.grad(ops.embedding(w, t), (w,), dy)
+        want = torch.zeros(V, 1, device=DEV).index_add_(0, t, dy)
+        assert torch.equal(dw, want)
+
+
 def test_embedding_table_past_32_bits():
     from layout2img_amd import ops
     V, D = (1 << 24) + 3, 136                                   # 2.3e9 values
@@ -314,6 +333,17 @@ def test_dropout_of_infinities_off_alignment_and_far_elements():
     tail = y[4 * first:].float().cpu()
     on = R.keep(2 ** 64 - 5, 77, 0, len(tail), 0.25, first)
     assert torch.equal(tail != 0, on)
+
+
+def test_dropout_of_more_elements_than_a_launch_takes():
+    from layout2img_amd import ops
+    rng = torch.tensor([3, 9], dtype=torch.int64, device=DEV)
+    n = (1 << 33) + 9
+    x = torch.ones(n, dtype=BF16, device=DEV)
+    y = ops.dropout(x, 0.25, rng, layer=2)
+    for first in (0, (1 << 31) - 8, 1 << 31):                 # in blocks of four
+        part = y[4 * first:4 * first + 64].float().cpu()
+        assert torch.equal(part != 0, R.keep(3, 9, 2, len(part), 0.25, first)), first
 
 
 def test_dropout_keeps_its_share_and_its_mask():
