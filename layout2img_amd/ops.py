@@ -2082,15 +2082,14 @@ def _wants_grad(*ts):
 
 
 def _group_norm_fwd(x, sizes, weight, bias, eps, act, op_dtype):
-    """sizes: (B, HW, C, G). -> y, (2, B, G) mean and rstd"""
+    """sizes: (B, HW, C, G). -> y, mean (B, G) and rstd (B, G) one behind the other, with the call's scratch behind them"""
     B, HW, C, G = sizes
-    dev = x.device
-    y = torch.empty(x.shape, dtype=op_dtype, device=dev)
-    st = torch.empty((2, B, G), dtype=torch.float32, device=dev)
+    y = torch.empty(x.shape, dtype=op_dtype, device=x.device)
+    n, wn = (2 * B * G + 3) & ~3, _scratch_floats("l2i_group_norm_scratch", B, HW, C, G, 0)
+    st = torch.empty(n + wn, dtype=torch.float32, device=x.device)
     mean = st.data_ptr()
-    ws, wp, wn = _scratch(dev, "l2i_group_norm_scratch", B, HW, C, G, 0)
     _lib.call("l2i_group_norm_fwd", x.data_ptr(), _code(x.dtype), _p(weight), _p(bias), y.data_ptr(), _code(op_dtype), mean, mean + 4 * B * G,
-              B, HW, C, G, eps, act, wp, wn, _stream())
+              B, HW, C, G, eps, act, mean + 4 * n, wn, _stream())
     return y, st
 
 
@@ -2145,16 +2144,44 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act=None, op_dty
     return _group_norm_fwd(x, sizes, weight, bias, eps, _ACTS[act], op_dtype)[0]
 
 
-def _strides3(t, what):
-    """Element strides of (batch, position, head), 0 for a dimension of one; refuses what the kernels do not read."""
-    s, n = t.stride(), t.shape
+def _strides3(s, n, what, bf16):
+    """Strides s of (batch, position, head), 0 for a dimension of one; refuses what the kernels do not read."""
     r = (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
-    if s[3] != 1 or (r[0] | r[1] | r[2]) & (7 if t.dtype is torch.bfloat16 else 3) or t.data_ptr() & 15:
-        raise RuntimeError(f"cross_attention: {what} needs consecutive head values and rows on 16-byte boundaries, got strides {s} "
-                           f"at address {t.data_ptr() % 16} modulo 16 (.contiguous() first)")
+    if s[3] != 1 or (r[0] | r[1] | r[2]) & (7 if bf16 else 3):
+        raise RuntimeError(f"cross_attention: {what} needs consecutive head values and rows on 16-byte boundaries, got strides {s} (.contiguous() first)")
     if r[1] >= 1 << 22 or r[2] >= 1 << 28:
         raise RuntimeError(f"cross_attention: {what} steps by less than 2^22 values from position to position and 2^28 from head to head, got {s}")
     return r
+
+
+@functools.lru_cache(maxsize=4096)
+def _xa_args(q, k, v, sq, sk, sv, mask, sm, bf16):
+    """(B, Lq, Lk, Hk, G, D) and the strides, as the library takes them, from the shapes and strides of q, k, v and the mask (or None): worked out once
+    for a set of them."""
+    for n, what in ((q, "q"), (k, "k"), (v, "v")):
+        if len(n) != 4:
+            raise RuntimeError(f"cross_attention: {what} is (B, L, heads, D), got {tuple(n)}")
+    B, Lq, H, D = q
+    if k != v or k[0] != B or k[3] != D:
+        raise RuntimeError(f"cross_attention: q {tuple(q)}, k {tuple(k)}, v {tuple(v)} do not belong together")
+    Lk, Hk = k[1], k[2]
+    if D % 8 or not 8 <= D <= 128:
+        raise RuntimeError(f"cross_attention: a head has a multiple of 8 values, at most 128; got {D}")
+    if Hk < 1 or H < 1 or H % Hk:
+        raise RuntimeError(f"cross_attention: {H} query heads do not divide over {Hk} state heads")
+    if B < 1 or Lq < 1:
+        raise RuntimeError(f"cross_attention: at least one query, got {tuple(q)}")
+    G = H // Hk
+    if G > 65536 or max(Lq * G, Lk) > 1 << 30 or B * Hk * max((Lq * G + 127) // 128, (Lk + 63) // 64, 1) > (1 << 24) - 8:
+        raise RuntimeError(f"cross_attention: less than 2^24 tiles of 128 rows or 64 states and groups of at most 65536 heads, got {tuple(q)} and {tuple(k)}")
+    args = (B, Lq, Lk, Hk, G, D) + _strides3(sq, q, "q", bf16) + _strides3(sk, k, "k", bf16) + _strides3(sv, v, "v", bf16)
+    if mask is None:
+        return args + (0, 0)
+    if len(mask) != 3 or mask[0] not in (1, B) or mask[1] not in (1, Lq) or mask[2] != Lk:
+        raise RuntimeError(f"cross_attention: mask is ({B} or 1, {Lq} or 1, {Lk}) bool, got {tuple(mask)}")
+    if Lk > 1 and sm[2] != 1:
+        raise RuntimeError("cross_attention: the mask's last dimension has to be consecutive (.contiguous() first)")
+    return args + (sm[0] if mask[0] > 1 else 0, sm[1] if mask[1] > 1 else 0)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2217,37 +2244,18 @@ def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
     A query that sees no state gives zeros. What `lengths` or a mask row shared by all queries takes out is not read, whatever it holds; a state
     that only some queries see has to be finite. The D values of a head are consecutive; the other strides may be any of whole 16 bytes (slices of
     a grouped projection, transposed heads, expanded batches), less than 2^22 values from position to position."""
-    for t, what in ((q, "cross_attention: q"), (k, "cross_attention: k"), (v, "cross_attention: v")):
-        if _op(t, what).dim() != 4:
-            raise RuntimeError(f"{what} is (B, L, heads, D), got {tuple(t.shape)}")
-        if t.dtype != q.dtype:
-            raise RuntimeError(f"cross_attention: q, k, v have one type, got {q.dtype} and {t.dtype}")
-    B, Lq, H, D = q.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
-        raise RuntimeError(f"cross_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not belong together")
-    Lk, Hk = k.shape[1], k.shape[2]
-    if D % 8 or not 8 <= D <= 128:
-        raise RuntimeError(f"cross_attention: a head has a multiple of 8 values, at most 128; got {D}")
-    if Hk < 1 or H < 1 or H % Hk:
-        raise RuntimeError(f"cross_attention: {H} query heads do not divide over {Hk} state heads")
-    if B < 1 or Lq < 1:
-        raise RuntimeError(f"cross_attention: at least one query, got {tuple(q.shape)}")
-    G = H // Hk
-    if G > 65536 or max(Lq * G, Lk) > 1 << 30 or B * Hk * max((Lq * G + 127) // 128, (Lk + 63) // 64, 1) > (1 << 24) - 8:
-        raise RuntimeError(f"cross_attention: less than 2^24 tiles of 128 rows or 64 states and groups of at most 65536 heads, got {tuple(q.shape)} and {tuple(k.shape)}")
-    args = (B, Lq, Lk, Hk, G, D) + _strides3(q, "q") + _strides3(k, "k") + _strides3(v, "v")
-    if lengths is not None and (_op(lengths, "cross_attention: lengths", torch.int32).shape != (B,) or not lengths.is_contiguous()):
-        raise RuntimeError(f"cross_attention: lengths is a contiguous ({B},) tensor, got {tuple(lengths.shape)}, strides {lengths.stride()}")
+    dtype = _op(q, "cross_attention: q").dtype
+    if _op(k, "cross_attention: k").dtype is not dtype or _op(v, "cross_attention: v").dtype is not dtype:
+        raise RuntimeError(f"cross_attention: q, k, v have one type, got {dtype}, {k.dtype} and {v.dtype}")
     if mask is not None:
-        if _op(mask, "cross_attention: mask", torch.bool).dim() != 3 or mask.shape[0] not in (1, B) or mask.shape[1] not in (1, Lq) or mask.shape[2] != Lk:
-            raise RuntimeError(f"cross_attention: mask is ({B} or 1, {Lq} or 1, {Lk}) bool, got {tuple(mask.shape)}")
-        if Lk > 1 and mask.stride(2) != 1:
-            raise RuntimeError("cross_attention: the mask's last dimension has to be consecutive (.contiguous() first)")
-        ms = mask.stride()
-        args += (ms[0] if mask.shape[0] > 1 else 0, ms[1] if mask.shape[1] > 1 else 0)
-    else:
-        args += (0, 0)
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+        _op(mask, "cross_attention: mask", torch.bool)
+    args = _xa_args(q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), None if mask is None else mask.shape,
+                    None if mask is None else mask.stride(), dtype is torch.bfloat16)
+    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        raise RuntimeError("cross_attention: q, k, v have to start on 16-byte boundaries (.contiguous() or .clone() first)")
+    if lengths is not None and (_op(lengths, "cross_attention: lengths", torch.int32).shape != (args[0],) or not lengths.is_contiguous()):
+        raise RuntimeError(f"cross_attention: lengths is a contiguous ({args[0]},) tensor, got {tuple(lengths.shape)}, strides {lengths.stride()}")
+    scale = 1.0 / math.sqrt(args[5]) if scale is None else float(scale)
     _same_device(q, k, v, lengths, mask)
     if _wants_grad(q, k, v):
         return CrossAttentionFn.apply(q, k, v, lengths, mask, scale, args)
