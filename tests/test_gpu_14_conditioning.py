@@ -69,6 +69,20 @@ def test_group_norm_of_a_map_off_its_alignment():
     R.close(ops.group_norm_act(x, 4, act="silu"), want[0], tol[0], "y")
 
 
+def test_group_norm_of_maps_past_32_bits():
+    """More values than 2^31; the last image is the first one again."""
+    from layout2img_amd import ops
+    gen = _gen(22)
+    x = _rnd(gen, 3, 700, 1024, 1024, dtype=BF16)
+    x[2] = x[0]
+    x.requires_grad_()
+    w = (1 + 0.2 * _rnd(gen, 1024)).requires_grad_()
+    y = ops.group_norm_act(x, 32, w, act="silu")
+    assert y.numel() > 1 << 31 and torch.equal(y[2], y[0])
+    (dx, dw) = torch.autograd.grad(y, (x, w), y.detach())
+    assert torch.equal(dx[2], dx[0]) and dw.isfinite().all()
+
+
 # ------------------------------------------------------------------------------------------------ cross attention
 def _xa(B, Lq, Lk, Hk, G, D, dtype, seed, lengths=None, mask=None):
     gen = _gen(seed)
@@ -217,6 +231,25 @@ def test_cross_attention_far_offsets_in_a_long_cache():
     q = _rnd(gen, B, 3, 1, D, dtype=BF16)
     a = ops.cross_attention(q, cache[:, :, :1], cache[:, :, 1:])
     assert torch.equal(a, ops.cross_attention(q, kv[:, :, :1].contiguous(), kv[:, :, 1:].contiguous()))
+
+
+def test_cross_attention_of_queries_past_32_bits():
+    """More query values than 2^31, a block of 128 rows over and over: its results repeat bit for bit, and dv's rows add up to the number of queries."""
+    from layout2img_amd import ops
+    gen = _gen(21)
+    n, D = (1 << 17) + 1, 128
+    block = _rnd(gen, 1, 128, 1, D, dtype=BF16)
+    q = block.repeat(1, n, 1, 1).requires_grad_()
+    k, v = (_rnd(gen, 1, 40, 1, D, dtype=BF16).requires_grad_() for _ in range(2))
+    y = ops.cross_attention(q, k, v)
+    assert y.numel() > 1 << 31
+    for part in (1, n // 2, n - 1):
+        assert torch.equal(y[:, 128 * part:128 * part + 128], y[:, :128]), part
+    dq, dk, dv = torch.autograd.grad(y, (q, k, v), torch.ones(1, device=DEV, dtype=BF16).expand_as(y).contiguous())
+    for part in (1, n // 2, n - 1):
+        assert torch.equal(dq[:, 128 * part:128 * part + 128], dq[:, :128]), part
+    # P and dv are rounded to bf16 (2^-9 each), a sum of 4096 steps a range in 32 bits errs by 2^-12: below 2^-7
+    assert torch.allclose(dv.double().sum(1), torch.tensor(128.0 * n, dtype=torch.float64, device=DEV), rtol=2.0 ** -7, atol=0.0) and dk.isfinite().all()
 
 
 def test_cross_attention_no_states():
