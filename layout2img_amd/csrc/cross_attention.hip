@@ -98,7 +98,8 @@ __device__ __forceinline__ void xa_zero1(f32x16_t& acc) {
 }
 // x = tile a . fa, y = tile b . fb (32 rows each; y on top of what it holds if not from0): two chains of products, one behind the other in turn
 template <typename T, int CH>
-__device__ __forceinline__ void xa_rows_dot2(f32x16_t& x, f32x16_t& y, const char* a, const char* b, const XaAddr<T, CH>& ad, const uint4 (&fa)[CH / 2], const uint4 (&fb)[CH / 2], bool from0 = true) {
+__device__ __forceinline__ void xa_rows_dot2(f32x16_t& x, f32x16_t& y, const char* a, const char* b, const XaAddr<T, CH>& ad, const uint4 (&fa)[CH / 2],
+                                             const uint4 (&fb)[CH / 2], bool from0 = true) {
     xa_zero1(x);
     if (from0) xa_zero1(y);
 #pragma unroll
@@ -656,7 +657,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void xa_dq_kernel(XaAr
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 float x = fmaf(sc[e], p.c, -ls);
-                if constexpr (M == 1) x = fminf(x, 8.f);
+                if constexpr (M == 1) x = x > 8.f ? 8.f : x;   // (not fminf: a NaN stays)
                 sc[e] = xa_exp2(x) * (dp[e] - dl);
                 if constexpr (M == 2) sc[e] = xa_pick(live[kb], e, sc[e], 0u);
             }
@@ -1096,6 +1097,7 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : DP == 64 ? 2
             for (int e = 0; e < 16; ++e) {
                 const int dd = wave * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
                 v[e] = (ob[dd * 32 + n] + ob[(DP + dd) * 32 + n]) + (ob[(2 * DP + dd) * 32 + n] + ob[(3 * DP + dd) * 32 + n]);
+                if (!(kbits >> n & 1)) v[e] = 0.f;   // (a dead key, whatever the rows hold)
             }
 #pragma unroll
             for (int a = 0; a < 4; ++a) {

@@ -168,6 +168,34 @@ def test_cross_attention_of_few_queries_over_many_ranges(B, Lq, Hk, G, D, dtype)
     _check_xa(q, k, v, g, mask=mask)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Lq,Lk", [(1, 20), (40, 20), (1, 50), (40, 50), (40, 130), (1, 5000)])
+def test_cross_attention_of_a_query_that_is_not_a_number(Lq, Lk, dtype):
+    """Its own rows and every live state's gradients are not numbers either; other images and rows are as they were, and a state that a length or a
+    mask of all queries takes out has no gradient (one that a query's own mask takes out weighs 0, and 0 times that query is not a number)."""
+    from layout2img_amd import ops
+    q, k, v, g = _xa(2, Lq, Lk, 1, 1, 40, dtype, 23)
+    bad = q.clone()
+    bad[0, Lq // 2, 0, 3] = math.nan
+    n = torch.tensor([Lk - 3, Lk], dtype=torch.int32, device=DEV)
+    shared = (torch.arange(Lk, device=DEV) % 4 > 0)[None, None]
+    for mask in (None, shared, shared.expand(1, Lq, Lk).contiguous()):
+        runs = []
+        for t in (q, bad):
+            leaves = [a.detach().requires_grad_() for a in (t, k, v)]
+            y = ops.cross_attention(*leaves, lengths=n, mask=mask)
+            runs.append([y, *torch.autograd.grad(y, leaves, g)])
+        live = torch.arange(Lk, device=DEV) < Lk - 3
+        if mask is not None:
+            live = live & mask[0, 0]
+        for a, b in zip(runs[0][:2], runs[1][:2]):
+            assert b[0, Lq // 2].isnan().all() and torch.equal(b[1], a[1]) and torch.equal(b[0, :Lq // 2].isnan(), a[0, :Lq // 2].isnan())
+            assert b[0, Lq // 2 + 1:].isfinite().all()
+        gone = ~live if mask is None or mask.shape[1] < Lq or Lq == 1 else torch.arange(Lk, device=DEV) >= Lk - 3
+        for a, b in zip(runs[0][2:], runs[1][2:]):
+            assert b[0, live].isnan().all() and not b[0, gone].any() and torch.equal(b[1], a[1])
+
+
 def test_cross_attention_with_scores_of_any_size():
     q, k, v, g = _xa(1, 50, 90, 1, 1, 64, F32, 6)
     _check_xa(q * 30, k, v, g, scale=0.5)                    # probabilities of one and zero
