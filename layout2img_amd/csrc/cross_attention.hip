@@ -591,8 +591,9 @@ __global__ __launch_bounds__(256) void xa_join_kernel(XaArgs p) {
 // ------------------------------------------------------------------------------------------------ backward: dq (and D)
 // Four waves x 32 rows, tiles of 64 keys, as the forward; also leaves D for the kernel behind it. 4096 queries over up to 512 states of 8 x 64, 16 images, bf16:
 // 135 us (570 TFLOP/s), of which reading q, g, out and what rounding left of it and writing dq (335 MB) takes 94 by itself.
+// In f32 up to 64 values a head fit two waves a SIMD (4096 queries over 200 states of 4 x 64, 16 images: 290 us at one, 235 at two).
 template <typename T, int DP>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void xa_dq_kernel(XaArgs p, int nqt, int total) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2) void xa_dq_kernel(XaArgs p, int nqt, int total) {
     constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, KT = 64, BYTES = KT * CH * 16;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int id = xa_tile_id(total);
@@ -705,7 +706,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void xa_dq_kernel(XaAr
 // 16 images of 4096 queries, up to 512 states of 8 x 64, bf16: 155 us (660 TFLOP/s); a workgroup's chain of products and exponentials takes 1.9 us a tile where
 // it is alone on its CU, two share 2.5. Three waves a SIMD do not fit the registers, and 64-row blocks side by side came out the same.
 template <typename T, int DP, int WK>
-__global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xa_dkv_kernel(XaArgs p, int nkt, int total) {
+__global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : 2) void xa_dkv_kernel(XaArgs p, int nkt, int total) {
     constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, RT = 64, BYTES = RT * CH * 16, KEYS = 32 * WK, ROWS = RT * WK / 4;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* rowv = reinterpret_cast<float*>(smem + 4 * BYTES);   // two of: [RT] lse, [RT] -D, [RT] query of the row
