@@ -589,22 +589,23 @@ __global__ __launch_bounds__(256) void xa_join_kernel(XaArgs p) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq (and D)
-// Four waves x 32 rows, tiles of 64 keys, as the forward; also leaves D for the kernel behind it. 4096 queries over up to 512 states of 8 x 64, 16 images, bf16:
+// Four waves x 32 rows, tiles of 64 keys, as the forward, in ns ranges joined by xa_fold_dq_kernel; also leaves D for the kernel behind it. 4096 queries over up to 512 states of 8 x 64, 16 images, bf16:
 // 135 us (570 TFLOP/s), of which reading q, g, out and what rounding left of it and writing dq (335 MB) takes 94 by itself.
 // In f32 up to 64 values a head fit two waves a SIMD (4096 queries over 200 states of 4 x 64, 16 images: 290 us at one, 235 at two).
 template <typename T, int DP>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2) void xa_dq_kernel(XaArgs p, int nqt, int total) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2) void xa_dq_kernel(XaArgs p, int nqt, int ns, int total) {
     constexpr int CH = DP * (int)sizeof(T) / 16, ND = DP / 32, S = CH / 2, KT = 64, BYTES = KT * CH * 16;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int id = xa_tile_id(total);
     if (id >= total) return;
-    const int j = id / nqt, qt = id - j * nqt, hk = j / p.B, b = j - hk * p.B, bh = b * p.Hk + hk;
+    const int j = id / (nqt * ns), rest = id - j * nqt * ns, split = rest / nqt, qt = rest - split * nqt;
+    const int hk = j / p.B, b = j - hk * p.B, bh = b * p.Hk + hk;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     const int r = qt * 128 + wave * 32 + (lane & 31);
     const bool on = r < p.R;
     const int iq = on ? xa_row_query(p, r) : 0, head = hk * p.G + (on ? r - iq * p.G : 0);
     const XaStates<T> st(p, b, hk);
-    const int nt = p.dq ? (st.len + KT - 1) / KT : 0;
+    const int nt = p.dq ? (st.len + KT - 1) / KT : 0, per = (nt + ns - 1) / ns, t0 = split * per, t1 = min(nt, t0 + per);
     const size_t orow = (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D;
     const unsigned char* mrow = st.mb && !st.kmask ? st.mb + (long long)iq * p.mq : nullptr;
     const unsigned lds = lds_addr_of(smem);
@@ -623,7 +624,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2) void xa_d
             dv.issue(vp, at + BYTES);
         }
     };
-    if (nt) issue(0, 0);
+    if (t0 < t1) issue(t0, 0);
     uint4 qf[S], gf[S];
     xa_row_frag<T, CH>(qf, on ? reinterpret_cast<const T*>(p.q) + b * p.qb + (long long)iq * p.ql + head * p.qh : nullptr, p.D, p.scale < 0.f);
     xa_row_frag<T, CH>(gf, on ? reinterpret_cast<const T*>(p.g) + orow : nullptr, p.D);
@@ -642,7 +643,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2) void xa_d
     }
     const float ls = on ? p.lse[(size_t)bh * p.R + r] : INFINITY;
     if (ls == INFINITY) dl = 0.f;   // (a row that sees nothing)
-    if (on && h == 0) p.delta[(size_t)bh * p.R + r] = dl;
+    if (on && h == 0 && split == 0) p.delta[(size_t)bh * p.R + r] = dl;
     XaAddr<T, CH> ad;
     f32x16_t acc[ND];
     xa_zero(acc);
@@ -669,11 +670,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2) void xa_d
     auto turn = [&](int t, int buf) {
         xa_wait_dma<0>();
         __syncthreads();
-        if (t + 1 < nt) issue(t + 1, buf ^ 1);
+        if (t + 1 < t1) issue(t + 1, buf ^ 1);
     };
     const unsigned none[2] = {};
-    const int tf = st.mb ? 0 : min(nt, st.len / KT);
-    int t = 0;
+    const int tf = st.mb ? t0 : min(t1, st.len / KT);
+    int t = t0;
     for (; t + 1 < tf; t += 2) {
         turn(t, 0);
         work(std::integral_constant<int, 0>(), smem, none);
@@ -682,11 +683,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2) void xa_d
     }
     int buf = 0;
     if (!st.mb || st.kmask)
-        for (; t < nt; ++t, buf ^= 1) {
+        for (; t < t1; ++t, buf ^= 1) {
             turn(t, buf);
             work(std::integral_constant<int, 1>(), smem + buf * 2 * BYTES, none);
         }
-    for (; t < nt; ++t, buf ^= 1) {
+    for (; t < t1; ++t, buf ^= 1) {
         const unsigned long long kbits = __ballot(st.live(t * KT + lane));
         unsigned live[2];
 #pragma unroll
@@ -696,8 +697,29 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2) void xa_d
     }
     xa_settle();
     if (!on || !p.dq) return;
+    if (ns > 1) {
+        float* part = p.part + (((size_t)split * p.B * p.Hk + bh) * p.R + r) * p.D;
 #pragma unroll
-    for (int d = 0; d < ND; ++d) xa_put<T>(reinterpret_cast<T*>(p.dq) + orow, acc[d], p.scale, d * 32, p.D);
+        for (int d = 0; d < ND; ++d) xa_put<float>(part, acc[d], p.scale, d * 32, p.D);
+    } else {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) xa_put<T>(reinterpret_cast<T*>(p.dq) + orow, acc[d], p.scale, d * 32, p.D);
+    }
+}
+// dq of rows whose states were cut in ns ranges: the ranges' shares, in range order
+template <typename T>
+__global__ __launch_bounds__(256) void xa_fold_dq_kernel(XaArgs p, int ns) {
+    const long long n = (long long)p.B * p.Hk * p.R * p.D, i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int k = 0; k < ns; ++k) {
+        const float4 a = *reinterpret_cast<const float4*>(p.part + (size_t)k * n + i);
+        s[0] += a.x; s[1] += a.y; s[2] += a.z; s[3] += a.w;
+    }
+    const long long row = i / p.D;
+    const int d = (int)(i - row * p.D), bh = (int)(row / p.R), r = (int)(row - (long long)bh * p.R), b = bh / p.Hk, hk = bh - b * p.Hk, iq = xa_row_query(p, r);
+    Op4<T>::store(reinterpret_cast<T*>(p.dq) + (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + hk * p.G + r - iq * p.G) * p.D + d, s);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
@@ -1117,8 +1139,9 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : DP == 64 ? 2
 }
 
 // ------------------------------------------------------------------------------------------------ entry points
-#define XA_WGS 512   // workgroups that fill the chip: 256 CUs, two each. Kernels of one workgroup a CU (the forward's few rows) take half of it: 32768
-                     // states of 128 x 8 heads, one query: 33 us at 512, 31 at 256; 32 images of 4096 x 8 x 64: 50 and 46
+#define XA_WGS 512   // workgroups that fill the chip: 256 CUs, two each. Kernels of one workgroup a CU (few rows forward; wide heads, as the registers of each
+                     // kernel allow) take half of it: 32768 states of 128 x 8 heads, one query: 33 us at 512, 31 at 256; 32 images of 4096 x 8 x 64: 50 and 46;
+                     // 1024 queries over 1024 states of 8 x 128, 4 images, f32, with the gradients: 834 and 758
 static int xa_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 // ranges of the states (forward) or rows (backward) for `tiles` workgroups over `nt` tiles of them: `wgs` workgroups, at least two tiles each
 static int xa_splits(long long tiles, long long nt, int wgs) {
@@ -1128,19 +1151,21 @@ static int xa_splits(long long tiles, long long nt, int wgs) {
     if (ns > XA_MAX_SPLITS) ns = XA_MAX_SPLITS;
     return ns < 1 ? 1 : (int)ns;
 }
-struct XaPlan { int wq, nqt, ns, wk, nkt, nsb, nwf, nwb; };   // nwf, nwb: workgroups an (image, state head) of the one-tile form has, 0: not that form
+struct XaPlan { int wq, nqt, ns, wk, nkt, nsb, nsq, nwf, nwb; };   // nwf, nwb: workgroups an (image, state head) of the one-tile form has, 0: not that form
 static bool xa_short_fits(int dp, int dtype) {
     return dtype ? (dp == 32 ? XaShort<bf16_t, 32>::OK : dp == 64 ? XaShort<bf16_t, 64>::OK : XaShort<bf16_t, 128>::OK)
                  : (dp == 32 ? XaShort<float, 32>::OK : dp == 64 ? XaShort<float, 64>::OK : XaShort<float, 128>::OK);
 }
 static XaPlan xa_plan(int B, long long R, int Lk, int Hk, int D, int dtype) {
     XaPlan q;
+    const int dp = xa_dp(D);
+    const bool f32 = !dtype;
     const long long bh = (long long)B * Hk, groups = (R + 127) / 128;   // a workgroup's four waves take at least a block of 32 rows each
     q.nwf = q.nwb = 0;
     // the one-tile form, forward and forward with backward, against the general one: 32 images of 4096 queries over 31 states of 4 x 32 bf16 17 and 47 us, not 25
     // and 104; of 4 x 64 f32 75 and 242, not 109 and 548; one query of 8 x 64 bf16 5 and 12, not 7 and 17. Workgroups: 1024 and 512 in all (2048 and 1024: 18 and 51,
     // 4096 each: 23 and 73): staging the states and joining the shares of dk and dv are paid less often
-    if (Lk <= 32 && xa_short_fits(xa_dp(D), dtype)) {
+    if (Lk <= 32 && xa_short_fits(dp, dtype)) {
         q.nwf = (int)std::min(groups, std::max(1LL, (1024 + bh - 1) / bh));
         q.nwb = (int)std::min(groups, std::max(1LL, (512 + bh - 1) / bh));
     }
@@ -1149,12 +1174,15 @@ static XaPlan xa_plan(int B, long long R, int Lk, int Hk, int D, int dtype) {
     q.wq = R <= 32 ? 1 : 4;
     q.nqt = (int)((R + 32 * q.wq - 1) / (32 * q.wq));
     const int kt = q.wq == 4 ? 64 : 128;   // keys a workgroup takes at a time
-    q.ns = xa_splits((long long)B * Hk * q.nqt, (Lk + kt - 1) / kt, q.wq == 4 ? XA_WGS : XA_WGS / 2);
+    q.ns = xa_splits((long long)B * Hk * q.nqt, (Lk + kt - 1) / kt, q.wq == 4 && !(f32 && dp == 128) ? XA_WGS : XA_WGS / 2);
     // 64 keys a workgroup where 128 would leave waves or CUs without any (f32, 64 states of 64 x 4 heads x 16 images: 278 -> 218 us for dq, dk, dv;
     // 77 states of 40 x 2 x 8, f32: 22 -> 16 us for dk, dv), else 128, which stage the rows half as often (2048 states, bf16: 510 us, not 560)
     q.wk = Lk <= 64 || (Lk <= 128 && bh * ((Lk + 127) / 128) < 256) ? 2 : 4;
     q.nkt = (Lk + 32 * q.wk - 1) / (32 * q.wk);
-    q.nsb = q.nwb ? q.nwb : xa_splits((long long)B * Hk * q.nkt, (R + 63) / 64, XA_WGS);
+    q.nsb = q.nwb ? q.nwb : xa_splits((long long)B * Hk * q.nkt, (R + 63) / 64, dp == 128 || (f32 && dp == 64) ? XA_WGS / 2 : XA_WGS);
+    // (few rows over many states, f32 with the gradients: 300 queries of 4 x 128 over 2000 states of 2 x 128 526 us unsplit, 140 split; 1000 of 8 x 128 over
+    // 2000 of 4 x 128 718 and 389)
+    q.nsq = q.nwb ? 1 : xa_splits(bh * groups, (Lk + 63) / 64, f32 && dp == 128 ? XA_WGS / 2 : XA_WGS);
     if (q.nwf) q.ns = 1;
     return q;
 }
@@ -1168,7 +1196,8 @@ extern "C" int l2i_cross_attention_scratch(int B, int Lq, int Lk, int Hk, int G,
     if (!floats || xa_bad(B, Lq, Lk, Hk, G, D, dtype)) return L2I_ERR_ARG;
     const long long R = (long long)Lq * G;
     const XaPlan q = xa_plan(B, R, Lk, Hk, D, dtype);
-    if (bwd) *floats = ((long long)B * Hk * R + 3) / 4 * 4 + (q.nsb > 1 ? 2LL * q.nsb * B * Hk * Lk * D : 0);
+    // (dq's shares are folded before the first of dk's and dv's is written: one place for both)
+    if (bwd) *floats = ((long long)B * Hk * R + 3) / 4 * 4 + std::max(q.nsb > 1 ? 2LL * q.nsb * B * Hk * Lk * D : 0LL, q.nsq > 1 ? (long long)q.nsq * B * Hk * R * D : 0LL);
     else *floats = q.ns > 1 ? (long long)q.ns * B * Hk * R * (D + 2) : 0;
     return L2I_OK;
 }
@@ -1228,10 +1257,14 @@ static int xa_bwd_launch(const XaArgs& a, const XaPlan& q, hipStream_t s) {
         }
         return L2I_OK;
     }
-    const int nqt = (a.R + 127) / 128, tq = a.B * a.Hk * nqt, tk = a.B * a.Hk * q.nkt * a.ns;
+    const int nqt = (a.R + 127) / 128, nsq = a.dq ? q.nsq : 1, tq = a.B * a.Hk * nqt * nsq, tk = a.B * a.Hk * q.nkt * a.ns;
     const size_t lq = (size_t)4 * 64 * DP * sizeof(T), lk = lq + 6 * 64 * sizeof(float);
     if (int e = xa_lds(xa_dq_kernel<T, DP>, lq)) return e;
-    hipLaunchKernelGGL((xa_dq_kernel<T, DP>), dim3(xa_grid(tq)), dim3(256), lq, s, a, nqt, tq);
+    hipLaunchKernelGGL((xa_dq_kernel<T, DP>), dim3(xa_grid(tq)), dim3(256), lq, s, a, nqt, nsq, tq);
+    if (nsq > 1) {
+        const long long n = (long long)a.B * a.Hk * a.R * a.D;
+        hipLaunchKernelGGL((xa_fold_dq_kernel<T>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, a, nsq);
+    }
     if (!a.dk || a.Lk == 0) return L2I_OK;
     if (q.wk == 4) {
         if (int e = xa_lds(xa_dkv_kernel<T, DP, 4>, lk)) return e;
