@@ -17,7 +17,7 @@
 // What bounds it: with 64 values a head, a wave's 32 x 64 scores cost 16 MFMAs (512 cycles) and 32 exponentials a lane with what surrounds
 // them (about 900 cycles), so the vector unit; tiles therefore come to LDS by LDS-DMA (no registers, no instructions of the waves), two
 // buffers deep, and the rescaling of the accumulators waits until the maximum has grown by 2^8. Measured in bf16: 4096 queries of 16 x 128 over 2048 states
-// of 4 x 128, four images, 261 us (1050 TFLOP/s); 4096 queries over up to 512 states of 8 x 64, 16 images, 97 us (530 TFLOP/s; 42 of them for q, out and
+// of 4 x 128, four images, 261 to 281 us from card to card (980 to 1050 TFLOP/s); 4096 queries over up to 512 states of 8 x 64, 16 images, 97 us (530 TFLOP/s; 42 of them for q, out and
 // what rounding left of it). One query of 16 x 128 over up to 4096 states of 4 x 128, 32 images: 35 us (5.8 TB/s) and 4 for the join.
 #include "igemm.h"
 #include <algorithm>
