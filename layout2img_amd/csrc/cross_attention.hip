@@ -1145,7 +1145,7 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 1 : DP == 64 ? 2
 static int xa_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 // ranges of the states (forward) or rows (backward) for `tiles` workgroups over `nt` tiles of them: `wgs` workgroups, at least two tiles each
 static int xa_splits(long long tiles, long long nt, int wgs) {
-    if (tiles >= wgs || nt < 2) return 1;
+    if (tiles < 1 || tiles >= wgs || nt < 2) return 1;   // (no tiles: a list without states)
     long long ns = (wgs + tiles - 1) / tiles;
     if (ns > nt / 2) ns = nt / 2;
     if (ns > XA_MAX_SPLITS) ns = XA_MAX_SPLITS;
