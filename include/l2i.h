@@ -498,7 +498,8 @@ int l2i_group_norm_bwd(const void* x, int x_dtype, const float* gamma, const flo
  * have to be finite. A query without a live key gives zeros (and no gradient).
  * out [B][Lq][Hk G][D] contiguous; lse [B][Hk][Lq G] (optional in fwd) is kept for bwd, as is out_lo (bf16 only, optional, out's layout: what the
  * rounding of out left; worth its bytes where l2i_cross_attention_wants_lo says 1).
- * bwd: out, dout, dq [B][Lq][Hk G][D] and dk, dv [B][Lk][Hk][D] contiguous and 16-byte aligned; dq, and dk with dv, optional. */
+ * bwd: out, dout, dq [B][Lq][Hk G][D] and dk, dv [B][Lk][Hk][D] contiguous and 16-byte aligned; dq, and dk with dv, optional. A tile of dout spans
+ * less than 2^31 bytes: min(Lq - 1, 1 + 62 / G) Hk G D + G D values. */
 int l2i_cross_attention_scratch(int B, int Lq, int Lk, int Hk, int G, int D, int dtype, int bwd, long long* floats);
 int l2i_cross_attention_wants_lo(int B, int Lq, int Lk, int Hk, int G, int D, int dtype);   /* 1 or 0 */
 int l2i_cross_attention_fwd(const void* q, const void* k, const void* v, int dtype, const int* lengths, const unsigned char* mask, void* out,

@@ -1283,6 +1283,11 @@ static bool xa_rows_ok(const void* t, long long sb, long long sl, long long sh, 
     if (((size_t)t & 15) || sb % e || sl % e || sh % e || sb < 0 || sl < 0 || sh < 0) return false;
     return sl < most / 512 && sh < most && 65 * sl * (16 / e) + heads * sh * (16 / e) + 1024 < most;
 }
+// the same for dout, which is contiguous: a tile's 64 rows lie in its first query and at most 1 + 62 / G further ones, Hk G D values apart
+static bool xa_dout_ok(int Lq, int Hk, int G, int D, int dtype) {
+    const long long steps = std::min(Lq - 1, 1 + 62 / G), values = steps * Hk * G * D + (long long)G * D;
+    return values * (dtype ? 2 : 4) < 1LL << 31;
+}
 static void xa_setup(XaArgs& a, const void* q, const void* k, const void* v, const int* lengths, const unsigned char* mask, int B, int Lq, int Lk, int Hk,
                      int G, int D, long long qb, long long ql, long long qh, long long kb, long long kl, long long kh, long long vb, long long vl, long long vh,
                      long long mb, long long mq, float scale) {
@@ -1319,7 +1324,7 @@ extern "C" int l2i_cross_attention_bwd(const void* q, const void* k, const void*
     long long need = 0;
     if (xa_bad(B, Lq, Lk, Hk, G, D, dtype) || !q || !out || !lse || !dout || (Lk && (!k || !v)) || mb < 0 || mq < 0) return L2I_ERR_ARG;
     if ((dk == nullptr) != (dv == nullptr) || (out_lo && !dtype) || (((size_t)out | (size_t)out_lo | (size_t)dout | (size_t)dq | (size_t)dk | (size_t)dv) & 15)) return L2I_ERR_ARG;
-    if (!xa_rows_ok(q, qb, ql, qh, G, dtype) || !xa_rows_ok(k, kb, kl, kh, 0, dtype) || !xa_rows_ok(v, vb, vl, vh, 0, dtype)) return L2I_ERR_ARG;
+    if (!xa_rows_ok(q, qb, ql, qh, G, dtype) || !xa_rows_ok(k, kb, kl, kh, 0, dtype) || !xa_rows_ok(v, vb, vl, vh, 0, dtype) || !xa_dout_ok(Lq, Hk, G, D, dtype)) return L2I_ERR_ARG;
     if (l2i_cross_attention_scratch(B, Lq, Lk, Hk, G, D, dtype, 1, &need) != L2I_OK || !scratch || ((size_t)scratch & 15) || scratch_floats < need) return L2I_ERR_ARG;
     XaArgs a = {};
     xa_setup(a, q, k, v, lengths, mask, B, Lq, Lk, Hk, G, D, qb, ql, qh, kb, kl, kh, vb, vl, vh, mb, mq, scale);

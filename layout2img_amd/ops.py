@@ -2185,6 +2185,13 @@ def _xa_args(q, k, v, sq, sk, sv, mask, sm, bf16):
 
 
 @functools.lru_cache(maxsize=4096)
+def _xa_backward_reaches(Lq, Hk, G, D, size):
+    """Whether the backward pass reads a tile of 64 rows of the result's gradient (contiguous, values of `size` bytes): the rows lie in their first query
+    and at most 1 + 62 // G further ones, and span less than 2^31 bytes."""
+    return (min(Lq - 1, 1 + 62 // G) * Hk * G * D + G * D) * size < 1 << 31
+
+
+@functools.lru_cache(maxsize=4096)
 def _wants_lo(*sizes):
     _lib.load()
     return bool(_lib._FN["l2i_cross_attention_wants_lo"](*sizes, _lib.BF16))   # (an answer, not a status)
@@ -2243,7 +2250,8 @@ def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
     lengths: (B,) int32, states at and behind a sequence's length do not exist. mask: (B | 1, Lq | 1, Lk) bool, False = query i does not see state j.
     A query that sees no state gives zeros. What `lengths` or a mask row shared by all queries takes out is not read, whatever it holds; a state
     that only some queries see has to be finite. The D values of a head are consecutive; the other strides may be any of whole 16 bytes (slices of
-    a grouped projection, transposed heads, expanded batches), less than 2^22 values from position to position."""
+    a grouped projection, transposed heads, expanded batches), less than 2^22 values from position to position. Where a gradient is wanted, the
+    result's queries lie less than 2^31 bytes apart over min(Lq - 1, 1 + 62 // (H // Hk)) steps of H * D values, and one group of heads beside them."""
     dtype = _op(q, "cross_attention: q").dtype
     if _op(k, "cross_attention: k").dtype is not dtype or _op(v, "cross_attention: v").dtype is not dtype:
         raise RuntimeError(f"cross_attention: q, k, v have one type, got {dtype}, {k.dtype} and {v.dtype}")
@@ -2256,8 +2264,11 @@ def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
     if lengths is not None and (_op(lengths, "cross_attention: lengths", torch.int32).shape != (args[0],) or not lengths.is_contiguous()):
         raise RuntimeError(f"cross_attention: lengths is a contiguous ({args[0]},) tensor, got {tuple(lengths.shape)}, strides {lengths.stride()}")
     scale = 1.0 / math.sqrt(args[5]) if scale is None else float(scale)
+    grad = _wants_grad(q, k, v)
+    if grad and not _xa_backward_reaches(args[1], *args[3:6], q.element_size()):
+        raise RuntimeError(f"cross_attention: the gradient of a result of {tuple(q.shape)} has queries further apart than its backward pass reads (2^31 bytes over a tile)")
     _same_device(q, k, v, lengths, mask)
-    if _wants_grad(q, k, v):
+    if grad:
         return CrossAttentionFn.apply(q, k, v, lengths, mask, scale, args)
     return _cross_attention_fwd(q, k, v, lengths, mask, scale, args, False)[0]
 

@@ -2,6 +2,7 @@
 import ctypes
 
 import pytest
+import torch
 
 
 def _lib():
@@ -19,3 +20,39 @@ def test_cross_attention_plans_a_list_without_states(D, dtype):
             assert _lib().l2i_cross_attention_scratch(B, Lq, 0, Hk, G, D, dtype, bwd, n) == 0, (B, Lq, Hk, G, bwd)
             assert n[0] == (B * Hk * Lq * G + 3) // 4 * 4 * bwd   # (the rows' D alone: nothing is cut in ranges)
         assert _lib().l2i_cross_attention_wants_lo(B, Lq, 0, Hk, G, D, dtype) in (0, 1)
+
+
+P = 1 << 20   # an address that is never read: every call below is refused before a launch
+
+
+def _backward(Lq, Hk, G, D, dtype):
+    st = (0, D, 0) * 3   # heads in front of positions: the checks of q, k and v pass whatever the number of heads
+    return _lib().l2i_cross_attention_bwd(P, P, P, dtype, None, None, P, None, P, P, P, P, P, 1, Lq, 64, Hk, G, D, *st, 0, 0, 1.0, P, 1 << 50, None)
+
+
+def _span(Lq, Hk, G, D):
+    """values between the first and the last of any 64 rows of a contiguous (Lq, Hk G, D) gradient that belong to one state head"""
+    at = lambda r: (r // G) * Hk * G * D + (r % G) * D
+    R = Lq * G
+    return max(at(min(R - 1, r + 63)) - (r // G) * Hk * G * D + D for r in range(min(R, 64 * G)))
+
+
+def test_cross_attention_refuses_a_gradient_whose_tiles_pass_32_bits():
+    """q and k with heads in front of positions step by D, but the gradient of the result, which is contiguous, by all heads: offsets that are counted in
+    32 bits would come round."""
+    from layout2img_amd import ops
+    for Lq, Hk, G, D, dtype in ((64, 1 << 21, 1, 8, 0), (64, 1 << 18, 1, 128, 1), (2, 1 << 23, 4, 128, 1), (33, 1 << 17, 2, 128, 0), (2, 1 << 22, 1, 128, 0)):
+        assert not ops._xa_backward_reaches(Lq, Hk, G, D, 2 if dtype else 4)
+        assert _backward(Lq, Hk, G, D, dtype) == -1, (Lq, Hk, G, D, dtype)
+    z = torch.zeros(1, 1, 1, 8)
+    q, k = z.expand(1, 64, 1 << 21, 8), z.expand(1, 64, 1 << 21, 8)
+    with pytest.raises(RuntimeError, match="further apart"):
+        ops.cross_attention(q.detach().requires_grad_(), k, k)
+    with pytest.raises(RuntimeError, match="GPU"):   # (the forward pass alone does not read it)
+        ops.cross_attention(q, k, k)
+    for G in (1, 2, 3, 5, 31, 32, 62, 63, 64, 65, 100):
+        for Lq in (1, 2, 3, 40, 64, 65, 200):
+            for Hk in (1, 7, 1 << 15, 1 << 18, 1 << 20):
+                for size in (2, 4):
+                    if ops._xa_backward_reaches(Lq, Hk, G, 128, size):
+                        assert _span(Lq, Hk, G, 128) * size < 1 << 31, (G, Lq, Hk, size)
