@@ -10,7 +10,7 @@ import functools
 import math
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -2074,6 +2074,12 @@ def _scratch(device, name, *sizes):
 
 
 def _wants_grad(*ts):
+    """Whether a call goes through its autograd function: where a gradient is wanted, and inside a level of forward-mode differentiation, where that function
+    refuses tensors with a tangent (a launch past it would drop the tangent). A trace would record the result's allocation, not the launch."""
+    if torch.jit.is_tracing():
+        raise RuntimeError("operators that launch the library's kernels cannot be traced")
+    if forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:

@@ -56,3 +56,40 @@ def test_cross_attention_refuses_a_gradient_whose_tiles_pass_32_bits():
                 for size in (2, 4):
                     if ops._xa_backward_reaches(Lq, Hk, G, 128, size):
                         assert _span(Lq, Hk, G, 128) * size < 1 << 31, (G, Lq, Hk, size)
+
+
+def _calls(monkeypatch):
+    """The operators as calls of one tensor that carries a derivative, with the launches themselves taken out: what the host layer does around them."""
+    from layout2img_amd import ops
+    monkeypatch.setattr(ops._lib, "call", lambda *a: 0)
+    monkeypatch.setattr(ops, "_same_device", lambda *a: None)
+    monkeypatch.setattr(ops, "_scratch_floats", lambda *a: 16)
+    monkeypatch.setattr(ops, "_stream", lambda: None)
+    q, kv, x, w = torch.randn(1, 2, 2, 16), torch.randn(1, 3, 2, 16), torch.randn(2, 3, 3, 8), torch.randn(8)
+    rng, tok = torch.zeros(2, dtype=torch.int64), torch.zeros(3, dtype=torch.int64)
+    return [(x, lambda t: ops.group_norm_act(t, 2)), (w, lambda t: ops.group_norm_act(x, 2, t)), (w, lambda t: ops.group_norm_act(x, 2, None, t)),
+            (q, lambda t: ops.cross_attention(t, kv, kv)), (kv, lambda t: ops.cross_attention(q, t, kv)), (kv, lambda t: ops.cross_attention(q, kv, t)),
+            (torch.randn(4, 8), lambda t: ops.embedding(t, tok)), (x, lambda t: ops.dropout(t, 0.5, rng)), (x, lambda t: ops.dropout(x, 0.5, rng, residual=t))]
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_derivatives_are_refused_not_dropped(monkeypatch, grad_mode):
+    fa = torch.autograd.forward_ad
+    for i, (t, f) in enumerate(_calls(monkeypatch)):
+        with torch.set_grad_enabled(grad_mode):
+            with fa.dual_level():
+                with pytest.raises(NotImplementedError, match="jvp"):
+                    f(fa.make_dual(t, torch.ones_like(t)))
+                assert f(t).shape is not None, i                  # (without a tangent the call is an ordinary one)
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                torch.func.jvp(f, (t,), (torch.ones_like(t),))
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                torch.func.vmap(f)(t[None])
+            assert f(t).shape is not None, i
+
+
+def test_a_trace_is_refused(monkeypatch):
+    for t, f in _calls(monkeypatch):
+        for grad in (False, True):
+            with pytest.raises(RuntimeError, match="traced"):
+                torch.jit.trace(f, (t.detach().requires_grad_(grad),), check_trace=False)
