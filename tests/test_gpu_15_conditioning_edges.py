@@ -1,5 +1,7 @@
 """GPU: calls at which the attention-conditioning operators can go wrong: lists without states, numbers that are not finite, means and single values
 far from the rest."""
+import math
+
 import pytest
 import torch
 
@@ -34,3 +36,35 @@ def test_cross_attention_to_a_list_without_states(Lq, D, dtype):
         assert not dq.any() and dk.shape == dv.shape == k.shape
         with torch.no_grad():
             assert not ops.cross_attention(q, k, v, **kw).any()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Lq,Lk,D", [(1, 20, 40), (40, 20, 40), (40, 20, 128), (1, 50, 40), (40, 50, 40), (40, 130, 128), (200, 130, 64), (1, 5000, 40), (300, 2000, 128)])
+def test_cross_attention_of_a_state_that_is_not_finite(Lq, Lk, D, dtype, bad):
+    """A key that is not a number makes the weights of every state of its image so: out, dq and the live states' dk and dv; the other image keeps its bits, and
+    states behind a length have no gradient. An infinite key does the same where it scores +inf."""
+    from layout2img_amd import ops
+    gen = _gen(Lq + Lk)
+    q, k, v, g = (_rnd(gen, 2, n, 1, D, dtype=dtype) for n in (Lq, Lk, Lk, Lq))
+    q[..., 3] = q[..., 3].abs() + 1                          # (an infinite key scores +inf)
+    n = torch.tensor([Lk - 3, Lk], dtype=torch.int32, device=DEV)
+    shared = (torch.arange(Lk, device=DEV) % 4 > 0)[None, None]
+    for mask in (None, shared, shared.expand(1, Lq, Lk).contiguous()):
+        runs = []
+        for broken in (False, True):
+            kk = k.clone()
+            if broken:
+                kk[0, Lk // 2 + (Lk // 2) % 2 + 1, 0, 3] = bad   # (live under the masks too: an odd state)
+            leaves = [a.detach().requires_grad_() for a in (q, kk, v)]
+            y = ops.cross_attention(*leaves, lengths=n, mask=mask)
+            runs.append([y.detach(), *torch.autograd.grad(y, leaves, g)])
+        live = torch.arange(Lk, device=DEV) < Lk - 3
+        if mask is not None:
+            live = live & mask[0, 0]
+        for clean, got, what in zip(runs[0], runs[1], ("out", "dq", "dk", "dv")):
+            assert torch.equal(got[1], clean[1]), what
+            if what in ("out", "dq"):
+                assert got[0].isnan().all(), what
+            else:
+                assert got[0, live].isnan().all() and not got[0, Lk - 3:].any(), what
