@@ -34,13 +34,14 @@ struct GnArgs {
 // silu: s = 1 / (1 + 2^(-z log2 e)) by the hardware's exp2 and reciprocal (relative 2^-21), silu' = s + z (s - s^2).
 #define GN_LOG2E 1.44269504088896340736f
 __device__ __forceinline__ float gn_sig(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -GN_LOG2E)); }
+// A z that is not a number stays one in every activation (not fmaxf: a group with such a value is not a number as a whole and must not come out as zeros).
 template <int ACT> __device__ __forceinline__ float gn_act(float z) {
-    if (ACT == 1) return fmaxf(z, 0.f);
+    if (ACT == 1) return z < 0.f ? 0.f : z;
     if (ACT == 2) return z * gn_sig(z);
     return z;
 }
 template <int ACT> __device__ __forceinline__ float gn_dact(float z, float dy) {
-    if (ACT == 1) return z > 0.f ? dy : 0.f;
+    if (ACT == 1) return z <= 0.f ? 0.f : dy;
     if (ACT == 2) { const float s = gn_sig(z); return dy * fmaf(z, fmaf(-s, s, s), s); }
     return dy;
 }
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs p) {
             }
             for (int o = 1; o < L; o <<= 1) { s += __shfl_xor(s, o, 64); q += __shfl_xor(q, o, 64); }
             if (g < p.G && gl == 0) {
-                const float dm = s / N, m = m0 + dm, rs = 1.f / sqrtf(fmaxf(q - s * dm, 0.f) / N + p.eps);
+                const float dm = s / N, m = m0 + dm, m2 = q - s * dm, rs = 1.f / sqrtf((m2 < 0.f ? 0.f : m2) / N + p.eps);   // (a NaN stays one)
                 gm[g] = m; gr[g] = rs;
                 if (ch == 0) { p.mean[(size_t)b * p.G + g] = m; p.rstd[(size_t)b * p.G + g] = rs; }
             }

@@ -18,6 +18,34 @@ def _rnd(gen, *shape, dtype=F32, scale=1.0):
     return (torch.randn(*shape, generator=gen, device=DEV) * scale).to(dtype)
 
 
+# ------------------------------------------------------------------------------------------------ group norm
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("at", [(0, 0), (2, 3), (-1, -1)])
+@pytest.mark.parametrize("act", [None, "relu", "silu"])
+@pytest.mark.parametrize("B,hw,C,G,dtype", [(2, (4, 4), 1024, 32, F32), (3, (16, 16), 96, 3, BF16), (2, (40, 40), 24, 3, F32), (2, (33, 9), 25, 5, F32), (2, (64, 48), 64, 4, BF16)])
+def test_group_norm_of_a_value_that_is_not_finite(B, hw, C, G, dtype, act, at, bad):
+    """Its group of its image is not a number as a whole, whatever the activation; every other value is as it was. Both forms."""
+    from layout2img_amd import ops
+    gen = _gen(C + G)
+    x, w, b, dy = _rnd(gen, B, *hw, C, dtype=dtype), 1 + 0.2 * _rnd(gen, C), _rnd(gen, C), _rnd(gen, B, *hw, C, dtype=dtype)
+    g, cg = 1, C // G
+    broken = x.clone()
+    broken[1, at[0], at[1], g * cg + cg // 2] = bad
+    runs = []
+    for t in (x, broken):
+        leaves = [a.detach().requires_grad_() for a in (t, w, b)]
+        y = ops.group_norm_act(leaves[0], G, leaves[1], leaves[2], act=act)
+        runs.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
+    group = torch.zeros(B, *hw, C, dtype=torch.bool, device=DEV)
+    group[1, ..., g * cg:(g + 1) * cg] = True
+    channel = torch.zeros(C, dtype=torch.bool, device=DEV)
+    channel[g * cg:(g + 1) * cg] = True
+    for clean, got, where, what in zip(runs[0], runs[1], (group, group, channel), ("y", "dx", "dw")):
+        assert got[where].isnan().all(), what
+        assert torch.equal(got[~where], clean[~where]), what
+    assert torch.equal(runs[1][3][~channel], runs[0][3][~channel])
+
+
 # ------------------------------------------------------------------------------------------------ cross attention
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("D", [40, 64, 72, 128])
