@@ -9,8 +9,8 @@
 //   resident: a workgroup holds all pixels of a slab of whole groups (at least 64 contiguous bytes a pixel) in registers: one launch, every
 //     value read once; used where a slab is at most 4096 values (8192 in bf16: maps up to 16 x 16 of the wide layers).
 //   split: the map is cut in NCH chunks of rows (pixels) per image. The first launch leaves every chunk's moments (mean and sum of squared
-//     deviations per group: sums around a value of the chunk itself, so that a mean far from zero costs no digits), the second joins
-//     them in a fixed order and writes the result, reading the map a second time -- from the chunk that was read last backwards, on the
+//     deviations per group, counted from origins that follow the values: neither a mean far from zero nor single values far from the rest cost digits), the
+//     second joins them in a fixed order and writes the result, reading the map a second time -- from the chunk that was read last backwards, on the
 //     XCD that read it, so that L2 and the Infinity Cache still hold what is read first.
 // Measured, B = 32 with silu: 64 x 64 x 128 in bf16 (33.5 MB a map): moments 8.6 us, result 17 (4.0 TB/s), backward sums 19, dx 21 (4.8 TB/s);
 // 128 x 128 x 64 in f32 (134 MB): 25, 43 (6.3 TB/s), 51 (5.2), 66 (6.1) -- what a copy of that size reaches. One 4 x 4 x 1024 image, resident: 6 us.
@@ -67,61 +67,95 @@ template <int V, typename F> __device__ __forceinline__ void gn_each(int c, int 
     const int b = id / p.nch, ch = id - b * p.nch;                                                                   \
     const long long r0 = ch * p.rows, r1 = r0 + p.rows < p.HW ? r0 + p.rows : p.HW;                                   \
     const size_t img = (size_t)b * p.HW * p.C;
-// rows r0 + ty, + nr, ... of the chunk: LOAD(k, r) puts row r into slot k, four rows in flight, then USE(k, r)
-#define GN_ROWS(LOAD, USE)                                                                                           \
+// rows r0 + ty, + nr, ... of the chunk: LOAD(k, r) puts row r into slot k, four rows in flight, then USE(k, r); FOUR in front of every four
+#define GN_ROWS_4(LOAD, FOUR, USE)                                                                                    \
     do {                                                                                                             \
         long long r = r0 + ty;                                                                                       \
         for (; r + 3 * nr < r1; r += 4 * nr) {                                                                       \
             LOAD(0, r) LOAD(1, r + nr) LOAD(2, r + 2 * nr) LOAD(3, r + 3 * nr)                                       \
+            FOUR                                                                                                     \
             USE(0, r) USE(1, r + nr) USE(2, r + 2 * nr) USE(3, r + 3 * nr)                                           \
         }                                                                                                            \
         for (; r < r1; r += nr) { LOAD(0, r) USE(0, r) }                                                             \
     } while (0)
+#define GN_ROWS(LOAD, USE) GN_ROWS_4(LOAD, , USE)
+
+// Sums around an origin lose the digits of the deviations where the origin lies far from the mean: q - s^2 / n cancels. Every thread therefore moves its
+// origin k, at first its first row, to the mean of its rows so far at 4, 16, 64, ... of them. At the end q <= 7 (q - s^2 / N), whatever the values and their
+// order: behind the last of the n rows that k is the mean of come at most 6 n, and N (mean - k)^2 is at most (N - n) / n times the deviations that part them
+// from the first n. The moments of threads, channels and chunks are joined around one of their means, the squared deviations around the joint one.
+// 32 images of 64 x 64 x 128 bf16: 7.4 us, without moving 7.0.
+template <int V> __device__ __forceinline__ void gn_recentre(float n, float (&k)[V], float (&s)[V], float (&q)[V]) {
+    const float rn = __builtin_amdgcn_rcpf(n);   // (k need not be the mean exactly)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const float k1 = fmaf(s[e], rn, k[e]), d = k1 - k[e];   // (d: what k really moves by)
+        q[e] -= d * (2.f * s[e] - n * d);
+        s[e] -= n * d;
+        k[e] = k1;
+    }
+}
 
 template <typename T, int V>
 __global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs p) {
-    extern __shared__ __attribute__((aligned(16))) float sm[];   // [C] means, [C] squared deviations, [256][2 V] row lanes
+    extern __shared__ __attribute__((aligned(16))) float sm[];   // [C] means, [C] squared deviations, [V][2][256] row lanes
     float *cm = sm, *cq = sm + p.Cp, *red = cq + p.Cp;
     GN_COLS(V, false)
     const T* x = reinterpret_cast<const T*>(p.x) + img;
-    const float n = (float)(r1 - r0), rn = 1.f / n;
+    const int rows = (int)(r1 - r0);
+    const float n = (float)rows, rn = 1.f / n;
     for (int t0 = 0; t0 < cv; t0 += tw) {
         const int c = (t0 + tx) * V;
-        const bool on = ty < nr && t0 + tx < cv;
+        const bool on = ty < nr && ty < rows && t0 + tx < cv;
         float s[V], q[V], k[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) { s[e] = 0.f; q[e] = 0.f; k[e] = 0.f; }
         if (on) {
             Vec<T, V> a[4];
-            a[0].load(x + (size_t)r0 * p.C + c);
+            a[0].load(x + (size_t)(r0 + ty) * p.C + c);
             a[0].get(k);
+            int seen = 0, next = 4;
 #define GN_L(K, R) a[K].load(x + (size_t)(R) * p.C + c);
 #define GN_U(K, R) { float v[V]; a[K].get(v); _Pragma("unroll") for (int e = 0; e < V; ++e) { const float d = v[e] - k[e]; s[e] += d; q[e] = fmaf(d, d, q[e]); } }
-            GN_ROWS(GN_L, GN_U);
+#define GN_FOUR if (seen == next) { gn_recentre<V>((float)seen, k, s, q); next *= 4; } seen += 4;
+            GN_ROWS_4(GN_L, GN_FOUR, GN_U);
+#undef GN_FOUR
 #undef GN_U
+            const float rl = 1.f / (float)((rows - ty + nr - 1) / nr);
+#pragma unroll
+            for (int e = 0; e < V; ++e) { const float m = s[e] * rl; q[e] -= s[e] * m; k[e] += m; }
         }
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < V; ++e) { red[e * 512 + threadIdx.x] = s[e]; red[e * 512 + 256 + threadIdx.x] = q[e]; }
+        for (int e = 0; e < V; ++e) { red[e * 512 + threadIdx.x] = k[e]; red[e * 512 + 256 + threadIdx.x] = q[e]; }
         __syncthreads();
-        // channel sums over the row lanes: thread (channel of the tile)
-        for (int i = threadIdx.x; i < tw * V; i += 256) {
-            const int e = i / tw, tt = i - e * tw;
-            if (t0 + tt >= cv) continue;
-            float ss = 0.f, qq = 0.f;
-            for (int j = 0; j < nr; ++j) { ss += red[e * 512 + j * tw + tt]; qq += red[e * 512 + 256 + j * tw + tt]; }
-            const int cc = (t0 + tt) * V + e;
-            const float m = ss * rn;
-            cm[cc] = OpT<T>::to(x[(size_t)r0 * p.C + cc]) + m;
-            cq[cc] = qq - ss * m;
+        // a channel's row lanes: lane j has the rows j, j + nr, ...; P threads of a wave a channel
+        const int lanes = rows < nr ? rows : nr, full = rows / nr, more = rows - full * nr;   // the first `more` lanes have full + 1 rows
+        int P = 1;
+        while (P < 64 && 2 * P * tw * V <= 256) P <<= 1;
+        const int sub = (int)threadIdx.x & (P - 1);
+        for (int i0 = 0; i0 < tw * V; i0 += 256 / P) {
+            const int i = min(i0 + (int)threadIdx.x / P, tw * V - 1), e = i / tw, tt = i - e * tw;   // (threads behind the last channel do it once more)
+            const float *ml = red + e * 512 + tt, *ql = ml + 256;
+            const float o = ml[0];
+            float m = 0.f, m2 = 0.f;
+#pragma unroll 4
+            for (int j = sub; j < lanes; j += P) m = fmaf((float)(j < more ? full + 1 : full), ml[j * tw] - o, m);
+            for (int w = 1; w < P; w <<= 1) m += __shfl_xor(m, w, 64);
+            m = fmaf(m, rn, o);
+#pragma unroll 4
+            for (int j = sub; j < lanes; j += P) { const float d = ml[j * tw] - m; m2 += fmaf((float)(j < more ? full + 1 : full) * d, d, ql[j * tw]); }
+            for (int w = 1; w < P; w <<= 1) m2 += __shfl_xor(m2, w, 64);
+            if (sub == 0 && t0 + tt < cv) { cm[(t0 + tt) * V + e] = m; cq[(t0 + tt) * V + e] = m2; }
         }
     }
     __syncthreads();
-    for (int g = threadIdx.x; g < p.G; g += 256) {   // the group's channels, all over the same n rows
+    for (int g = threadIdx.x; g < p.G; g += 256) {   // the group's channels, all over the same rows
+        const float *m_ = cm + g * p.cg, *q_ = cq + g * p.cg, o = m_[0];
         float m = 0.f, m2 = 0.f;
-        for (int c = g * p.cg; c < (g + 1) * p.cg; ++c) m += cm[c];
-        m /= (float)p.cg;
-        for (int c = g * p.cg; c < (g + 1) * p.cg; ++c) { const float d = cm[c] - m; m2 += cq[c] + n * d * d; }
+        for (int c = 0; c < p.cg; ++c) m += m_[c] - o;
+        m = o + m / (float)p.cg;
+        for (int c = 0; c < p.cg; ++c) { const float d = m_[c] - m; m2 += fmaf(n * d, d, q_[c]); }
         *reinterpret_cast<float2*>(p.part + (((size_t)b * p.nch + ch) * p.G + g) * 2) = make_float2(m, m2);
     }
 }
@@ -139,24 +173,42 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs p) {
     GN_COLS(V, true)
     {
         GN_LANES
-        const float cgf = (float)p.cg, N = (float)p.HW * cgf;
+        const float cgf = (float)p.cg, N = (float)p.HW * cgf, full = (float)p.rows * cgf, last = (float)(p.HW - (p.nch - 1) * p.rows) * cgf;
         for (int g0 = 0; g0 < p.G; g0 += gs) {
             const int g = g0 + (int)threadIdx.x / L;
-            float m0 = 0.f, s = 0.f, q = 0.f;
-            if (g < p.G) {
-                const float2* src = reinterpret_cast<const float2*>(p.part) + (size_t)b * p.nch * p.G + g;
-                m0 = src[0].x;   // the first chunk's mean as the origin of the sums
-                for (int i = gl; i < p.nch; i += L) {
-                    const float2 a = src[(size_t)i * p.G];
-                    const long long ra = i * p.rows, rb = ra + p.rows < p.HW ? ra + p.rows : p.HW;
-                    const float nn = (float)(rb - ra) * cgf, d = a.x - m0;
-                    s = fmaf(nn, d, s);
-                    q += fmaf(nn * d, d, a.y);
-                }
+            // the mean around the first chunk's, then the squared deviations around the mean; four chunks in flight, the first four kept
+            const float2* src = reinterpret_cast<const float2*>(p.part) + (size_t)b * p.nch * p.G + (g < p.G ? g : 0);
+            const float m0 = src[0].x;
+            float2 a[4];
+            auto load = [&](int i0) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) a[k] = src[(size_t)min(i0 + k * L, p.nch - 1) * p.G];
+            };
+            auto values = [&](int i) { return i < p.nch - 1 ? full : i == p.nch - 1 ? last : 0.f; };   // in chunk i; one that is not there has none
+            float s = 0.f, q = 0.f;
+            load(gl);
+            float2 first[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) first[k] = a[k];
+            for (int i = gl;;) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s = fmaf(values(i + k * L), a[k].x - m0, s);
+                if ((i += 4 * L) >= p.nch) break;
+                load(i);
             }
-            for (int o = 1; o < L; o <<= 1) { s += __shfl_xor(s, o, 64); q += __shfl_xor(q, o, 64); }
+            for (int o = 1; o < L; o <<= 1) s += __shfl_xor(s, o, 64);
+            const float m = m0 + s / N;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a[k] = first[k];
+            for (int i = gl;;) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { const float d = a[k].x - m, v = values(i + k * L); q += fmaf(v * d, d, v > 0.f ? a[k].y : 0.f); }
+                if ((i += 4 * L) >= p.nch) break;
+                load(i);
+            }
+            for (int o = 1; o < L; o <<= 1) q += __shfl_xor(q, o, 64);
             if (g < p.G && gl == 0) {
-                const float dm = s / N, m = m0 + dm, m2 = q - s * dm, rs = 1.f / sqrtf((m2 < 0.f ? 0.f : m2) / N + p.eps);   // (a NaN stays one)
+                const float rs = 1.f / sqrtf((q < 0.f ? 0.f : q) / N + p.eps);   // (a NaN stays one)
                 gm[g] = m; gr[g] = rs;
                 if (ch == 0) { p.mean[(size_t)b * p.G + g] = m; p.rstd[(size_t)b * p.G + g] = rs; }
             }

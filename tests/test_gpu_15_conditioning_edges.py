@@ -5,6 +5,8 @@ import math
 import pytest
 import torch
 
+from tests import conditioning_ref as R
+
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 F32, BF16 = torch.float32, torch.bfloat16
@@ -44,6 +46,35 @@ def test_group_norm_of_a_value_that_is_not_finite(B, hw, C, G, dtype, act, at, b
         assert got[where].isnan().all(), what
         assert torch.equal(got[~where], clean[~where]), what
     assert torch.equal(runs[1][3][~channel], runs[0][3][~channel])
+
+
+def _check_statistics(x, G, what):
+    """Group norm alone: a mean off by r standard deviations and by roundings of its own size, a standard deviation off by r of itself, where r is what n
+    values add up to around a mean of their own: 8 sqrt(n) + 64 roundings."""
+    from layout2img_amd import ops
+    y = ops.group_norm_act(x, G, op_dtype=F32)
+    B, C = x.shape[0], x.shape[-1]
+    xd = x.double().reshape(B, -1, G, C // G)
+    n = xd.shape[1] * xd.shape[3]
+    m = xd.mean((1, 3), keepdim=True)
+    rs = ((xd - m).pow(2).mean((1, 3), keepdim=True) + 1e-5).rsqrt()
+    xh = (xd - m) * rs
+    r = (8 * math.sqrt(n) + 64) * R.U32
+    R.close(y, xh.reshape(x.shape), (r * (1 + xh.abs()) + R.U32 * m.abs() * rs).reshape(x.shape), what)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,hw,C,G", [(2, (64, 64), 8, 4), (600, (64, 64), 4, 1), (2, (96, 50), 25, 5), (1, (256, 256), 8, 1), (1, (300, 200), 32, 4), (2, (40, 40), 24, 3)])
+def test_group_norm_of_a_border_far_from_the_rest(B, hw, C, G, dtype):
+    """One pixel, a column or rows hundreds of deviations away from the others, wherever the kernel starts to count from them."""
+    gen = _gen(7)
+    x = _rnd(gen, B, *hw, C)
+    for name, where in (("first pixel", (slice(None), 0, 0)), ("last pixel", (slice(None), -1, -1)), ("left column", (slice(None), slice(None), 0)),
+                        ("right column", (slice(None), slice(None), -1)), ("first row", (slice(None), 0)), ("a channel", (Ellipsis, 0))):
+        far = x.clone()
+        far[where] += 300.0
+        _check_statistics(far.to(dtype), G, name)
+        _check_statistics((-far).to(dtype), G, name)
 
 
 # ------------------------------------------------------------------------------------------------ cross attention
