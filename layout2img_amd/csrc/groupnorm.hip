@@ -7,7 +7,8 @@
 //
 // Bound by bytes. Two forms:
 //   resident: a workgroup holds all pixels of a slab of whole groups (at least 64 contiguous bytes a pixel) in registers: one launch, every
-//     value read once; used where a slab is at most 4096 values (8192 in bf16: maps up to 16 x 16 of the wide layers).
+//     value read once; used where a slab is at most 4096 values (8192 in bf16: maps up to 16 x 16 of the wide layers). A group's mean is summed around
+//     its first value, the squared deviations around the mean.
 //   split: the map is cut in NCH chunks of rows (pixels) per image. The first launch leaves every chunk's moments (mean and sum of squared
 //     deviations per group, counted from origins that follow the values: neither a mean far from zero nor single values far from the rest cost digits), the
 //     second joins them in a fixed order and writes the result, reading the map a second time -- from the chunk that was read last backwards, on the
@@ -369,18 +370,18 @@ __global__ __launch_bounds__(256) void gn_res_kernel(GnArgs p) {
     float *red = sm, *chan = sm + p.nr * p.Cs, *gres = chan + p.Cs;
     GN_RES(V)
     const TI* x = reinterpret_cast<const TI*>(p.x) + base;
+    const TI* origin = reinterpret_cast<const TI*>(p.x) + (size_t)b * p.HW * p.C;   // a group's first value of the first pixel: what its sum is counted from
     Vec<TI, V> a[R];
-    float s[V], v[V];
+    float s[V], v[V], k[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) s[e] = 0.f;
+    for (int j = 0; j < R; ++j) if (on && ty + j * p.nr < p.HW) a[j].load(x + j * step);
+    gn_each<V>(on ? c : c0, p.cg, [&](int e, int, int g) { k[e] = OpT<TI>::to(origin[g * p.cg]); s[e] = 0.f; });
 #pragma unroll
-    for (int k = 0; k < R; ++k) if (on && ty + k * p.nr < p.HW) a[k].load(x + k * step);
+    for (int j = 0; j < R; ++j)
+        if (on && ty + j * p.nr < p.HW) {
+            a[j].get(v);
 #pragma unroll
-    for (int k = 0; k < R; ++k)
-        if (on && ty + k * p.nr < p.HW) {
-            a[k].get(v);
-#pragma unroll
-            for (int e = 0; e < V; ++e) s[e] += v[e];
+            for (int e = 0; e < V; ++e) s[e] += v[e] - k[e];
         }
     const float rn = 1.f / ((float)p.HW * (float)p.cg);
     gn_channel_sums<V>(p, cs, tx, ty, on, s, red, chan);
@@ -388,7 +389,7 @@ __global__ __launch_bounds__(256) void gn_res_kernel(GnArgs p) {
         float t = 0.f;
         for (int i = lane; i < p.cg; i += 64) t += chan[g * p.cg + i];
         t = wave_sum(t);
-        if (lane == 0) gres[g] = t * rn;
+        if (lane == 0) gres[g] = fmaf(t, rn, OpT<TI>::to(origin[(g0 + g) * p.cg]));
     }
     __syncthreads();
     float m[V], r[V];

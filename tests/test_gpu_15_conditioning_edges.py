@@ -64,7 +64,8 @@ def _check_statistics(x, G, what):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("B,hw,C,G", [(2, (64, 64), 8, 4), (600, (64, 64), 4, 1), (2, (96, 50), 25, 5), (1, (256, 256), 8, 1), (1, (300, 200), 32, 4), (2, (40, 40), 24, 3)])
+@pytest.mark.parametrize("B,hw,C,G", [(2, (64, 64), 8, 4), (600, (64, 64), 4, 1), (2, (96, 50), 25, 5), (1, (256, 256), 8, 1), (1, (300, 200), 32, 4), (2, (40, 40), 24, 3),
+                                       (32, (4, 4), 1024, 32), (4, (12, 12), 512, 32), (3, (16, 16), 96, 3)])
 def test_group_norm_of_a_border_far_from_the_rest(B, hw, C, G, dtype):
     """One pixel, a column or rows hundreds of deviations away from the others, wherever the kernel starts to count from them."""
     gen = _gen(7)
@@ -75,6 +76,14 @@ def test_group_norm_of_a_border_far_from_the_rest(B, hw, C, G, dtype):
         far[where] += 300.0
         _check_statistics(far.to(dtype), G, name)
         _check_statistics((-far).to(dtype), G, name)
+
+
+@pytest.mark.parametrize("mean", [3.0, 1000.0, -30000.0])
+@pytest.mark.parametrize("B,hw,C,G", [(32, (4, 4), 1024, 32), (8, (12, 12), 512, 32), (64, (8, 8), 64, 8), (4, (40, 40), 24, 3), (2, (9, 9), 4096, 1), (1, (128, 128), 16, 16)])
+def test_group_norm_of_a_mean_far_from_zero(B, hw, C, G, mean):
+    """A mean up to 30000 deviations away, in both forms: it is held in f32, and that rounding is all that it costs."""
+    gen = _gen(9)
+    _check_statistics(_rnd(gen, B, *hw, C) + mean, G, "y")
 
 
 # ------------------------------------------------------------------------------------------------ cross attention
