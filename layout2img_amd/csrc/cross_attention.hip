@@ -214,6 +214,7 @@ template <typename T, int CH, int NR, int TH> struct XaDma {
         for (int i = 0; i < N; ++i) off[i] = chunk(i) * 16 < D * (int)sizeof(T) ? (unsigned)(row(i) * stride * (int)sizeof(T)) + chunk(i) * 16 : XA_OOB;
     }
     template <typename F> __device__ __forceinline__ void issue(const T* base, unsigned lds, F rows) const {   // base, lds: the same for all lanes
+        if constexpr (TH == 64) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // a wave refills a tile of its own behind no barrier: its reads of it are done
         const u32x4_t r = make_rsrc(base, XA_SPAN);
         const unsigned at = lds + (TH == 64 ? 0 : (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024));
 #pragma unroll
