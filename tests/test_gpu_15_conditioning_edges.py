@@ -86,6 +86,24 @@ def test_group_norm_of_a_mean_far_from_zero(B, hw, C, G, mean):
     _check_statistics(_rnd(gen, B, *hw, C) + mean, G, "y")
 
 
+def test_group_norm_of_a_map_past_32_bits_against_64_bits():
+    """More values than 2^31: the last, the first and a middle group of every image, and their channels' gradients, against a map of those channels alone."""
+    from layout2img_amd import ops
+    gen = _gen(12)
+    B, hw, C, G = 3, (700, 1024), 1024, 256
+    x, dy = (torch.randn(B, *hw, C, generator=gen, device=DEV, dtype=BF16) for _ in range(2))
+    assert x.numel() > 1 << 31
+    w, b = 1 + 0.2 * _rnd(gen, C), 0.2 * _rnd(gen, C)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = ops.group_norm_act(*leaves[:1], G, *leaves[1:], act="silu")
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    for g in (0, 130, G - 1):
+        ch = slice(g * (C // G), (g + 1) * (C // G))
+        want, tol = R.group_norm_act(x[..., ch], 1, w[ch], b[ch], 1e-5, "silu", BF16, dy[..., ch])
+        for got, ref, t, what in zip((y[..., ch], dx[..., ch], dw[ch], db[ch]), want, tol, ("y", "dx", "dw", "db")):
+            R.close(got, ref, t, (g, what))
+
+
 # ------------------------------------------------------------------------------------------------ cross attention
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("D", [40, 64, 72, 128])
