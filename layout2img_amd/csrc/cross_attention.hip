@@ -313,10 +313,12 @@ template <typename T> __device__ __forceinline__ void xa_put(T* row, const f32x1
     }
 }
 #define XA_NINF 0xff800000u
-// log2 of a row's denominator l over the reference m, and 1 / l: +inf and 0 for a row without a live key (l = 0). A denominator that is not a number (a key or
-// a query is not) stays one, so that the backward pass does not take the row for one that sees nothing.
-__device__ __forceinline__ float xa_lse(float m, float l) { return l == 0.f ? INFINITY : m + log2f(l); }
-__device__ __forceinline__ float xa_inv(float l) { return l == 0.f ? 0.f : 1.f / l; }
+// log2 of a row's denominator l over the reference m, and 1 / l: +inf and 0 for a row without a live key (l = 0 and no maximum). Any other denominator that is no
+// use shows: one that is not a number (a key or a query is not) stays so, so that the backward pass does not take the row for one that sees nothing, and
+// one that vanished or overflowed beside a finite maximum (scores beyond 2^30, whose roundings in f32 pass the exponent's range) gives NaN, not zeros.
+__device__ __forceinline__ bool xa_no_key(float m, float l) { return l == 0.f && m == -INFINITY; }
+__device__ __forceinline__ float xa_lse(float m, float l) { return xa_no_key(m, l) ? INFINITY : l > 0.f && l < INFINITY ? m + log2f(l) : NAN; }
+__device__ __forceinline__ float xa_inv(float m, float l) { return xa_no_key(m, l) ? 0.f : 1.f / l; }
 // Between a matrix instruction and the first read of its result no branch may join: the compiler's wait count there follows one of the joining
 // paths only. Live bits are therefore made in front of the products, masked and unmasked tiles are separate straight bodies, and behind a
 // loop of products this wait stands.
@@ -520,7 +522,7 @@ __global__ __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : (sizeof
             }
         return;
     }
-    const float inv = xa_inv(l);
+    const float inv = xa_inv(m, l);
     if (p.lse && h == 0 && (WQ == 4 || wave == 0)) p.lse[row] = xa_lse(m, l);
     const size_t o = (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D;
 #pragma unroll
@@ -577,7 +579,7 @@ __global__ __launch_bounds__(256) void xa_join_kernel(XaArgs p) {
             o[0] += a.x; o[1] += a.y; o[2] += a.z; o[3] += a.w;
         }
     }
-    const float inv = xa_inv(l);
+    const float inv = xa_inv(mn, l);
     if (p.lse && d == 0) p.lse[row] = xa_lse(mn, l);
     if (d >= p.D) return;
 #pragma unroll
@@ -986,7 +988,7 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 2 : 4) void xa_s
 #pragma unroll
             for (int e = 0; e < 16; ++e) oacc[d][e] = 0.f;
         xa_tdot<CH, ND>(oacc, vs, ad, sc);
-        const float inv = xa_inv(l);
+        const float inv = xa_inv(m, l);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -994,7 +996,7 @@ __global__ __launch_bounds__(256, DP == 128 || sizeof(T) == 4 ? 2 : 4) void xa_s
         const int r = blk * 32 + (lane & 31);
         if (r < p.R) {
             const int iq = xa_row_query(p, r), head = hk * p.G + r - iq * p.G;
-            if (p.lse && h == 0) p.lse[(size_t)bh * p.R + r] = xa_lse(ref, l);
+            if (p.lse && h == 0) p.lse[(size_t)bh * p.R + r] = xa_lse(m == -INFINITY ? m : ref, l);
             T* o = reinterpret_cast<T*>(p.o) + (((size_t)b * p.Lq + iq) * (p.Hk * p.G) + head) * p.D;
 #pragma unroll
             for (int d = 0; d < ND; ++d) xa_put<T>(o, oacc[d], 1.f, d * 32, p.D);

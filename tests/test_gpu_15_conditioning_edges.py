@@ -154,3 +154,24 @@ def test_cross_attention_of_a_state_that_is_not_finite(Lq, Lk, D, dtype, bad):
                 assert got[0].isnan().all(), what
             else:
                 assert got[0, live].isnan().all() and not got[0, Lk - 3:].any(), what
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Lq,Lk", [(1, 20), (60, 20), (1, 300), (60, 50), (200, 300), (1, 5000)])
+def test_cross_attention_of_scores_past_the_exponents_range(Lq, Lk, dtype):
+    """Scores of 10^12 and more, whose f32 roundings alone are more than an exponent holds: a row is the state of its largest score, or not a number, and never zeros."""
+    from layout2img_amd import ops
+    gen = _gen(Lq + Lk)
+    q, k, g = (_rnd(gen, 2, n, 1, 64, scale=1e6).to(dtype) for n in (Lq, Lk, Lq))
+    v = (1 + torch.rand(2, Lk, 1, 64, generator=gen, device=DEV)).to(dtype)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    y = ops.cross_attention(*leaves)
+    top = (q.detach().double()[:, :, 0] @ k.detach().double()[:, :, 0].transpose(1, 2)).argmax(2)
+    want = torch.stack([v[b, top[b]] for b in range(2)])
+    ok = y.isnan().all(3, keepdim=True) | (y - want).abs().le(2 * R.u(dtype) * want.abs()).all(3, keepdim=True)
+    assert ok.all()
+    lost = y.isnan().all(3)[..., 0]
+    dq, dk, dv = torch.autograd.grad(y, leaves, g)
+    for b in range(2):
+        if lost[b].any():
+            assert dq[b, lost[b]].isnan().all() and dk[b].isnan().any() and dv[b].isnan().any()
