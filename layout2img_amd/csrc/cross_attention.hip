@@ -12,7 +12,7 @@
 // and sum are in-lane plus one exchange between the wave's halves, and the accumulator's registers ARE the B operand of P V with no
 // movement, because the sum over keys may run in any order as long as V is read in the same one: bf16 V^T comes from LDS by
 // the transposing read (ds_read_b64_tr_b16), f32 V by plain reads. Probabilities enter P V (and dS the gradient products) rounded to bf16 in
-// the bf16 kernels (relative 2^-9, as small as the rounding of the inputs); maxima, sums, S, D and all accumulators are f32.
+// the bf16 kernels (relative 2^-8, as small as the rounding of the inputs); maxima, sums, S, D and all accumulators are f32.
 //
 // What bounds it: with 64 values a head, a wave's 32 x 64 scores cost 16 MFMAs (512 cycles) and 32 exponentials a lane with what surrounds
 // them (about 900 cycles), so the vector unit; tiles therefore come to LDS by LDS-DMA (no registers, no instructions of the waves), two
@@ -28,7 +28,7 @@ typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 
 struct XaArgs {
     const void *q, *k, *v; void* o;          // o, g, dq: [B][Lq][H][D]; dk, dv: [B][Lk][Hk][D]
-    bf16_t* lo;                               // what rounding o to bf16 left, or null: D = g . (o + lo) is exact to f32 then (o alone: relative 2^-9 of |g| |o|,
+    bf16_t* lo;                               // what rounding o to bf16 left, or null: D = g . (o + lo) is off by 2^-16 of |g| |o| then (o alone: by 2^-8,
                                               // which where few keys share the weight is more than the rounding of dS itself)
     const void* g; void *dq, *dk, *dv;
     float* lse;                               // [B Hk][R] log2 of the softmax's denominator; +inf for a row without a live key
@@ -919,7 +919,7 @@ __global__ __launch_bounds__(256) void xa_fold_kernel(XaArgs p) {
 }
 
 // ------------------------------------------------------------------------------------------------ states that fit one tile
-// 32 images of 4096 queries over 31 states of 4 x 32 with a mask, bf16: forward 24 us (71 MB), backward 34 (105 MB) and 4 for the fold.
+// 32 images of 4096 queries over 31 states of 4 x 32 with a mask a query, bf16: forward 22 us (71 MB), backward 30 (105 MB) and 4 for the fold.
 // At most 32 states (a layout's objects): K and V stand in LDS for a whole workgroup, whose waves each walk row blocks of 32 on their own, with no
 // barrier. Bound by bytes: q and out forward; q, g and dq backward -- S, P and D = sum_j P_ij (g_i . v_j) are made from them in registers, so
 // that one launch gives dq and (through a transpose of P and dS in LDS) its rows' share of dk and dv.
@@ -1169,9 +1169,10 @@ static XaPlan xa_plan(int B, long long R, int Lk, int Hk, int D, int dtype) {
     const bool f32 = !dtype;
     const long long bh = (long long)B * Hk, groups = (R + 127) / 128;   // a workgroup's four waves take at least a block of 32 rows each
     q.nwf = q.nwb = 0;
-    // the one-tile form, forward and forward with backward, against the general one: 32 images of 4096 queries over 31 states of 4 x 32 bf16 17 and 47 us, not 25
-    // and 104; of 4 x 64 f32 75 and 242, not 109 and 548; one query of 8 x 64 bf16 5 and 12, not 7 and 17. Workgroups: 1024 and 512 in all (2048 and 1024: 18 and 51,
-    // 4096 each: 23 and 73): staging the states and joining the shares of dk and dv are paid less often
+    // the one-tile form, forward and forward with backward, against the general one: 32 images of 4096 queries over 31 states of 4 x 32 bf16 17 and 42 us, not 25
+    // and 100 (with a mask a query 22 and 54, not 37 and 135); of 4 x 64 f32 73 and 245, not 109 and 488; one query of 8 x 64 bf16 5 and 12, not 6 and 16.
+    // Workgroups: 1024 and 512 in all (2048 and 1024: 18 and 51 where these took 17 and 47, 4096 each: 23 and 73): staging the states and joining the shares of dk
+    // and dv are paid less often
     if (Lk <= 32 && xa_short_fits(dp, dtype)) {
         q.nwf = (int)std::min(groups, std::max(1LL, (1024 + bh - 1) / bh));
         q.nwb = (int)std::min(groups, std::max(1LL, (512 + bh - 1) / bh));

@@ -2257,7 +2257,8 @@ def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
     A query that sees no state gives zeros. What `lengths` or a mask row shared by all queries takes out is not read, whatever it holds; a state
     that only some queries see has to be finite. The D values of a head are consecutive; the other strides may be any of whole 16 bytes (slices of
     a grouped projection, transposed heads, expanded batches), less than 2^22 values from position to position. Where a gradient is wanted, the
-    result's queries lie less than 2^31 bytes apart over min(Lq - 1, 1 + 62 // (H // Hk)) steps of H * D values, and one group of heads beside them."""
+    result's queries lie less than 2^31 bytes apart over min(Lq - 1, 1 + 62 // (H // Hk)) steps of H * D values, and one group of heads beside them.
+    A score is held in 32 bits: a weight is off by 2^-24 of it relative to itself, and a row whose scores pass 2^30 is NaN."""
     dtype = _op(q, "cross_attention: q").dtype
     if _op(k, "cross_attention: k").dtype is not dtype or _op(v, "cross_attention: v").dtype is not dtype:
         raise RuntimeError(f"cross_attention: q, k, v have one type, got {dtype}, {k.dtype} and {v.dtype}")
